@@ -365,6 +365,71 @@ int usaf_build_ov_cbptr(const int32_t *row_ptr, const int32_t *col, int32_t E, i
                         int32_t *out, void *stream);
 const char *usaf_version(void);
 
+/* ---- dense parameters around the experts -----------------------------------
+ * No counterparts in the reference, which trains the experts and the routers
+ * only: the operators that give a model's norms and embedding their forward
+ * and gradients, and the step over those tensors.  Rows are contiguous values
+ * at a stride of ld* elements; outputs are dense.
+ *
+ * usaf_rms_norm_fwd: s = x, or s = dtype(x + res) written to sum (res and sum
+ * go together); r = 1/sqrt(mean(s^2) + eps); y = dtype(s r w).  w has the
+ * rows' dtype or fp32.  rstd: fp32 [rows] for the backward pass, or NULL.
+ * usaf_rms_norm_bwd: x is the normed row (s of the forward); dx =
+ * dtype(r (g - s r mean(g s r)) + dsum), g = dy w, dsum the gradient of s as
+ * an output of its own (or NULL); dw [H] = sum over rows of dy s r in a fixed
+ * order, or NULL.  ws: usaf_rms_norm_workspace_bytes(rows, H) bytes when dw is
+ * given.  H <= 32768 (USAF_EUNSUPPORTED above). */
+int64_t usaf_rms_norm_workspace_bytes(int64_t rows, int32_t H);
+int usaf_rms_norm_fwd(const void *x, int64_t ldx, const void *res, int64_t ldr, const void *w,
+                      int32_t dtype, int32_t w_dtype, int64_t rows, int32_t H, double eps,
+                      void *sum, void *y, float *rstd, void *stream);
+int usaf_rms_norm_bwd(const void *dy, int64_t lddy, const void *x, int64_t ldx, const void *w,
+                      const float *rstd, const void *dsum, int64_t ldds, int32_t dtype,
+                      int32_t w_dtype, int64_t rows, int32_t H, void *dx, void *dw, void *ws,
+                      void *stream);
+
+/* usaf_embedding_fwd: out[t] = dtype(scale * table[ids[t]]), table [V, H],
+ * ids int32 or int64 (ids_bits).  A token outside [0, V) gives a row of zeros
+ * and sets USAF_ERR_BAD_INDEX in *err (err may be NULL).
+ * usaf_embedding_bwd: grad [V, H] (dy's dtype or fp32) = scale * the sum of
+ * dy[t] over the tokens t of each row, in fp32 and ascending t, rounded once;
+ * rows without tokens become 0, or with accumulate keep their values and the
+ * sum is added to the others'.  Tokens equal to padding_idx (< 0: none) are
+ * left out, tokens outside [0, V) too (USAF_ERR_BAD_INDEX).  ws:
+ * usaf_embedding_workspace_bytes(tokens, V, H) bytes. */
+int usaf_embedding_fwd(const void *ids, int32_t ids_bits, int64_t tokens, const void *table,
+                       int32_t dtype, int64_t V, int32_t H, double scale, void *out, int32_t *err,
+                       void *stream);
+int64_t usaf_embedding_workspace_bytes(int64_t tokens, int64_t V, int32_t H);
+int usaf_embedding_bwd(const void *dy, const void *ids, int32_t ids_bits, int64_t tokens,
+                       int32_t dtype, int64_t V, int32_t H, double scale, int64_t padding_idx,
+                       int32_t accumulate, void *grad, int32_t grad_dtype, void *ws, int32_t *err,
+                       void *stream);
+
+/* usaf_adamw: one AdamW step (decoupled weight decay) over n_tensors tensors
+ * of one dtype, gradients of the same dtype or fp32:
+ *   g = grad / grad_div; m = b1 m + (1-b1) g; v = b2 v + (1-b2) g^2;
+ *   p = p (1 - lr wd) - lr/(1-b1^step) * m / (sqrt(v)/sqrt(1-b2^step) + eps)
+ * `tensors` is a HOST array, read before the call returns.  m, v (and master,
+ * the fp32 weights that p is rounded from, or NULL) are flat buffers that all
+ * tensors share; tensor i takes numel values from `start`, a multiple of 256.
+ * bits 32: m, v fp32.  bits 8: m and sqrt(v) as e4m3 bytes, each group of 256
+ * values times m_scale / v_scale [values / 256] (fp32; the group's largest
+ * magnitude / 448, 0 for a group below 1e-30); a sqrt(v) above zero is stored
+ * as the lowest code at least.  The values between a tensor's end and the next
+ * multiple of 256 stay what they are in 32 bits and are written as zeros in 8. */
+typedef struct {
+    void *p;
+    const void *g;
+    int64_t numel;
+    int64_t start;
+    double weight_decay;
+} usaf_adamw_tensor;
+int usaf_adamw(const usaf_adamw_tensor *tensors, int32_t n_tensors, int32_t p_dtype,
+               int32_t g_dtype, float *master, int32_t bits, void *m, void *v, float *m_scale,
+               float *v_scale, double grad_div, int32_t step, double lr, double beta1,
+               double beta2, double eps, void *stream);
+
 /* ---- expert parallelism ------------------------------------------------------
  * No counterpart in the reference (it runs in a single process).  Plan:
  * rank r of W owns experts [r*El, (r+1)*El), tokens stay data-parallel and an

@@ -77,6 +77,13 @@ _SIGS = {
     "usaf_dot": (I32, [P, P, I32, I64, P, P]),
     "usaf_build_rowptr": (I32, [P, I64, I64, P, P]),
     "usaf_build_ov_cbptr": (I32, [P, P, I32, I32, I32, P, P]),
+    "usaf_rms_norm_workspace_bytes": (I64, [I64, I32]),
+    "usaf_rms_norm_fwd": (I32, [P, I64, P, I64, P, I32, I32, I64, I32, F64, P, P, P, P]),
+    "usaf_rms_norm_bwd": (I32, [P, I64, P, I64, P, P, P, I64, I32, I32, I64, I32, P, P, P, P]),
+    "usaf_embedding_fwd": (I32, [P, I32, I64, P, I32, I64, I32, F64, P, P, P]),
+    "usaf_embedding_workspace_bytes": (I64, [I64, I64, I32]),
+    "usaf_embedding_bwd": (I32, [P, P, I32, I64, I32, I64, I32, F64, I64, I32, P, I32, P, P, P]),
+    "usaf_adamw": (I32, [P, I32, I32, I32, P, I32, P, P, P, P, F64, I32, F64, F64, F64, F64, P]),
     "usaf_version": (C.c_char_p, []),
 }
 
@@ -106,6 +113,16 @@ def call(name: str, *args):
     rc = getattr(LIB, name)(*args)
     if rc != 0:
         raise UsafError(f"{name} failed: {_STATUS.get(rc, rc)} (status {rc})")
+
+
+def call_on(device: torch.device, name: str, *args):
+    """:func:`call` on the current stream of ``device`` (appended as the last
+    argument), whichever device is current."""
+    if device.index == torch.cuda.current_device():
+        call(name, *args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, torch.cuda.current_stream().cuda_stream)
 
 
 def dtype_code(dt: torch.dtype) -> int:

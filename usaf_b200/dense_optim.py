@@ -1,0 +1,278 @@
+"""AdamW over many tensors at once, states in 32 or 8 bits, on the device.
+
+Beside :class:`usaf_b200.sparse_optim.SparseAdam`, which steps the selected
+coordinates of the experts: :class:`AdamW` steps whole tensors (norms,
+embedding, routers) with decoupled weight decay, all of them in one launch per
+parameter type.  :func:`adamw_step` is the step itself over tensors and state
+buffers that the caller keeps.
+
+States lie in flat buffers shared by the tensors, each tensor from a multiple
+of 256 values on (:func:`state_layout`).  With 8-bit states the first moment m
+and the root of the second, sqrt(v), are e4m3 values times one fp32 scale per
+256 values: 2.03 bytes a value instead of 8.  Every operation of the step is
+rounded by itself in fp32, in a fixed order.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Dict, Iterable, List, Optional, Sequence, Tuple, Union
+
+import numpy as np
+import torch
+
+from . import _lib
+from ._lib import call_on, ptr
+
+BLOCK = 256
+
+_TENSOR = np.dtype([("p", np.uint64), ("g", np.uint64), ("numel", np.int64), ("start", np.int64),
+                    ("weight_decay", np.float64)])
+
+Packed = Tuple[torch.Tensor, torch.Tensor]
+
+
+def state_layout(numels: Iterable[int]) -> Tuple[List[int], int]:
+    """Where the states of tensors of these sizes start, and the size of the
+    flat buffers that hold them."""
+    starts, at = [], 0
+    for n in numels:
+        starts.append(at)
+        at += -(-int(n) // BLOCK) * BLOCK
+    return starts, at
+
+
+def _check_flat(name: str, t: torch.Tensor, n: int, dtype: torch.dtype, device: torch.device) -> None:
+    if t.numel() != n or t.dtype != dtype or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name}: expected {n} contiguous {dtype} values on {device}, got {t.numel()} {t.dtype} "
+                         f"on {t.device}")
+
+
+def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m: Union[torch.Tensor, Packed],
+               v: Union[torch.Tensor, Packed], *, step: int, lr: float, betas: Tuple[float, float] = (0.9, 0.999),
+               eps: float = 1e-8, weight_decay: Union[float, Sequence[float]] = 0.0,
+               masters: Optional[torch.Tensor] = None, grad_div: float = 1.0,
+               starts: Optional[Sequence[int]] = None) -> None:
+    """One AdamW step in place over ``params`` (one type, contiguous) with
+    ``grads`` (the parameters' type or fp32).
+
+    ``m`` and ``v`` are flat fp32 buffers in :func:`state_layout`'s order, or
+    for states in 8 bits the pairs ``(values, scales)`` of flat float8_e4m3fn
+    values (of m and of sqrt(v)) and one fp32 scale per 256 of them.
+    ``masters``: flat fp32 weights that the step updates and ``params`` are
+    rounded from.  ``weight_decay``: one value, or one for each tensor.
+    ``grad_div`` divides the gradients first.  ``starts`` gives the tensors'
+    places when they are not all that the buffers hold."""
+    params, grads = list(params), list(grads)
+    n = len(params)
+    if len(grads) != n:
+        raise ValueError(f"{len(grads)} gradients for {n} parameters")
+    if step < 1:
+        raise ValueError(f"step: expected >= 1, got {step}")
+    if grad_div == 0:
+        raise ValueError("grad_div must not be 0")
+    eight = not isinstance(m, torch.Tensor)
+    if eight == isinstance(v, torch.Tensor):
+        raise TypeError("m and v: both flat tensors, or both (values, scales) pairs")
+    if n == 0:
+        return
+    dev, dtype, g_dtype = params[0].device, params[0].dtype, grads[0].dtype
+    if g_dtype not in (dtype, torch.float32):
+        raise TypeError(f"gradients: expected {dtype} or torch.float32, got {g_dtype}")
+    tab = np.zeros(n, dtype=_TENSOR)
+    numels = [p.numel() for p in params]
+    for i, (p, g) in enumerate(zip(params, grads)):
+        if p.dtype != dtype or g.dtype != g_dtype:
+            raise TypeError(f"tensor {i}: {p.dtype} with a gradient of {g.dtype}, the first has {dtype} and {g_dtype}")
+        if p.device != dev or g.device != dev:
+            raise ValueError(f"tensor {i}: expected on {dev}")
+        if g.shape != p.shape or not p.is_contiguous() or not g.is_contiguous():
+            raise ValueError(f"tensor {i}: the parameter and a gradient of its shape must be contiguous")
+    tab["p"] = [ptr(p) for p in params]
+    tab["g"] = [g.data_ptr() for g in grads]
+    tab["numel"] = numels
+    tab["weight_decay"] = weight_decay
+    by_address = tab[tab["numel"] > 0]
+    by_address = by_address[np.argsort(by_address["p"])]
+    ends = by_address["p"] + (by_address["numel"] * params[0].element_size()).astype(np.uint64)
+    if (ends[:-1] > by_address["p"][1:]).any():
+        raise ValueError("a parameter is listed twice, or two share memory")
+    if starts is None:
+        places, total = state_layout(numels)
+    else:
+        places = [int(a) for a in starts]
+        total = (m[0] if eight else m).numel()
+        order = sorted(range(n), key=places.__getitem__) if len(places) == n else []
+        ends = [-(-(places[i] + numels[i]) // BLOCK) * BLOCK for i in order]
+        if (not order or places[order[0]] < 0 or ends[-1] > total or any(a % BLOCK for a in places)
+                or any(e > places[i] for e, i in zip(ends, order[1:]))):
+            raise ValueError("starts: one multiple of 256 for each tensor, within the states, none overlapping")
+    tab["start"] = places
+    ms = vs = None
+    if eight:
+        (m, ms), (v, vs) = m, v
+        for nm, t, sc in (("m", m, ms), ("v", v, vs)):
+            _check_flat(nm, t, total, torch.float8_e4m3fn, dev)
+            _check_flat(f"{nm} scales", sc, total // BLOCK, torch.float32, dev)
+    else:
+        _check_flat("m", m, total, torch.float32, dev)
+        _check_flat("v", v, total, torch.float32, dev)
+    if masters is not None:
+        _check_flat("masters", masters, total, torch.float32, dev)
+    call_on(dev, "usaf_adamw", tab.ctypes.data_as(ctypes.c_void_p), n, _lib.dtype_code(dtype),
+            _lib.dtype_code(g_dtype), ptr(masters), 8 if eight else 32, ptr(m), ptr(v), ptr(ms), ptr(vs),
+            float(grad_div), int(step), float(lr), float(betas[0]), float(betas[1]), float(eps))
+
+
+class _Group:
+    """The tensors of one type and their flat states."""
+
+    def __init__(self, names: List[str], params: List[torch.Tensor], bits: int, masters: bool):
+        dev = params[0].device
+        self.names = names
+        self.starts, self.total = state_layout(p.numel() for p in params)
+        self.place = dict(zip(names, self.starts))
+        f32 = dict(dtype=torch.float32, device=dev)
+        if bits == 8:
+            self.m, self.v = ((torch.zeros(self.total, dtype=torch.float8_e4m3fn, device=dev),
+                               torch.zeros(self.total // BLOCK, **f32)) for _ in range(2))
+        else:
+            self.m, self.v = torch.zeros(self.total, **f32), torch.zeros(self.total, **f32)
+        self.masters = torch.zeros(self.total, **f32) if masters else None
+
+    def parts(self, name: str, numel: int) -> Dict[str, torch.Tensor]:
+        """Views of one tensor's states in the flat buffers."""
+        a = self.place[name]
+        b = slice(a // BLOCK, a // BLOCK + -(-numel // BLOCK))
+        out = {}
+        for k, t in (("m", self.m), ("v", self.v)):
+            if isinstance(t, tuple):
+                out[k], out[f"{k}_scale"] = t[0][a:a + numel], t[1][b]
+            else:
+                out[k] = t[a:a + numel]
+        if self.masters is not None:
+            out["master"] = self.masters[a:a + numel]
+        return out
+
+
+class AdamW:
+    """AdamW over named tensors; the step of one call covers all of them.
+
+    ``state_bits``: 32, or 8 for m and sqrt(v) as e4m3 values with block
+    scales.  ``master_weights``: fp32 copies of 16-bit parameters, from which
+    they are rounded after each step (default: for every parameter that is
+    not fp32).  ``no_decay``: names that ``weight_decay`` leaves alone."""
+
+    def __init__(self, named_params: Dict[str, torch.nn.Parameter], lr: float = 1e-4, betas: tuple = (0.9, 0.999),
+                 eps: float = 1e-8, weight_decay: float = 0.01, no_decay: Iterable[str] = (), state_bits: int = 32,
+                 master_weights: bool = True):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        self.lr, self.betas, self.eps, self.weight_decay = lr, betas, eps, weight_decay
+        self.state_bits = state_bits
+        self._named = dict(named_params)
+        self.no_decay = frozenset(no_decay)
+        unknown = self.no_decay - self._named.keys()
+        if unknown:
+            raise ValueError(f"no_decay: no parameter named {sorted(unknown)}")
+        self._step = 0
+        by_type: Dict[tuple, List[str]] = {}
+        for name, p in self._named.items():
+            if not p.is_cuda:
+                raise TypeError("usaf_b200 AdamW keeps its state on the parameter's CUDA device")
+            _lib.dtype_code(p.dtype)
+            if not p.is_contiguous():
+                raise ValueError(f"{name}: must be contiguous")
+            by_type.setdefault((p.dtype, p.device), []).append(name)
+        self._groups = [_Group(names, [self._named[n] for n in names], state_bits,
+                               master_weights and dt != torch.float32) for (dt, _), names in by_type.items()]
+        self._group_of = {n: g for g in self._groups for n in g.names}
+        self.refresh_masters()
+
+    def refresh_masters(self) -> None:
+        """Take the masters from the parameters again (after loading weights)."""
+        for g in self._groups:
+            if g.masters is not None:
+                for name in g.names:
+                    p = self._named[name]
+                    g.parts(name, p.numel())["master"].copy_(p.detach().reshape(-1))
+
+    def zero_grad(self, set_to_none: bool = True):
+        for p in self._named.values():
+            if p.grad is not None:
+                if set_to_none:
+                    p.grad = None
+                else:
+                    p.grad.zero_()
+
+    def step(self, grads: Optional[Dict[str, torch.Tensor]] = None, grad_div: float = 1.0):
+        """One step with ``grads`` by name (default: the parameters' ``.grad``);
+        a parameter without a gradient stays as it is.  ``grad_div`` divides
+        the gradients first, as in :meth:`SparseAdam.step`."""
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW.step counts its steps on the host; a captured one would repeat the same step")
+        work = []
+        for g in self._groups:
+            by_type: Dict[torch.dtype, list] = {}
+            for name, start in zip(g.names, g.starts):
+                p = self._named[name]
+                d = p.grad if grads is None else grads.get(name)
+                if d is not None:
+                    by_type.setdefault(d.dtype, []).append(
+                        (p.detach(), d.detach().contiguous(), start,
+                         0.0 if name in self.no_decay else self.weight_decay))
+            work += [(g, *map(list, zip(*rows))) for rows in by_type.values()]
+        for g, params, ds, starts, decays in work:
+            adamw_step(params, ds, g.m, g.v, step=self._step + 1, lr=self.lr, betas=self.betas, eps=self.eps,
+                       weight_decay=decays, masters=g.masters, grad_div=grad_div, starts=starts)
+        self._step += 1
+
+    def state(self, name: str) -> Dict[str, torch.Tensor]:
+        """fp32 m and v of one parameter as the step reads them (and its
+        master), in the parameter's shape."""
+        p = self._named[name]
+        s = self._group_of[name].parts(name, p.numel())
+        out = {}
+        for k in ("m", "v"):
+            t = s[k].float()
+            if self.state_bits == 8:
+                t = t * s[f"{k}_scale"].repeat_interleave(BLOCK)[:t.numel()]
+                t = t * t if k == "v" else t
+            out[k] = t.view(p.shape)
+        if "master" in s:
+            out["master"] = s["master"].view(p.shape)
+        return out
+
+    def state_dict(self) -> dict:
+        """CPU tensors by name; 8-bit states as their bytes and scales."""
+        out: dict = {"step": self._step, "state_bits": self.state_bits}
+        for name, p in self._named.items():
+            for k, t in self._group_of[name].parts(name, p.numel()).items():
+                t = t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t
+                out.setdefault(k, {})[name] = t.detach().cpu().clone()
+        return out
+
+    def load_state_dict(self, sd: dict) -> None:
+        """Refuses states of another width or size (``ValueError``) before any
+        of them is taken over."""
+        if int(sd["state_bits"]) != self.state_bits:
+            raise ValueError(f"states of {sd['state_bits']} bits for an AdamW of {self.state_bits}")
+        todo = []
+        for name, p in self._named.items():
+            for k, t in self._group_of[name].parts(name, p.numel()).items():
+                new = sd.get(k, {}).get(name)
+                held = t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t
+                if new is None or new.numel() != t.numel() or new.dtype != held.dtype:
+                    raise ValueError(f"{name}: no {k} of {t.numel()} {held.dtype} values in the state")
+                todo.append((held, new))
+        for held, new in todo:
+            held.copy_(new.reshape(-1))
+        self._step = int(sd["step"])
+
+    @property
+    def optimizer_memory_mb(self) -> float:
+        n = 0
+        for g in self._groups:
+            for t in (*(g.m if isinstance(g.m, tuple) else (g.m,)), *(g.v if isinstance(g.v, tuple) else (g.v,)),
+                      g.masters):
+                n += 0 if t is None else t.numel() * t.element_size()
+        return n / (1024 * 1024)

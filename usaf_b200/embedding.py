@@ -1,0 +1,118 @@
+"""Embedding lookup with scaling, and the gradient of the table, on the device.
+
+:func:`embedding` is differentiable in the table; :func:`embedding_backward`
+gives the gradient by itself, or adds it to one that is there (the
+micro-batches of an accumulated step then touch only the rows of their own
+tokens, where autograd writes and adds whole tables).  The rows of equal
+tokens are summed in fp32 in ascending position, so the gradient repeats bit
+for bit.
+
+A token outside the table gives a row of zeros and no gradient, and sets
+``ERR_BAD_INDEX`` in the int32 error word ``err`` where one is given (as the
+blocks' error words; reading it waits for the device, so the caller chooses
+when).
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import _lib
+from ._lib import call_on, ptr
+
+
+def _check_ids(ids: torch.Tensor, device: torch.device) -> torch.Tensor:
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"ids: expected int32 or int64, got {ids.dtype}")
+    if ids.device != device:
+        raise ValueError(f"ids: expected on {device}, got {ids.device}")
+    return ids.contiguous()
+
+
+def _check_err(err: Optional[torch.Tensor], device: torch.device) -> None:
+    if err is not None and (err.dtype != torch.int32 or err.numel() < 1 or err.device != device):
+        raise ValueError(f"err: expected an int32 word on {device}")
+
+
+def _padding(padding_idx: Optional[int], V: int) -> int:
+    if padding_idx is None:
+        return -1
+    if not -V <= padding_idx < V:
+        raise ValueError(f"padding_idx {padding_idx} outside a table of {V} rows")
+    return padding_idx % V
+
+
+def embedding_forward(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
+                      err: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``scale * table[ids]``, rounded once to the table's type."""
+    if table.dim() != 2 or table.shape[1] < 1:
+        raise ValueError(f"table: expected [rows, width], got {tuple(table.shape)}")
+    if not table.is_contiguous():
+        raise ValueError("table: must be contiguous")
+    ids = _check_ids(ids, table.device)
+    _check_err(err, table.device)
+    V, H = table.shape
+    out = torch.empty(*ids.shape, H, dtype=table.dtype, device=table.device)
+    call_on(table.device, "usaf_embedding_fwd", ptr(ids), 8 * ids.element_size(), ids.numel(), ptr(table),
+            _lib.dtype_code(table.dtype), V, H, float(scale), ptr(out), ptr(err))
+    return out
+
+
+def embedding_backward(dout: torch.Tensor, ids: torch.Tensor, num_embeddings: int, scale: float = 1.0,
+                       padding_idx: Optional[int] = None, grad: Optional[torch.Tensor] = None,
+                       err: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Gradient of the table: ``scale`` times the sum of ``dout``'s rows at each
+    token's positions, zeros in the other rows and in ``padding_idx``'s.  With
+    ``grad`` ([num_embeddings, width], ``dout``'s type or fp32) the sums are
+    added into it instead, and rows without tokens are not touched."""
+    V = int(num_embeddings)
+    if V < 0:
+        raise ValueError(f"num_embeddings: expected >= 0, got {V}")
+    if dout.dim() < 1 or dout.shape[:-1] != ids.shape or dout.shape[-1] < 1:
+        raise ValueError(f"dout: expected shape {tuple(ids.shape)} + (width,), got {tuple(dout.shape)}")
+    H = dout.shape[-1]
+    ids = _check_ids(ids, dout.device)
+    _check_err(err, dout.device)
+    pad = _padding(padding_idx, V)
+    dout = dout.contiguous()
+    adds = grad is not None
+    if adds:
+        if tuple(grad.shape) != (V, H):
+            raise ValueError(f"grad: expected shape {(V, H)}, got {tuple(grad.shape)}")
+        if grad.dtype not in (dout.dtype, torch.float32):
+            raise TypeError(f"grad: expected {dout.dtype} or torch.float32, got {grad.dtype}")
+        if grad.device != dout.device or not grad.is_contiguous():
+            raise ValueError(f"grad: must be contiguous, on {dout.device}")
+    else:
+        grad = torch.empty(V, H, dtype=dout.dtype, device=dout.device)
+    n = ids.numel()
+    ws = torch.empty(max(int(_lib.LIB.usaf_embedding_workspace_bytes(n, V, H)), 16), dtype=torch.uint8,
+                     device=dout.device)
+    call_on(dout.device, "usaf_embedding_bwd", ptr(dout), ptr(ids), 8 * ids.element_size(), n,
+            _lib.dtype_code(dout.dtype), V, H, float(scale), pad, int(adds), ptr(grad),
+            _lib.dtype_code(grad.dtype), ptr(ws), ptr(err))
+    return grad
+
+
+class _EmbeddingFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, table, scale, padding_idx, err):
+        ctx.save_for_backward(ids)
+        ctx.args = (table.shape[0], scale, padding_idx)
+        return embedding_forward(ids, table, scale, err)
+
+    @staticmethod
+    def backward(ctx, dout):
+        (ids,) = ctx.saved_tensors
+        return None, embedding_backward(dout, ids, *ctx.args), None, None, None
+
+
+def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, padding_idx: Optional[int] = None,
+              err: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``scale * table[ids]`` (any shape of ``ids``), differentiable in the
+    table; ``padding_idx``'s row gets no gradient."""
+    _padding(padding_idx, table.shape[0])
+    if torch.is_grad_enabled() and table.requires_grad:
+        return _EmbeddingFn.apply(ids, table, scale, padding_idx, err)
+    return embedding_forward(ids, table, scale, err)

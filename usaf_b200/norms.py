@@ -1,0 +1,140 @@
+"""RMS norm with its backward pass, on the device.
+
+The norms of a decoder layer (``x / sqrt(mean(x^2) + eps) * weight`` over the
+last dimension), with the residual addition in front of them fused:
+:func:`rms_norm` is differentiable; :func:`rms_norm_forward` and
+:func:`rms_norm_backward` are its two passes for a caller that sequences them
+itself, as :class:`usaf_b200.engine.MoEBlock` does.  Sums and products run in
+fp32 and every output is rounded once; the weight's gradient is summed in a
+fixed order, so results repeat bit for bit.
+
+Rows may be strided views as long as the last dimension is contiguous and the
+leading ones fold into one stride (others are copied).  Types: fp32, bf16 or
+fp16 rows; the weight has the rows' type or fp32.
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+from ._lib import call_on, ptr
+
+MAX_WIDTH = 32768
+
+
+def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """``t`` (or a copy) as rows of its last dimension, and their stride."""
+    H = t.shape[-1]
+    if t.is_contiguous():
+        return t, H
+    if t.stride(-1) == 1:
+        try:
+            v = t.view(-1, H)
+            return v, v.stride(0)
+        except RuntimeError:      # the leading dimensions do not fold into one stride
+            pass
+    return t.contiguous(), H
+
+
+def _check(x: torch.Tensor, weight: torch.Tensor) -> int:
+    if x.dim() < 1 or weight.dim() != 1 or weight.shape[0] != x.shape[-1] or x.shape[-1] < 1:
+        raise ValueError(f"weight: expected shape ({x.shape[-1] if x.dim() else '?'},), got {tuple(weight.shape)}")
+    if x.shape[-1] > MAX_WIDTH:
+        raise ValueError(f"rows of {x.shape[-1]} values; at most {MAX_WIDTH} are handled")
+    if weight.dtype not in (x.dtype, torch.float32):
+        raise TypeError(f"weight: expected {x.dtype} or torch.float32, got {weight.dtype}")
+    if weight.device != x.device:
+        raise ValueError("weight: expected on the device of the rows")
+    if not weight.is_contiguous():
+        raise ValueError("weight: must be contiguous")
+    return _lib.dtype_code(x.dtype)
+
+
+def _check_like(name: str, t: torch.Tensor, x: torch.Tensor) -> None:
+    if t.shape != x.shape:
+        raise ValueError(f"{name}: expected shape {tuple(x.shape)}, got {tuple(t.shape)}")
+    if t.dtype != x.dtype:
+        raise TypeError(f"{name}: expected dtype {x.dtype}, got {t.dtype}")
+    if t.device != x.device:
+        raise ValueError(f"{name}: expected on {x.device}, got {t.device}")
+
+
+def rms_norm_forward(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
+                     residual: Optional[torch.Tensor] = None, want_rstd: bool = True):
+    """``(y, rstd, total)``: ``total`` is ``x + residual`` rounded to the rows'
+    type (``x`` itself without a residual), ``y`` its norm, ``rstd`` the fp32
+    1/sqrt(mean + eps) of every row for :func:`rms_norm_backward` (None unless
+    wanted)."""
+    dtc = _check(x, weight)
+    if not eps >= 0:
+        raise ValueError(f"eps: expected >= 0, got {eps}")
+    H = x.shape[-1]
+    n = x.numel() // H
+    xr, ldx = _rows(x)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    rstd = torch.empty(n, dtype=torch.float32, device=x.device) if want_rstd else None
+    total, rr, ldr = x, None, 0
+    if residual is not None:
+        _check_like("residual", residual, x)
+        rr, ldr = _rows(residual)
+        total = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    call_on(x.device, "usaf_rms_norm_fwd", ptr(xr), ldx, ptr(rr), ldr, ptr(weight), dtc,
+            _lib.dtype_code(weight.dtype), n, H, float(eps), None if rr is None else ptr(total), ptr(y), ptr(rstd))
+    return y, rstd, total
+
+
+def rms_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor,
+                      dsum: Optional[torch.Tensor] = None, want_dw: bool = True):
+    """``(dx, dw)`` from the gradient ``dy`` of ``y``; ``x`` is the ``total`` of
+    :func:`rms_norm_forward`.  ``dsum``, the gradient of ``total`` where it is
+    used further, is added to ``dx``, which is then the gradient of ``x`` and of
+    ``residual`` alike.  ``dw`` has the weight's type (None unless wanted)."""
+    dtc = _check(x, weight)
+    H = x.shape[-1]
+    n = x.numel() // H
+    _check_like("dy", dy, x)
+    if rstd.numel() != n or rstd.dtype != torch.float32 or rstd.device != x.device or not rstd.is_contiguous():
+        raise ValueError(f"rstd: expected {n} contiguous fp32 values on {x.device}")
+    xr, ldx = _rows(x)
+    dyr, lddy = _rows(dy)
+    dsr, ldds = None, 0
+    if dsum is not None:
+        _check_like("dsum", dsum, x)
+        dsr, ldds = _rows(dsum)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dw = ws = None
+    if want_dw:
+        dw = torch.empty_like(weight)
+        ws = torch.empty(max(int(_lib.LIB.usaf_rms_norm_workspace_bytes(n, H)), 16), dtype=torch.uint8,
+                         device=x.device)
+    call_on(x.device, "usaf_rms_norm_bwd", ptr(dyr), lddy, ptr(xr), ldx, ptr(weight), ptr(rstd), ptr(dsr), ldds, dtc,
+            _lib.dtype_code(weight.dtype), n, H, ptr(dx), ptr(dw), ptr(ws))
+    return dx, dw
+
+
+class _RmsNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, eps, residual):
+        y, rstd, total = rms_norm_forward(x, weight, eps, residual)
+        ctx.save_for_backward(total, weight, rstd)
+        ctx.has_residual = residual is not None
+        return (y, total) if ctx.has_residual else y
+
+    @staticmethod
+    def backward(ctx, dy, dsum=None):
+        total, weight, rstd = ctx.saved_tensors
+        dx, dw = rms_norm_backward(dy, total, weight, rstd, dsum, want_dw=ctx.needs_input_grad[1])
+        return dx, dw, None, dx if ctx.has_residual else None
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: Optional[torch.Tensor] = None):
+    """``y``, the RMS norm of ``x`` over its last dimension; with ``residual``
+    the pair ``(y, total)`` of the norm of ``x + residual`` and that sum.
+    Differentiable in ``x``, ``weight`` and ``residual``."""
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
+                                    or (residual is not None and residual.requires_grad)):
+        return _RmsNormFn.apply(x, weight, eps, residual)
+    y, _, total = rms_norm_forward(x, weight, eps, residual, want_rstd=False)
+    return y if residual is None else (y, total)
