@@ -117,12 +117,14 @@ def call(name: str, *args):
 
 def call_on(device: torch.device, name: str, *args):
     """:func:`call` on the current stream of ``device`` (appended as the last
-    argument), whichever device is current."""
+    argument), whichever device is current.  The raw stream handle is taken
+    directly: building the Stream object costs as much as a launch."""
+    st = torch._C._cuda_getCurrentRawStream(device.index)
     if device.index == torch.cuda.current_device():
-        call(name, *args, torch.cuda.current_stream().cuda_stream)
+        call(name, *args, st)
     else:
         with torch.cuda.device(device):
-            call(name, *args, torch.cuda.current_stream().cuda_stream)
+            call(name, *args, st)
 
 
 def dtype_code(dt: torch.dtype) -> int:

@@ -11,7 +11,8 @@
 
 namespace usaf {
 
-constexpr int kNormMaxPartials = 296;   // two CTAs per SM
+constexpr int kNormMaxPartials = 592;   // four CTAs per SM
+constexpr int kNormMaxBlock = 512;      // 128 registers a thread
 constexpr int kNormMaxH = 32768;        // fp32 dw sums of a row in shared memory
 
 template <int NT> __device__ __forceinline__ float block_sum(float v, float *red) {
@@ -25,7 +26,220 @@ template <int NT> __device__ __forceinline__ float block_sum(float v, float *red
     return s;
 }
 
-// any width, stride and alignment: one CTA per row
+// ---- rows in registers --------------------------------------------------------
+// `tpr` threads (a power of two up to 32, or whole warps) hold one row, NV
+// vectors of VN values each: vector i of thread t is columns (i tpr + t) VN ...,
+// so that every load of a warp is contiguous.  A CTA holds blockDim / tpr rows
+// at a time and walks down the rows with the weight kept in registers, each row
+// read once.
+template <typename T, int VN> struct alignas(sizeof(T) * VN) Vec { T v[VN]; };
+
+template <typename T, int VN> __device__ __forceinline__ Vec<T, VN> load_vec(const T *p) {
+    Vec<T, VN> r;
+    constexpr int B = sizeof(T) * VN;
+    if constexpr (B >= 16) {                 // 16 bytes a load (fp32 weights of 8 values: two)
+#pragma unroll
+        for (int i = 0; i < B / 16; ++i)
+            reinterpret_cast<uint4 *>(&r)[i] = reinterpret_cast<const uint4 *>(p)[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < VN; ++i) r.v[i] = p[i];
+    }
+    return r;
+}
+
+template <typename T, int VN> __device__ __forceinline__ void store_vec(T *p, const Vec<T, VN> &r) {
+    if constexpr (sizeof(T) * VN == 16) *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(&r);
+    else
+#pragma unroll
+        for (int i = 0; i < VN; ++i) p[i] = r.v[i];
+}
+
+// sum over the row's threads, in the same order for each of them; `red` holds
+// a value per warp, and rows alternate between two of them so that one barrier
+// a row is enough
+__device__ __forceinline__ float row_sum(float v, int tpr, int group, float *red) {
+    for (int o = min(tpr, 32) >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (tpr > 32) {
+        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+        asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(tpr) : "memory");
+        const int n = tpr >> 5;
+        v = 0.0f;
+        for (int i = 0; i < n; ++i) v += red[group * n + i];
+    }
+    return v;
+}
+
+struct NormFwd {
+    const void *x; int64_t ldx;
+    const void *res; int64_t ldr;
+    const void *w;
+    int64_t rows; int H; float eps;
+    void *sum, *y; float *rstd;
+};
+
+struct NormBwd {
+    const void *dy; int64_t lddy;
+    const void *x; int64_t ldx;
+    const void *w; const float *rstd;
+    const void *dsum; int64_t ldds;
+    int64_t rows; int H;
+    void *dx, *dw; float *part;
+};
+
+template <typename T, typename W, int VN, int NV, bool RES>
+__global__ void __launch_bounds__(kNormMaxBlock) norm_fwd_rows(const NormFwd a, int tpr) {
+    __shared__ float red[2][32];
+    const int group = threadIdx.x / tpr, t = threadIdx.x - group * tpr, groups = blockDim.x / tpr;
+    const T *x = static_cast<const T *>(a.x), *res = static_cast<const T *>(a.res);
+    const W *w = static_cast<const W *>(a.w);
+    Vec<W, VN> wv[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * tpr + t) * VN;
+        if (c < a.H) wv[i] = load_vec<W, VN>(w + c);
+    }
+    const float inv_h = 1.0f / (float)a.H;
+    int flip = 0;
+    // every thread takes every turn: the shuffles and barriers are for whole groups
+    for (int64_t base = (int64_t)blockIdx.x * groups; base < a.rows; base += (int64_t)gridDim.x * groups) {
+        const int64_t row = base + group;
+        const bool in = row < a.rows;
+        Vec<T, VN> v[NV], q[RES ? NV : 1];
+        float ss = 0.0f;
+        if (in) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int c = (i * tpr + t) * VN;
+                if (c < a.H) {
+                    v[i] = load_vec<T, VN>(x + row * a.ldx + c);
+                    if constexpr (RES) q[i] = load_vec<T, VN>(res + row * a.ldr + c);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int c = (i * tpr + t) * VN;
+                if (c < a.H) {
+                    if constexpr (RES) {
+#pragma unroll
+                        for (int k = 0; k < VN; ++k) v[i].v[k] = from_f<T>(to_f(v[i].v[k]) + to_f(q[i].v[k]));
+                        store_vec<T, VN>(static_cast<T *>(a.sum) + row * a.H + c, v[i]);
+                    }
+#pragma unroll
+                    for (int k = 0; k < VN; ++k) ss = fmaf(to_f(v[i].v[k]), to_f(v[i].v[k]), ss);
+                }
+            }
+        }
+        ss = row_sum(ss, tpr, group, red[flip]);
+        flip ^= 1;
+        const float r = __frcp_rn(__fsqrt_rn(ss * inv_h + a.eps));
+        if (in) {
+            if (a.rstd && t == 0) a.rstd[row] = r;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int c = (i * tpr + t) * VN;
+                if (c < a.H) {
+                    Vec<T, VN> o;
+#pragma unroll
+                    for (int k = 0; k < VN; ++k) o.v[k] = from_f<T>(to_f(v[i].v[k]) * r * to_f(wv[i].v[k]));
+                    store_vec<T, VN>(static_cast<T *>(a.y) + row * a.H + c, o);
+                }
+            }
+        }
+    }
+}
+
+template <typename T, typename W, int VN, int NV, bool DSUM, bool DW>
+__global__ void __launch_bounds__(kNormMaxBlock) norm_bwd_rows(const NormBwd a, int tpr) {
+    __shared__ float red[2][32];
+    extern __shared__ float fold[];          // [groups][H], where a CTA has several rows
+    const int group = threadIdx.x / tpr, t = threadIdx.x - group * tpr, groups = blockDim.x / tpr;
+    const T *x = static_cast<const T *>(a.x), *dy = static_cast<const T *>(a.dy), *ds = static_cast<const T *>(a.dsum);
+    const W *w = static_cast<const W *>(a.w);
+    Vec<W, VN> wv[NV];
+    float acc[DW ? NV : 1][VN];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * tpr + t) * VN;
+        if (c < a.H) wv[i] = load_vec<W, VN>(w + c);
+        if constexpr (DW)
+#pragma unroll
+            for (int k = 0; k < VN; ++k) acc[i][k] = 0.0f;
+    }
+    const float inv_h = 1.0f / (float)a.H;
+    int flip = 0;
+    for (int64_t base = (int64_t)blockIdx.x * groups; base < a.rows; base += (int64_t)gridDim.x * groups) {
+        const int64_t row = base + group;
+        const bool in = row < a.rows;
+        Vec<T, VN> xv[NV], dv[NV], sv[DSUM ? NV : 1];
+        float dot = 0.0f, r = 0.0f;
+        if (in) {
+            r = a.rstd[row];
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int c = (i * tpr + t) * VN;
+                if (c < a.H) {
+                    xv[i] = load_vec<T, VN>(x + row * a.ldx + c);
+                    dv[i] = load_vec<T, VN>(dy + row * a.lddy + c);
+                    if constexpr (DSUM) sv[i] = load_vec<T, VN>(ds + row * a.ldds + c);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int c = (i * tpr + t) * VN;
+                if (c < a.H) {
+#pragma unroll
+                    for (int k = 0; k < VN; ++k) {
+                        const float d = to_f(dv[i].v[k]), hat = to_f(xv[i].v[k]) * r;
+                        dot = fmaf(d * to_f(wv[i].v[k]), hat, dot);
+                        if constexpr (DW) acc[i][k] = fmaf(d, hat, acc[i][k]);
+                    }
+                }
+            }
+        }
+        dot = row_sum(dot, tpr, group, red[flip]) * inv_h;
+        flip ^= 1;
+        if (in) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int c = (i * tpr + t) * VN;
+                if (c < a.H) {
+                    Vec<T, VN> o;
+#pragma unroll
+                    for (int k = 0; k < VN; ++k) {
+                        const float hat = to_f(xv[i].v[k]) * r;
+                        float v = r * (to_f(dv[i].v[k]) * to_f(wv[i].v[k]) - hat * dot);
+                        if constexpr (DSUM) v += to_f(sv[i].v[k]);
+                        o.v[k] = from_f<T>(v);
+                    }
+                    store_vec<T, VN>(static_cast<T *>(a.dx) + row * a.H + c, o);
+                }
+            }
+        }
+    }
+    if constexpr (DW) {
+        float *part = a.part + (int64_t)blockIdx.x * a.H;
+        float *to = groups > 1 ? fold + (int64_t)group * a.H : part;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * tpr + t) * VN;
+            if (c < a.H)
+#pragma unroll
+                for (int k = 0; k < VN; ++k) to[c + k] = acc[i][k];
+        }
+        if (groups > 1) {
+            __syncthreads();
+            for (int c = threadIdx.x; c < a.H; c += blockDim.x) {
+                float v = 0.0f;
+                for (int g = 0; g < groups; ++g) v += fold[g * a.H + c];
+                part[c] = v;
+            }
+        }
+    }
+}
+
+// ---- any width, stride and alignment ---------------------------------------------
+// one CTA per row, rows wider than the registers of a CTA or not aligned: read twice
 template <typename T, typename W>
 __global__ void __launch_bounds__(256)
 norm_fwd_any(const T *__restrict__ x, int64_t ldx, const T *__restrict__ res, int64_t ldr,
@@ -82,44 +296,85 @@ norm_bwd_any(const T *__restrict__ dy, int64_t lddy, const T *__restrict__ x, in
         for (int c = threadIdx.x; c < H; c += 256) part[(int64_t)blockIdx.x * H + c] = acc[c];
 }
 
-// dw[c] = sum over the P partial rows: 32 columns a CTA, 8 warps over the rows,
-// their sums added in warp order
+// dw[c] = sum over the P partial rows: 32 columns a CTA, 32 warps over the rows
+// (a few loads each, all in flight), their sums added in warp order
 template <typename W>
-__global__ void __launch_bounds__(256) norm_dw_kernel(const float *__restrict__ part, int P, int H,
-                                                      W *__restrict__ dw) {
-    __shared__ float s[8][32];
-    const int c = blockIdx.x * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5;
+__global__ void __launch_bounds__(1024) norm_dw_kernel(const float *__restrict__ part, int P, int H,
+                                                       W *__restrict__ dw) {
+    __shared__ float s[32][33];
+    const int lane = threadIdx.x & 31, k = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     float v = 0.0f;
-    if (c < H)
-        for (int p = k; p < P; p += 8) v += part[(int64_t)p * H + c];
-    s[k][threadIdx.x & 31] = v;
-    __syncthreads();
-    if (k == 0 && c < H) {
-        float t = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) t += s[i][threadIdx.x];
-        dw[c] = from_f<W>(t);
+    if (c < H) {
+#pragma unroll 10
+        for (int p = k; p < P; p += 32) v += part[(int64_t)p * H + c];
     }
+    s[k][lane] = v;
+    __syncthreads();
+    v = warp_sum(s[lane][k]);                // warp k adds column k of the CTA
+    if (lane == 0 && blockIdx.x * 32 + k < H) dw[blockIdx.x * 32 + k] = from_f<W>(v);
 }
 
-struct NormFwd {
-    const void *x; int64_t ldx;
-    const void *res; int64_t ldr;
-    const void *w;
-    int64_t rows; int H; float eps;
-    void *sum, *y; float *rstd;
+// How the rows are cut: vectors of 16 bytes where every row starts on a 16-byte
+// boundary, else single values; NV vectors a thread, threads a row, threads a CTA.
+struct RowPlan {
+    int vn, nv, tpr, block;
 };
 
-struct NormBwd {
-    const void *dy; int64_t lddy;
-    const void *x; int64_t ldx;
-    const void *w; const float *rstd;
-    const void *dsum; int64_t ldds;
-    int64_t rows; int H;
-    void *dx, *dw; float *part;
-};
+template <typename T> static RowPlan plan_rows(int H, bool aligned) {
+    RowPlan p{aligned ? 16 / (int)sizeof(T) : 1, 8, 0, 0};
+    const int n = (H + p.vn - 1) / p.vn;     // vectors of a row
+    if (aligned) p.nv = n <= 32 ? 1 : n <= 2 * kNormMaxBlock ? 2 : 4;
+    const int t = (n + p.nv - 1) / p.nv;
+    if (t > 32) {
+        p.tpr = (t + 31) / 32 * 32;
+    } else {
+        p.tpr = 1;
+        while (p.tpr < t) p.tpr *= 2;
+    }
+    p.block = p.tpr >= 256 ? p.tpr : 256 / p.tpr * p.tpr;
+    if (p.tpr > kNormMaxBlock) p.nv = 0;     // too wide for a CTA's registers
+    return p;
+}
+
+static bool on16(const void *p, int64_t ld_bytes) { return ((uintptr_t)p | (uintptr_t)ld_bytes) % 16 == 0; }
+
+// CTAs that are resident at once, or fewer where the rows are fewer
+template <typename K> static int row_grid(K kernel, int block, int smem, int64_t rows, int groups, int most) {
+    int per_sm = 1;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, block, smem) != cudaSuccess || per_sm < 1) {
+        (void)cudaGetLastError();
+        return 0;
+    }
+    return (int)std::min<int64_t>((rows + groups - 1) / groups, std::min(148 * per_sm, most));
+}
+
+template <typename T, typename W, int VN, int NV, bool RES>
+static int fwd_launch(const NormFwd &a, const RowPlan &p, cudaStream_t st) {
+    const int grid = row_grid(norm_fwd_rows<T, W, VN, NV, RES>, p.block, 0, a.rows, p.block / p.tpr, 1 << 30);
+    if (grid < 1) return USAF_ECUDA;
+    norm_fwd_rows<T, W, VN, NV, RES><<<grid, p.block, 0, st>>>(a, p.tpr);
+    USAF_CHECK_LAUNCH();
+    return USAF_OK;
+}
+
+template <typename T, typename W, int VN, int NV>
+static int fwd_launch(const NormFwd &a, const RowPlan &p, cudaStream_t st) {
+    return a.res ? fwd_launch<T, W, VN, NV, true>(a, p, st) : fwd_launch<T, W, VN, NV, false>(a, p, st);
+}
 
 template <typename T, typename W> static int norm_fwd(const NormFwd &a, cudaStream_t st) {
+    constexpr int N = 16 / (int)sizeof(T);
+    const int64_t row = (int64_t)a.H * sizeof(T);
+    const bool aligned = on16(a.x, a.ldx * sizeof(T)) && on16(a.y, row) && on16(a.w, 0) &&
+                         (!a.res || (on16(a.res, a.ldr * sizeof(T)) && on16(a.sum, row)));
+    const RowPlan p = plan_rows<T>(a.H, aligned);
+    if (p.vn > 1) {
+        if (p.nv == 1) return fwd_launch<T, W, N, 1>(a, p, st);
+        if (p.nv == 2) return fwd_launch<T, W, N, 2>(a, p, st);
+        if (p.nv == 4) return fwd_launch<T, W, N, 4>(a, p, st);
+    } else if (p.nv) {
+        return fwd_launch<T, W, 1, 8>(a, p, st);
+    }
     const unsigned grid = (unsigned)std::min<int64_t>(a.rows, 148 * 8);
     norm_fwd_any<T, W><<<grid, 256, 0, st>>>((const T *)a.x, a.ldx, (const T *)a.res, a.ldr, (const W *)a.w, a.rows,
                                              a.H, a.eps, (T *)a.sum, (T *)a.y, a.rstd);
@@ -127,20 +382,59 @@ template <typename T, typename W> static int norm_fwd(const NormFwd &a, cudaStre
     return USAF_OK;
 }
 
+// the partial rows of a launch: P of them
+template <typename T, typename W, int VN, int NV, bool DSUM, bool DW>
+static int bwd_launch(const NormBwd &a, const RowPlan &p, int *P, cudaStream_t st) {
+    const int groups = p.block / p.tpr, smem = DW && groups > 1 ? groups * a.H * 4 : 0;
+    const int grid = row_grid(norm_bwd_rows<T, W, VN, NV, DSUM, DW>, p.block, smem, a.rows, groups,
+                              DW ? kNormMaxPartials : 1 << 30);
+    if (grid < 1) return USAF_ECUDA;
+    norm_bwd_rows<T, W, VN, NV, DSUM, DW><<<grid, p.block, smem, st>>>(a, p.tpr);
+    USAF_CHECK_LAUNCH();
+    *P = grid;
+    return USAF_OK;
+}
+
+template <typename T, typename W, int VN, int NV>
+static int bwd_launch(const NormBwd &a, const RowPlan &p, int *P, cudaStream_t st) {
+    if (a.dw)
+        return a.dsum ? bwd_launch<T, W, VN, NV, true, true>(a, p, P, st) : bwd_launch<T, W, VN, NV, false, true>(a, p, P, st);
+    return a.dsum ? bwd_launch<T, W, VN, NV, true, false>(a, p, P, st) : bwd_launch<T, W, VN, NV, false, false>(a, p, P, st);
+}
+
+template <typename T, typename W> static int bwd_rows(const NormBwd &a, int *P, cudaStream_t st) {
+    constexpr int N = 16 / (int)sizeof(T);
+    const bool aligned = on16(a.x, a.ldx * sizeof(T)) && on16(a.dy, a.lddy * sizeof(T)) && on16(a.w, 0) &&
+                         on16(a.dx, (int64_t)a.H * sizeof(T)) && (!a.dsum || on16(a.dsum, a.ldds * sizeof(T)));
+    const RowPlan p = plan_rows<T>(a.H, aligned);
+    if (p.vn > 1) {
+        if (p.nv == 1) return bwd_launch<T, W, N, 1>(a, p, P, st);
+        if (p.nv == 2) return bwd_launch<T, W, N, 2>(a, p, P, st);
+        if (p.nv == 4) return bwd_launch<T, W, N, 4>(a, p, P, st);
+    } else if (p.nv) {
+        return bwd_launch<T, W, 1, 8>(a, p, P, st);
+    }
+    const int smem = a.dw ? a.H * 4 : 0;
+    if (smem > 48 * 1024 && cudaFuncSetAttribute(norm_bwd_any<T, W>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 kNormMaxH * 4) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return USAF_ECUDA;
+    }
+    *P = (int)std::min<int64_t>(a.rows, kNormMaxPartials);
+    norm_bwd_any<T, W><<<*P, 256, smem, st>>>((const T *)a.dy, a.lddy, (const T *)a.x, a.ldx, (const W *)a.w, a.rstd,
+                                              (const T *)a.dsum, a.ldds, a.rows, a.H, (T *)a.dx, a.dw ? a.part : nullptr);
+    USAF_CHECK_LAUNCH();
+    return USAF_OK;
+}
+
 template <typename T, typename W> static int norm_bwd(const NormBwd &a, cudaStream_t st) {
-    const int P = (int)std::min<int64_t>(a.rows, kNormMaxPartials);
-    float *part = a.dw ? a.part : nullptr;
-    if (P) {
-        const int smem = part ? a.H * 4 : 0;
-        if (smem > 48 * 1024 &&
-            cudaFuncSetAttribute(norm_bwd_any<T, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-            return USAF_ECUDA;
-        norm_bwd_any<T, W><<<P, 256, smem, st>>>((const T *)a.dy, a.lddy, (const T *)a.x, a.ldx, (const W *)a.w, a.rstd,
-                                                 (const T *)a.dsum, a.ldds, a.rows, a.H, (T *)a.dx, part);
-        USAF_CHECK_LAUNCH();
+    int P = 0;
+    if (a.rows) {
+        const int rc = bwd_rows<T, W>(a, &P, st);
+        if (rc) return rc;
     }
     if (a.dw) {
-        norm_dw_kernel<W><<<cdiv(a.H, 32), 256, 0, st>>>(a.part, P, a.H, (W *)a.dw);
+        norm_dw_kernel<W><<<cdiv(a.H, 32), 1024, 0, st>>>(a.part, P, a.H, (W *)a.dw);
         USAF_CHECK_LAUNCH();
     }
     return USAF_OK;
