@@ -127,14 +127,14 @@ def call_on(device: torch.device, name: str, *args):
             call(name, *args, st)
 
 
+_DTYPES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
+
+
 def dtype_code(dt: torch.dtype) -> int:
-    if dt == torch.float32:
-        return F32
-    if dt == torch.bfloat16:
-        return BF16
-    if dt == torch.float16:
-        return F16
-    raise TypeError(f"unsupported dtype {dt}")
+    code = _DTYPES.get(dt)
+    if code is None:
+        raise TypeError(f"unsupported dtype {dt}")
+    return code
 
 
 def ptr(t):

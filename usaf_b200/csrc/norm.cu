@@ -87,42 +87,109 @@ struct NormBwd {
     void *dx, *dw; float *part;
 };
 
+// ---- rows ahead -----------------------------------------------------------------
+// Aligned rows come through a ring in shared memory that every thread fills for
+// itself by asynchronous copies: a thread has D - 1 rows' vectors on their way
+// and reads back only what it copied, so no barrier and no register is spent on
+// them.  384 bytes a thread keep about 100 KB in flight on an SM.
+__device__ __forceinline__ void copy_ahead(uint32_t to, const void *from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ uint4 ring_read(uint32_t at) {
+    uint4 u;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(at));
+    return u;
+}
+constexpr int ring_depth(int nv, int tensors) {
+    const int d = 12 / (nv * tensors);
+    return d > 6 ? 6 : d < 2 ? 2 : d;
+}
+
+// NT tensors' rows of one thread: `p[k]`, `ld[k]`; vector i of the row of turn n
+template <typename T, int VN, int NV, int NT> struct RowRing {
+    static constexpr int D = ring_depth(NV, NT);
+    const T *p[NT];
+    int64_t ld[NT];
+    uint32_t base;               // this thread's 16 bytes of the first slot
+    int tpr, t, H;
+    int64_t rows;
+
+    __device__ __forceinline__ uint32_t slot(int stage, int k, int i) const {
+        return base + (uint32_t)(((stage * NT + k) * NV + i) * blockDim.x) * 16u;
+    }
+    __device__ __forceinline__ void fetch(int stage, int64_t row) const {
+        if (row < rows) {
+#pragma unroll
+            for (int k = 0; k < NT; ++k)
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    const int c = (i * tpr + t) * VN;
+                    if (c < H) copy_ahead(slot(stage, k, i), p[k] + row * ld[k] + c);
+                }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    __device__ __forceinline__ static void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(D - 1) : "memory"); }
+    // vector i of tensor k: from the ring, or for single values from memory
+    __device__ __forceinline__ Vec<T, VN> get(int stage, int k, int i, int64_t row) const {
+        Vec<T, VN> v;
+        if constexpr (VN > 1) *reinterpret_cast<uint4 *>(&v) = ring_read(slot(stage, k, i));
+        else v.v[0] = p[k][row * ld[k] + i * tpr + t];
+        return v;
+    }
+};
+
 template <typename T, typename W, int VN, int NV, bool RES>
 __global__ void __launch_bounds__(kNormMaxBlock) norm_fwd_rows(const NormFwd a, int tpr) {
     __shared__ float red[2][32];
+    extern __shared__ uint4 dyn[];
     const int group = threadIdx.x / tpr, t = threadIdx.x - group * tpr, groups = blockDim.x / tpr;
-    const T *x = static_cast<const T *>(a.x), *res = static_cast<const T *>(a.res);
-    const W *w = static_cast<const W *>(a.w);
+    using Ring = RowRing<T, VN, NV, RES ? 2 : 1>;
+    Ring ring;
+    ring.p[0] = static_cast<const T *>(a.x);
+    ring.ld[0] = a.ldx;
+    if constexpr (RES) {
+        ring.p[1] = static_cast<const T *>(a.res);
+        ring.ld[1] = a.ldr;
+    }
+    ring.base = (uint32_t)__cvta_generic_to_shared(dyn + threadIdx.x);
+    ring.tpr = tpr;
+    ring.t = t;
+    ring.H = a.H;
+    ring.rows = a.rows;
+    const int64_t step = (int64_t)gridDim.x * groups;
+    const int64_t start = (int64_t)blockIdx.x * groups;
+    if constexpr (VN > 1)
+#pragma unroll
+        for (int d = 0; d < Ring::D - 1; ++d) ring.fetch(d, start + d * step + group);
     Vec<W, VN> wv[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (i * tpr + t) * VN;
-        if (c < a.H) wv[i] = load_vec<W, VN>(w + c);
+        if (c < a.H) wv[i] = load_vec<W, VN>(static_cast<const W *>(a.w) + c);
     }
     const float inv_h = 1.0f / (float)a.H;
-    int flip = 0;
+    int flip = 0, stage = 0;
     // every thread takes every turn: the shuffles and barriers are for whole groups
-    for (int64_t base = (int64_t)blockIdx.x * groups; base < a.rows; base += (int64_t)gridDim.x * groups) {
+    for (int64_t base = start; base < a.rows; base += step) {
         const int64_t row = base + group;
         const bool in = row < a.rows;
-        Vec<T, VN> v[NV], q[RES ? NV : 1];
+        if constexpr (VN > 1) {
+            ring.fetch(stage == 0 ? Ring::D - 1 : stage - 1, row + (Ring::D - 1) * step);
+            Ring::wait();
+        }
+        Vec<T, VN> v[NV];
         float ss = 0.0f;
         if (in) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int c = (i * tpr + t) * VN;
                 if (c < a.H) {
-                    v[i] = load_vec<T, VN>(x + row * a.ldx + c);
-                    if constexpr (RES) q[i] = load_vec<T, VN>(res + row * a.ldr + c);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int c = (i * tpr + t) * VN;
-                if (c < a.H) {
+                    v[i] = ring.get(stage, 0, i, row);
                     if constexpr (RES) {
+                        const Vec<T, VN> q = ring.get(stage, RES ? 1 : 0, i, row);
 #pragma unroll
-                        for (int k = 0; k < VN; ++k) v[i].v[k] = from_f<T>(to_f(v[i].v[k]) + to_f(q[i].v[k]));
+                        for (int k = 0; k < VN; ++k) v[i].v[k] = from_f<T>(to_f(v[i].v[k]) + to_f(q.v[k]));
                         store_vec<T, VN>(static_cast<T *>(a.sum) + row * a.H + c, v[i]);
                     }
 #pragma unroll
@@ -132,6 +199,7 @@ __global__ void __launch_bounds__(kNormMaxBlock) norm_fwd_rows(const NormFwd a, 
         }
         ss = row_sum(ss, tpr, group, red[flip]);
         flip ^= 1;
+        stage = stage == Ring::D - 1 ? 0 : stage + 1;
         const float r = __frcp_rn(__fsqrt_rn(ss * inv_h + a.eps));
         if (in) {
             if (a.rstd && t == 0) a.rstd[row] = r;
@@ -152,74 +220,97 @@ __global__ void __launch_bounds__(kNormMaxBlock) norm_fwd_rows(const NormFwd a, 
 template <typename T, typename W, int VN, int NV, bool DSUM, bool DW>
 __global__ void __launch_bounds__(kNormMaxBlock) norm_bwd_rows(const NormBwd a, int tpr) {
     __shared__ float red[2][32];
-    extern __shared__ float fold[];          // [groups][H], where a CTA has several rows
+    extern __shared__ uint4 dyn[];           // the ring; at the end [groups][H] sums, where a CTA has several rows
     const int group = threadIdx.x / tpr, t = threadIdx.x - group * tpr, groups = blockDim.x / tpr;
-    const T *x = static_cast<const T *>(a.x), *dy = static_cast<const T *>(a.dy), *ds = static_cast<const T *>(a.dsum);
-    const W *w = static_cast<const W *>(a.w);
+    using Ring = RowRing<T, VN, NV, DSUM ? 3 : 2>;
+    Ring ring;
+    ring.p[0] = static_cast<const T *>(a.x);
+    ring.ld[0] = a.ldx;
+    ring.p[1] = static_cast<const T *>(a.dy);
+    ring.ld[1] = a.lddy;
+    if constexpr (DSUM) {
+        ring.p[2] = static_cast<const T *>(a.dsum);
+        ring.ld[2] = a.ldds;
+    }
+    ring.base = (uint32_t)__cvta_generic_to_shared(dyn + threadIdx.x);
+    ring.tpr = tpr;
+    ring.t = t;
+    ring.H = a.H;
+    ring.rows = a.rows;
+    const int64_t step = (int64_t)gridDim.x * groups;
+    const int64_t start = (int64_t)blockIdx.x * groups;
+    if constexpr (VN > 1)
+#pragma unroll
+        for (int d = 0; d < Ring::D - 1; ++d) ring.fetch(d, start + d * step + group);
     Vec<W, VN> wv[NV];
     float acc[DW ? NV : 1][VN];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (i * tpr + t) * VN;
-        if (c < a.H) wv[i] = load_vec<W, VN>(w + c);
+        if (c < a.H) wv[i] = load_vec<W, VN>(static_cast<const W *>(a.w) + c);
         if constexpr (DW)
 #pragma unroll
             for (int k = 0; k < VN; ++k) acc[i][k] = 0.0f;
     }
     const float inv_h = 1.0f / (float)a.H;
-    int flip = 0;
-    for (int64_t base = (int64_t)blockIdx.x * groups; base < a.rows; base += (int64_t)gridDim.x * groups) {
+    int flip = 0, stage = 0;
+    float r = start + group < a.rows ? a.rstd[start + group] : 0.0f;
+    for (int64_t base = start; base < a.rows; base += step) {
         const int64_t row = base + group;
         const bool in = row < a.rows;
-        Vec<T, VN> xv[NV], dv[NV], sv[DSUM ? NV : 1];
-        float dot = 0.0f, r = 0.0f;
+        const float r_next = row + step < a.rows ? a.rstd[row + step] : 0.0f;
+        if constexpr (VN > 1) {
+            ring.fetch(stage == 0 ? Ring::D - 1 : stage - 1, row + (Ring::D - 1) * step);
+            Ring::wait();
+        }
+        float dot = 0.0f;
         if (in) {
-            r = a.rstd[row];
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int c = (i * tpr + t) * VN;
                 if (c < a.H) {
-                    xv[i] = load_vec<T, VN>(x + row * a.ldx + c);
-                    dv[i] = load_vec<T, VN>(dy + row * a.lddy + c);
-                    if constexpr (DSUM) sv[i] = load_vec<T, VN>(ds + row * a.ldds + c);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int c = (i * tpr + t) * VN;
-                if (c < a.H) {
+                    const Vec<T, VN> x = ring.get(stage, 0, i, row), d = ring.get(stage, 1, i, row);
 #pragma unroll
                     for (int k = 0; k < VN; ++k) {
-                        const float d = to_f(dv[i].v[k]), hat = to_f(xv[i].v[k]) * r;
-                        dot = fmaf(d * to_f(wv[i].v[k]), hat, dot);
-                        if constexpr (DW) acc[i][k] = fmaf(d, hat, acc[i][k]);
+                        dot = fmaf(to_f(d.v[k]) * to_f(wv[i].v[k]), to_f(x.v[k]), dot);
+                        if constexpr (DW) acc[i][k] = fmaf(to_f(d.v[k]), to_f(x.v[k]) * r, acc[i][k]);
                     }
                 }
             }
         }
-        dot = row_sum(dot, tpr, group, red[flip]) * inv_h;
+        // hat c = s r mean(g s r): s times this
+        const float along = row_sum(dot, tpr, group, red[flip]) * inv_h * r * r * r;
         flip ^= 1;
         if (in) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int c = (i * tpr + t) * VN;
-                if (c < a.H) {
+                if (c < a.H) {               // read again: cheaper than the registers to keep them
+                    const Vec<T, VN> x = ring.get(stage, 0, i, row), d = ring.get(stage, 1, i, row);
                     Vec<T, VN> o;
+                    float v[VN];
 #pragma unroll
-                    for (int k = 0; k < VN; ++k) {
-                        const float hat = to_f(xv[i].v[k]) * r;
-                        float v = r * (to_f(dv[i].v[k]) * to_f(wv[i].v[k]) - hat * dot);
-                        if constexpr (DSUM) v += to_f(sv[i].v[k]);
-                        o.v[k] = from_f<T>(v);
+                    for (int k = 0; k < VN; ++k)
+                        v[k] = fmaf(to_f(d.v[k]) * to_f(wv[i].v[k]), r, -along * to_f(x.v[k]));
+                    if constexpr (DSUM) {
+                        const Vec<T, VN> s = ring.get(stage, DSUM ? 2 : 0, i, row);
+#pragma unroll
+                        for (int k = 0; k < VN; ++k) v[k] += to_f(s.v[k]);
                     }
+#pragma unroll
+                    for (int k = 0; k < VN; ++k) o.v[k] = from_f<T>(v[k]);
                     store_vec<T, VN>(static_cast<T *>(a.dx) + row * a.H + c, o);
                 }
             }
         }
+        stage = stage == Ring::D - 1 ? 0 : stage + 1;
+        r = r_next;
     }
     if constexpr (DW) {
-        float *part = a.part + (int64_t)blockIdx.x * a.H;
+        float *part = a.part + (int64_t)blockIdx.x * a.H, *fold = reinterpret_cast<float *>(dyn);
         float *to = groups > 1 ? fold + (int64_t)group * a.H : part;
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncthreads();                     // the ring is read; its space takes the sums
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * tpr + t) * VN;
@@ -323,7 +414,7 @@ struct RowPlan {
 template <typename T> static RowPlan plan_rows(int H, bool aligned) {
     RowPlan p{aligned ? 16 / (int)sizeof(T) : 1, 8, 0, 0};
     const int n = (H + p.vn - 1) / p.vn;     // vectors of a row
-    if (aligned) p.nv = n <= 32 ? 1 : n <= 2 * kNormMaxBlock ? 2 : 4;
+    if (aligned) p.nv = n <= 4 ? 1 : n <= 2 * kNormMaxBlock ? 2 : 4;
     const int t = (n + p.nv - 1) / p.nv;
     if (t > 32) {
         p.tpr = (t + 31) / 32 * 32;
@@ -338,21 +429,30 @@ template <typename T> static RowPlan plan_rows(int H, bool aligned) {
 
 static bool on16(const void *p, int64_t ld_bytes) { return ((uintptr_t)p | (uintptr_t)ld_bytes) % 16 == 0; }
 
-// CTAs that are resident at once, or fewer where the rows are fewer
-template <typename K> static int row_grid(K kernel, int block, int smem, int64_t rows, int groups, int most) {
-    int per_sm = 1;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, block, smem) != cudaSuccess || per_sm < 1) {
-        (void)cudaGetLastError();
-        return 0;
-    }
+// CTAs that fit the SMs at once by shared memory and `regs` registers a thread,
+// or fewer where the rows are fewer
+static int row_grid(const RowPlan &p, int smem, int regs, int64_t rows, int most) {
+    const int per_sm = std::max(1, std::min({227 * 1024 / (smem + 1024 + 256), 65536 / (regs * p.block),
+                                             2048 / p.block}));
+    const int groups = p.block / p.tpr;
     return (int)std::min<int64_t>((rows + groups - 1) / groups, std::min(148 * per_sm, most));
+}
+
+template <typename K> static bool allow_smem(K kernel, int smem) {
+    if (smem + 256 <= 48 * 1024 ||       // 256 bytes are the reduction's
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess)
+        return true;
+    (void)cudaGetLastError();
+    return false;
 }
 
 template <typename T, typename W, int VN, int NV, bool RES>
 static int fwd_launch(const NormFwd &a, const RowPlan &p, cudaStream_t st) {
-    const int grid = row_grid(norm_fwd_rows<T, W, VN, NV, RES>, p.block, 0, a.rows, p.block / p.tpr, 1 << 30);
-    if (grid < 1) return USAF_ECUDA;
-    norm_fwd_rows<T, W, VN, NV, RES><<<grid, p.block, 0, st>>>(a, p.tpr);
+    constexpr int NT = RES ? 2 : 1;
+    const int smem = VN > 1 ? NV * NT * ring_depth(NV, NT) * 16 * p.block : 0;
+    if (!allow_smem(norm_fwd_rows<T, W, VN, NV, RES>, smem)) return USAF_ECUDA;
+    const int grid = row_grid(p, smem, NV == 4 ? 128 : 64, a.rows, 1 << 30);
+    norm_fwd_rows<T, W, VN, NV, RES><<<grid, p.block, smem, st>>>(a, p.tpr);
     USAF_CHECK_LAUNCH();
     return USAF_OK;
 }
@@ -385,10 +485,11 @@ template <typename T, typename W> static int norm_fwd(const NormFwd &a, cudaStre
 // the partial rows of a launch: P of them
 template <typename T, typename W, int VN, int NV, bool DSUM, bool DW>
 static int bwd_launch(const NormBwd &a, const RowPlan &p, int *P, cudaStream_t st) {
-    const int groups = p.block / p.tpr, smem = DW && groups > 1 ? groups * a.H * 4 : 0;
-    const int grid = row_grid(norm_bwd_rows<T, W, VN, NV, DSUM, DW>, p.block, smem, a.rows, groups,
-                              DW ? kNormMaxPartials : 1 << 30);
-    if (grid < 1) return USAF_ECUDA;
+    constexpr int NT = DSUM ? 3 : 2;
+    const int groups = p.block / p.tpr, fold = DW && groups > 1 ? groups * a.H * 4 : 0;
+    const int smem = std::max(VN > 1 ? NV * NT * ring_depth(NV, NT) * 16 * p.block : 0, fold);
+    if (!allow_smem(norm_bwd_rows<T, W, VN, NV, DSUM, DW>, smem)) return USAF_ECUDA;
+    const int grid = row_grid(p, smem, NV == 4 ? 128 : 64, a.rows, DW ? kNormMaxPartials : 1 << 30);
     norm_bwd_rows<T, W, VN, NV, DSUM, DW><<<grid, p.block, smem, st>>>(a, p.tpr);
     USAF_CHECK_LAUNCH();
     *P = grid;
@@ -415,7 +516,7 @@ template <typename T, typename W> static int bwd_rows(const NormBwd &a, int *P, 
         return bwd_launch<T, W, 1, 8>(a, p, P, st);
     }
     const int smem = a.dw ? a.H * 4 : 0;
-    if (smem > 48 * 1024 && cudaFuncSetAttribute(norm_bwd_any<T, W>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    if (smem + 256 > 48 * 1024 && cudaFuncSetAttribute(norm_bwd_any<T, W>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                  kNormMaxH * 4) != cudaSuccess) {
         (void)cudaGetLastError();
         return USAF_ECUDA;

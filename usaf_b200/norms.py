@@ -39,26 +39,32 @@ def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
 
 
 def _check(x: torch.Tensor, weight: torch.Tensor) -> int:
+    """The width of the rows."""
     if x.dim() < 1 or weight.dim() != 1 or weight.shape[0] != x.shape[-1] or x.shape[-1] < 1:
         raise ValueError(f"weight: expected shape ({x.shape[-1] if x.dim() else '?'},), got {tuple(weight.shape)}")
-    if x.shape[-1] > MAX_WIDTH:
-        raise ValueError(f"rows of {x.shape[-1]} values; at most {MAX_WIDTH} are handled")
-    if weight.dtype not in (x.dtype, torch.float32):
+    H = x.shape[-1]
+    if H > MAX_WIDTH:
+        raise ValueError(f"rows of {H} values; at most {MAX_WIDTH} are handled")
+    if weight.dtype is not x.dtype and weight.dtype is not torch.float32:
         raise TypeError(f"weight: expected {x.dtype} or torch.float32, got {weight.dtype}")
     if weight.device != x.device:
         raise ValueError("weight: expected on the device of the rows")
     if not weight.is_contiguous():
         raise ValueError("weight: must be contiguous")
-    return _lib.dtype_code(x.dtype)
+    return H
 
 
 def _check_like(name: str, t: torch.Tensor, x: torch.Tensor) -> None:
     if t.shape != x.shape:
         raise ValueError(f"{name}: expected shape {tuple(x.shape)}, got {tuple(t.shape)}")
-    if t.dtype != x.dtype:
+    if t.dtype is not x.dtype:
         raise TypeError(f"{name}: expected dtype {x.dtype}, got {t.dtype}")
     if t.device != x.device:
         raise ValueError(f"{name}: expected on {x.device}, got {t.device}")
+
+
+def _dense_like(x: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
 def rms_norm_forward(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
@@ -67,20 +73,19 @@ def rms_norm_forward(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     type (``x`` itself without a residual), ``y`` its norm, ``rstd`` the fp32
     1/sqrt(mean + eps) of every row for :func:`rms_norm_backward` (None unless
     wanted)."""
-    dtc = _check(x, weight)
+    H = _check(x, weight)
     if not eps >= 0:
         raise ValueError(f"eps: expected >= 0, got {eps}")
-    H = x.shape[-1]
     n = x.numel() // H
     xr, ldx = _rows(x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    rstd = torch.empty(n, dtype=torch.float32, device=x.device) if want_rstd else None
+    y = _dense_like(x)
+    rstd = x.new_empty(n, dtype=torch.float32) if want_rstd else None
     total, rr, ldr = x, None, 0
     if residual is not None:
         _check_like("residual", residual, x)
         rr, ldr = _rows(residual)
-        total = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    call_on(x.device, "usaf_rms_norm_fwd", ptr(xr), ldx, ptr(rr), ldr, ptr(weight), dtc,
+        total = _dense_like(x)
+    call_on(x.device, "usaf_rms_norm_fwd", ptr(xr), ldx, ptr(rr), ldr, ptr(weight), _lib.dtype_code(x.dtype),
             _lib.dtype_code(weight.dtype), n, H, float(eps), None if rr is None else ptr(total), ptr(y), ptr(rstd))
     return y, rstd, total
 
@@ -91,8 +96,7 @@ def rms_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, r
     :func:`rms_norm_forward`.  ``dsum``, the gradient of ``total`` where it is
     used further, is added to ``dx``, which is then the gradient of ``x`` and of
     ``residual`` alike.  ``dw`` has the weight's type (None unless wanted)."""
-    dtc = _check(x, weight)
-    H = x.shape[-1]
+    H = _check(x, weight)
     n = x.numel() // H
     _check_like("dy", dy, x)
     if rstd.numel() != n or rstd.dtype != torch.float32 or rstd.device != x.device or not rstd.is_contiguous():
@@ -103,14 +107,13 @@ def rms_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, r
     if dsum is not None:
         _check_like("dsum", dsum, x)
         dsr, ldds = _rows(dsum)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dx = _dense_like(x)
     dw = ws = None
     if want_dw:
         dw = torch.empty_like(weight)
-        ws = torch.empty(max(int(_lib.LIB.usaf_rms_norm_workspace_bytes(n, H)), 16), dtype=torch.uint8,
-                         device=x.device)
-    call_on(x.device, "usaf_rms_norm_bwd", ptr(dyr), lddy, ptr(xr), ldx, ptr(weight), ptr(rstd), ptr(dsr), ldds, dtc,
-            _lib.dtype_code(weight.dtype), n, H, ptr(dx), ptr(dw), ptr(ws))
+        ws = x.new_empty(_lib.LIB.usaf_rms_norm_workspace_bytes(n, H), dtype=torch.uint8)
+    call_on(x.device, "usaf_rms_norm_bwd", ptr(dyr), lddy, ptr(xr), ldx, ptr(weight), ptr(rstd), ptr(dsr), ldds,
+            _lib.dtype_code(x.dtype), _lib.dtype_code(weight.dtype), n, H, ptr(dx), ptr(dw), ptr(ws))
     return dx, dw
 
 
