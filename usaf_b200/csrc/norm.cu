@@ -26,49 +26,187 @@ template <int NT> __device__ __forceinline__ float block_sum(float v, float *red
     return s;
 }
 
-// ---- rows in registers --------------------------------------------------------
+// ---- rows of whole 16-byte vectors ------------------------------------------------
 // `tpr` threads (a power of two up to 32, or whole warps) hold one row, NV
-// vectors of VN values each: vector i of thread t is columns (i tpr + t) VN ...,
-// so that every load of a warp is contiguous.  A CTA holds blockDim / tpr rows
-// at a time and walks down the rows with the weight kept in registers, each row
-// read once.
-template <typename T, int VN> struct alignas(sizeof(T) * VN) Vec { T v[VN]; };
+// vectors of 16 bytes each: vector i of thread t is the row's vector i tpr + t, so
+// that every load of a warp is contiguous.  A CTA holds blockDim / tpr rows at a
+// time and walks down the rows with the weight in registers.
+//
+// A row costs few bytes and many instructions (counted: the first form of these
+// kernels issued 45 a value in the backward pass and was bound by that), so
+// products run in pairs (f32x2), 16-bit values are taken apart by a shift and a
+// mask and put together two at a time, and addresses are carried along.
 
-template <typename T, int VN> __device__ __forceinline__ Vec<T, VN> load_vec(const T *p) {
-    Vec<T, VN> r;
-    constexpr int B = sizeof(T) * VN;
-    if constexpr (B >= 16) {                 // 16 bytes a load (fp32 weights of 8 values: two)
-#pragma unroll
-        for (int i = 0; i < B / 16; ++i)
-            reinterpret_cast<uint4 *>(&r)[i] = reinterpret_cast<const uint4 *>(p)[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < VN; ++i) r.v[i] = p[i];
-    }
+// two fp32 values in one register pair
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 halves(uint64_t p) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
+    return f;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
     return r;
 }
 
-template <typename T, int VN> __device__ __forceinline__ void store_vec(T *p, const Vec<T, VN> &r) {
-    if constexpr (sizeof(T) * VN == 16) *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(&r);
-    else
+// 16 bytes of T as pairs, and back (rounded to the nearest)
+template <typename T> constexpr int kPairs = 8 / (int)sizeof(T);
+
+__device__ __forceinline__ uint64_t unpack_word(uint32_t u, __nv_bfloat16) {
+    return pair(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+__device__ __forceinline__ uint64_t unpack_word(uint32_t u, __half) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u));
+    return pair(f.x, f.y);
+}
+__device__ __forceinline__ uint32_t pack_word(float2 f, __nv_bfloat16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t pack_word(float2 f, __half) {
+    const __half2 h = __floats2half2_rn(f.x, f.y);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <typename T> __device__ __forceinline__ void unpack(const uint4 &u, uint64_t *p) {
+    if constexpr (sizeof(T) == 4) {
+        p[0] = pair(__uint_as_float(u.x), __uint_as_float(u.y));
+        p[1] = pair(__uint_as_float(u.z), __uint_as_float(u.w));
+    } else {
+        p[0] = unpack_word(u.x, T());
+        p[1] = unpack_word(u.y, T());
+        p[2] = unpack_word(u.z, T());
+        p[3] = unpack_word(u.w, T());
+    }
+}
+template <typename T> __device__ __forceinline__ uint4 pack(const uint64_t *p) {
+    if constexpr (sizeof(T) == 4) {
+        const float2 a = halves(p[0]), b = halves(p[1]);
+        return make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y));
+    } else {
+        return make_uint4(pack_word(halves(p[0]), T()), pack_word(halves(p[1]), T()), pack_word(halves(p[2]), T()),
+                          pack_word(halves(p[3]), T()));
+    }
+}
+// the weight of the columns of one vector of rows
+template <typename T, typename W> __device__ __forceinline__ void load_weight(const W *w, uint64_t *p) {
+    constexpr int N = 2 * kPairs<T>;
+    uint4 u[N * sizeof(W) / 16];
 #pragma unroll
-        for (int i = 0; i < VN; ++i) p[i] = r.v[i];
+    for (int i = 0; i < (int)(N * sizeof(W) / 16); ++i) u[i] = __ldg(reinterpret_cast<const uint4 *>(w) + i);
+#pragma unroll
+    for (int i = 0; i < (int)(N * sizeof(W) / 16); ++i) unpack<W>(u[i], p + i * kPairs<W>);
 }
 
-// sum over the row's threads, in the same order for each of them; `red` holds
-// a value per warp, and rows alternate between two of them so that one barrier
-// a row is enough
-__device__ __forceinline__ float row_sum(float v, int tpr, int group, float *red) {
-    for (int o = min(tpr, 32) >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+// Sum over the row's threads, the same bits for each of them.  `red` holds 16
+// values a group, those behind its warps zero; rows alternate between two of
+// them, so that one barrier a row is enough.
+__device__ __forceinline__ float row_sum(float v, int tpr, int group, float (*red)[16]) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        if (o < tpr) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (tpr > 32) {
-        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+        if ((threadIdx.x & 31) == 0) red[group][(threadIdx.x - group * tpr) >> 5] = v;
         asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(tpr) : "memory");
-        const int n = tpr >> 5;
         v = 0.0f;
-        for (int i = 0; i < n; ++i) v += red[group * n + i];
+        for (int i = 0; i * 128 < tpr; ++i) {
+            const float4 q = *reinterpret_cast<const float4 *>(&red[group][4 * i]);
+            v += (q.x + q.y) + (q.z + q.w);
+        }
     }
     return v;
 }
+
+// Rows ahead: NT tensors' rows come through a ring in shared memory that every
+// thread fills for itself by asynchronous copies: it has D - 1 rows' vectors on
+// their way and reads back only what it copied, so no barrier and no register is
+// spent on them.  12 slots of 16 bytes a thread are 1024 threads' share of an
+// SM's shared memory.  A slot's 16 bytes of neighbouring threads lie side by side:
+// with each thread's slots together instead, the copies' scattered writes made the
+// forward pass of 8192 x 2048 rows take 28 us instead of 21.
+constexpr int ring_depth(int nv, int tensors) {
+    const int d = 12 / (nv * tensors);
+    return d > 6 ? 6 : d < 2 ? 2 : d;
+}
+constexpr int ring_slots(int nv, int tensors) { return ring_depth(nv, tensors) * nv * tensors; }
+
+template <typename T, int NV, int NT> struct RowRing {
+    static constexpr int D = ring_depth(NV, NT);
+    const char *p[NT];           // this thread's first vector of the next row to fetch
+    int64_t ahead[NT];           // bytes from a turn's row to the next turn's
+    int64_t row, step, rows;     // the next row to fetch
+    uint32_t base, in_at, out_at, slot;   // slot: bytes of a slot of all threads
+    int hop;                     // bytes between a thread's vectors
+    uint32_t has;                // bit i: vector i lies in the row
+
+    __device__ __forceinline__ void open(uint4 *dyn, int tpr, int t, int H, int64_t first, int64_t step_, int64_t rows_) {
+        row = first;
+        step = step_;
+        rows = rows_;
+        hop = tpr * 16;
+        has = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if ((i * tpr + t) * 2 * kPairs<T> < H) has |= 1u << i;
+        base = in_at = out_at = (uint32_t)__cvta_generic_to_shared(dyn + threadIdx.x);
+        slot = blockDim.x * 16;
+    }
+    __device__ __forceinline__ void tensor(int k, const void *q, int64_t ld, int t) {
+        p[k] = static_cast<const char *>(q) + row * ld * (int64_t)sizeof(T) + t * 16;
+        ahead[k] = step * ld * (int64_t)sizeof(T);
+    }
+    __device__ __forceinline__ uint32_t next(uint32_t at) const {
+        return at == base + (D - 1) * NV * NT * slot ? base : at + NV * NT * slot;
+    }
+    __device__ __forceinline__ void fetch() {
+        if (row < rows) {
+#pragma unroll
+            for (int k = 0; k < NT; ++k)
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+                    if (has >> i & 1)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(in_at + (k * NV + i) * slot),
+                                     "l"(p[k] + i * hop)
+                                     : "memory");
+        }
+#pragma unroll
+        for (int k = 0; k < NT; ++k) p[k] += ahead[k];
+        row += step;
+        in_at = next(in_at);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    __device__ __forceinline__ void fill() {
+#pragma unroll
+        for (int d = 0; d < D - 1; ++d) fetch();
+    }
+    // one more row on its way, the turn's row is there
+    __device__ __forceinline__ void turn() {
+        fetch();
+        asm volatile("cp.async.wait_group %0;" ::"n"(D - 1) : "memory");
+    }
+    __device__ __forceinline__ uint4 get(int k, int i) const {
+        uint4 u;
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+                     : "r"(out_at + (k * NV + i) * slot));
+        return u;
+    }
+    __device__ __forceinline__ void done() { out_at = next(out_at); }
+};
 
 struct NormFwd {
     const void *x; int64_t ldx;
@@ -87,237 +225,169 @@ struct NormBwd {
     void *dx, *dw; float *part;
 };
 
-// ---- rows ahead -----------------------------------------------------------------
-// Aligned rows come through a ring in shared memory that every thread fills for
-// itself by asynchronous copies: a thread has D - 1 rows' vectors on their way
-// and reads back only what it copied, so no barrier and no register is spent on
-// them.  384 bytes a thread keep about 100 KB in flight on an SM.
-__device__ __forceinline__ void copy_ahead(uint32_t to, const void *from) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
-}
-__device__ __forceinline__ uint4 ring_read(uint32_t at) {
-    uint4 u;
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(at));
-    return u;
-}
-constexpr int ring_depth(int nv, int tensors) {
-    const int d = 12 / (nv * tensors);
-    return d > 6 ? 6 : d < 2 ? 2 : d;
-}
-
-// NT tensors' rows of one thread: `p[k]`, `ld[k]`; vector i of the row of turn n
-template <typename T, int VN, int NV, int NT> struct RowRing {
-    static constexpr int D = ring_depth(NV, NT);
-    const T *p[NT];
-    int64_t ld[NT];
-    uint32_t base;               // this thread's 16 bytes of the first slot
-    int tpr, t, H;
-    int64_t rows;
-
-    __device__ __forceinline__ uint32_t slot(int stage, int k, int i) const {
-        return base + (uint32_t)(((stage * NT + k) * NV + i) * blockDim.x) * 16u;
-    }
-    __device__ __forceinline__ void fetch(int stage, int64_t row) const {
-        if (row < rows) {
-#pragma unroll
-            for (int k = 0; k < NT; ++k)
-#pragma unroll
-                for (int i = 0; i < NV; ++i) {
-                    const int c = (i * tpr + t) * VN;
-                    if (c < H) copy_ahead(slot(stage, k, i), p[k] + row * ld[k] + c);
-                }
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    }
-    __device__ __forceinline__ static void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(D - 1) : "memory"); }
-    // vector i of tensor k: from the ring, or for single values from memory
-    __device__ __forceinline__ Vec<T, VN> get(int stage, int k, int i, int64_t row) const {
-        Vec<T, VN> v;
-        if constexpr (VN > 1) *reinterpret_cast<uint4 *>(&v) = ring_read(slot(stage, k, i));
-        else v.v[0] = p[k][row * ld[k] + i * tpr + t];
-        return v;
-    }
-};
-
-template <typename T, typename W, int VN, int NV, bool RES>
+template <typename T, typename W, int NV, bool RES>
 __global__ void __launch_bounds__(kNormMaxBlock) norm_fwd_rows(const NormFwd a, int tpr) {
-    __shared__ float red[2][32];
+    __shared__ alignas(16) float red[2][8][16];
     extern __shared__ uint4 dyn[];
+    constexpr int N2 = kPairs<T>;
     const int group = threadIdx.x / tpr, t = threadIdx.x - group * tpr, groups = blockDim.x / tpr;
-    using Ring = RowRing<T, VN, NV, RES ? 2 : 1>;
-    Ring ring;
-    ring.p[0] = static_cast<const T *>(a.x);
-    ring.ld[0] = a.ldx;
-    if constexpr (RES) {
-        ring.p[1] = static_cast<const T *>(a.res);
-        ring.ld[1] = a.ldr;
-    }
-    ring.base = (uint32_t)__cvta_generic_to_shared(dyn + threadIdx.x);
-    ring.tpr = tpr;
-    ring.t = t;
-    ring.H = a.H;
-    ring.rows = a.rows;
+    for (int i = threadIdx.x; i < 256; i += blockDim.x) (&red[0][0][0])[i] = 0.0f;
+    __syncthreads();
     const int64_t step = (int64_t)gridDim.x * groups;
-    const int64_t start = (int64_t)blockIdx.x * groups;
-    if constexpr (VN > 1)
+    int64_t row = (int64_t)blockIdx.x * groups + group;
+    RowRing<T, NV, RES ? 2 : 1> ring;
+    ring.open(dyn, tpr, t, a.H, row, step, a.rows);
+    ring.tensor(0, a.x, a.ldx, t);
+    if constexpr (RES) ring.tensor(1, a.res, a.ldr, t);
+    ring.fill();
+    uint64_t w[NV][N2];
 #pragma unroll
-        for (int d = 0; d < Ring::D - 1; ++d) ring.fetch(d, start + d * step + group);
-    Vec<W, VN> wv[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (i * tpr + t) * VN;
-        if (c < a.H) wv[i] = load_vec<W, VN>(static_cast<const W *>(a.w) + c);
-    }
+    for (int i = 0; i < NV; ++i)
+        if (ring.has >> i & 1) load_weight<T, W>(static_cast<const W *>(a.w) + (i * tpr + t) * 2 * N2, w[i]);
     const float inv_h = 1.0f / (float)a.H;
-    int flip = 0, stage = 0;
+    const int64_t out = step * a.H * (int64_t)sizeof(T);
+    char *y = static_cast<char *>(a.y) + row * a.H * (int64_t)sizeof(T) + t * 16;
+    char *sum = RES ? static_cast<char *>(a.sum) + row * a.H * (int64_t)sizeof(T) + t * 16 : nullptr;
+    int flip = 0;
     // every thread takes every turn: the shuffles and barriers are for whole groups
-    for (int64_t base = start; base < a.rows; base += step) {
-        const int64_t row = base + group;
+    for (int64_t base = (int64_t)blockIdx.x * groups; base < a.rows; base += step) {
         const bool in = row < a.rows;
-        if constexpr (VN > 1) {
-            ring.fetch(stage == 0 ? Ring::D - 1 : stage - 1, row + (Ring::D - 1) * step);
-            Ring::wait();
-        }
-        Vec<T, VN> v[NV];
-        float ss = 0.0f;
+        ring.turn();
+        uint4 v[NV];
+        uint64_t ss = 0;
         if (in) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const int c = (i * tpr + t) * VN;
-                if (c < a.H) {
-                    v[i] = ring.get(stage, 0, i, row);
+                if (ring.has >> i & 1) {
+                    uint64_t x[N2];
+                    v[i] = ring.get(0, i);
+                    unpack<T>(v[i], x);
                     if constexpr (RES) {
-                        const Vec<T, VN> q = ring.get(stage, RES ? 1 : 0, i, row);
+                        uint64_t q[N2];
+                        unpack<T>(ring.get(RES ? 1 : 0, i), q);
 #pragma unroll
-                        for (int k = 0; k < VN; ++k) v[i].v[k] = from_f<T>(to_f(v[i].v[k]) + to_f(q.v[k]));
-                        store_vec<T, VN>(static_cast<T *>(a.sum) + row * a.H + c, v[i]);
+                        for (int k = 0; k < N2; ++k) q[k] = add2(x[k], q[k]);
+                        v[i] = pack<T>(q);
+                        *reinterpret_cast<uint4 *>(sum + i * ring.hop) = v[i];
+                        unpack<T>(v[i], x);
                     }
 #pragma unroll
-                    for (int k = 0; k < VN; ++k) ss = fmaf(to_f(v[i].v[k]), to_f(v[i].v[k]), ss);
+                    for (int k = 0; k < N2; ++k) ss = fma2(x[k], x[k], ss);
                 }
             }
         }
-        ss = row_sum(ss, tpr, group, red[flip]);
+        const float2 h = halves(ss);
+        const float r = __frcp_rn(__fsqrt_rn(row_sum(h.x + h.y, tpr, group, red[flip]) * inv_h + a.eps));
         flip ^= 1;
-        stage = stage == Ring::D - 1 ? 0 : stage + 1;
-        const float r = __frcp_rn(__fsqrt_rn(ss * inv_h + a.eps));
+        ring.done();
         if (in) {
             if (a.rstd && t == 0) a.rstd[row] = r;
+            const uint64_t r2 = pair(r, r);
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const int c = (i * tpr + t) * VN;
-                if (c < a.H) {
-                    Vec<T, VN> o;
+                if (ring.has >> i & 1) {
+                    uint64_t x[N2];
+                    unpack<T>(v[i], x);
 #pragma unroll
-                    for (int k = 0; k < VN; ++k) o.v[k] = from_f<T>(to_f(v[i].v[k]) * r * to_f(wv[i].v[k]));
-                    store_vec<T, VN>(static_cast<T *>(a.y) + row * a.H + c, o);
+                    for (int k = 0; k < N2; ++k) x[k] = mul2(mul2(x[k], r2), w[i][k]);
+                    *reinterpret_cast<uint4 *>(y + i * ring.hop) = pack<T>(x);
                 }
             }
         }
+        row += step;
+        y += out;
+        if constexpr (RES) sum += out;
     }
 }
 
-template <typename T, typename W, int VN, int NV, bool DSUM, bool DW>
+template <typename T, typename W, int NV, bool DSUM, bool DW>
 __global__ void __launch_bounds__(kNormMaxBlock) norm_bwd_rows(const NormBwd a, int tpr) {
-    __shared__ float red[2][32];
+    __shared__ alignas(16) float red[2][8][16];
     extern __shared__ uint4 dyn[];           // the ring; at the end [groups][H] sums, where a CTA has several rows
+    constexpr int N2 = kPairs<T>;
     const int group = threadIdx.x / tpr, t = threadIdx.x - group * tpr, groups = blockDim.x / tpr;
-    using Ring = RowRing<T, VN, NV, DSUM ? 3 : 2>;
-    Ring ring;
-    ring.p[0] = static_cast<const T *>(a.x);
-    ring.ld[0] = a.ldx;
-    ring.p[1] = static_cast<const T *>(a.dy);
-    ring.ld[1] = a.lddy;
-    if constexpr (DSUM) {
-        ring.p[2] = static_cast<const T *>(a.dsum);
-        ring.ld[2] = a.ldds;
-    }
-    ring.base = (uint32_t)__cvta_generic_to_shared(dyn + threadIdx.x);
-    ring.tpr = tpr;
-    ring.t = t;
-    ring.H = a.H;
-    ring.rows = a.rows;
+    for (int i = threadIdx.x; i < 256; i += blockDim.x) (&red[0][0][0])[i] = 0.0f;
+    __syncthreads();
     const int64_t step = (int64_t)gridDim.x * groups;
-    const int64_t start = (int64_t)blockIdx.x * groups;
-    if constexpr (VN > 1)
-#pragma unroll
-        for (int d = 0; d < Ring::D - 1; ++d) ring.fetch(d, start + d * step + group);
-    Vec<W, VN> wv[NV];
-    float acc[DW ? NV : 1][VN];
+    int64_t row = (int64_t)blockIdx.x * groups + group;
+    RowRing<T, NV, DSUM ? 3 : 2> ring;
+    ring.open(dyn, tpr, t, a.H, row, step, a.rows);
+    ring.tensor(0, a.x, a.ldx, t);
+    ring.tensor(1, a.dy, a.lddy, t);
+    if constexpr (DSUM) ring.tensor(2, a.dsum, a.ldds, t);
+    ring.fill();
+    uint64_t w[NV][N2], acc[DW ? NV : 1][N2];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int c = (i * tpr + t) * VN;
-        if (c < a.H) wv[i] = load_vec<W, VN>(static_cast<const W *>(a.w) + c);
+        if (ring.has >> i & 1) load_weight<T, W>(static_cast<const W *>(a.w) + (i * tpr + t) * 2 * N2, w[i]);
         if constexpr (DW)
 #pragma unroll
-            for (int k = 0; k < VN; ++k) acc[i][k] = 0.0f;
+            for (int k = 0; k < N2; ++k) acc[i][k] = 0;
     }
     const float inv_h = 1.0f / (float)a.H;
-    int flip = 0, stage = 0;
-    float r = start + group < a.rows ? a.rstd[start + group] : 0.0f;
-    for (int64_t base = start; base < a.rows; base += step) {
-        const int64_t row = base + group;
+    const int64_t out = step * a.H * (int64_t)sizeof(T);
+    char *dx = static_cast<char *>(a.dx) + row * a.H * (int64_t)sizeof(T) + t * 16;
+    int flip = 0;
+    float r = row < a.rows ? a.rstd[row] : 0.0f;
+    for (int64_t base = (int64_t)blockIdx.x * groups; base < a.rows; base += step) {
         const bool in = row < a.rows;
-        const float r_next = row + step < a.rows ? a.rstd[row + step] : 0.0f;
-        if constexpr (VN > 1) {
-            ring.fetch(stage == 0 ? Ring::D - 1 : stage - 1, row + (Ring::D - 1) * step);
-            Ring::wait();
-        }
-        float dot = 0.0f;
+        row += step;
+        const float r_next = row < a.rows ? a.rstd[row] : 0.0f;
+        ring.turn();
+        const uint64_t r2 = pair(r, r);
+        uint64_t dot = 0;
         if (in) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const int c = (i * tpr + t) * VN;
-                if (c < a.H) {
-                    const Vec<T, VN> x = ring.get(stage, 0, i, row), d = ring.get(stage, 1, i, row);
+                if (ring.has >> i & 1) {
+                    uint64_t x[N2], d[N2];
+                    unpack<T>(ring.get(0, i), x);
+                    unpack<T>(ring.get(1, i), d);
 #pragma unroll
-                    for (int k = 0; k < VN; ++k) {
-                        dot = fmaf(to_f(d.v[k]) * to_f(wv[i].v[k]), to_f(x.v[k]), dot);
-                        if constexpr (DW) acc[i][k] = fmaf(to_f(d.v[k]), to_f(x.v[k]) * r, acc[i][k]);
+                    for (int k = 0; k < N2; ++k) {
+                        dot = fma2(mul2(d[k], w[i][k]), x[k], dot);
+                        if constexpr (DW) acc[i][k] = fma2(d[k], mul2(x[k], r2), acc[i][k]);
                     }
                 }
             }
         }
+        const float2 h = halves(dot);
         // hat c = s r mean(g s r): s times this
-        const float along = row_sum(dot, tpr, group, red[flip]) * inv_h * r * r * r;
+        const float along = row_sum(h.x + h.y, tpr, group, red[flip]) * inv_h * r * r * r;
         flip ^= 1;
         if (in) {
+            const uint64_t back = pair(-along, -along);
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const int c = (i * tpr + t) * VN;
-                if (c < a.H) {               // read again: cheaper than the registers to keep them
-                    const Vec<T, VN> x = ring.get(stage, 0, i, row), d = ring.get(stage, 1, i, row);
-                    Vec<T, VN> o;
-                    float v[VN];
+                if (ring.has >> i & 1) {     // read again: cheaper than the registers to keep them
+                    uint64_t x[N2], d[N2];
+                    unpack<T>(ring.get(0, i), x);
+                    unpack<T>(ring.get(1, i), d);
 #pragma unroll
-                    for (int k = 0; k < VN; ++k)
-                        v[k] = fmaf(to_f(d.v[k]) * to_f(wv[i].v[k]), r, -along * to_f(x.v[k]));
+                    for (int k = 0; k < N2; ++k) x[k] = fma2(mul2(d[k], w[i][k]), r2, mul2(x[k], back));
                     if constexpr (DSUM) {
-                        const Vec<T, VN> s = ring.get(stage, DSUM ? 2 : 0, i, row);
+                        unpack<T>(ring.get(DSUM ? 2 : 0, i), d);
 #pragma unroll
-                        for (int k = 0; k < VN; ++k) v[k] += to_f(s.v[k]);
+                        for (int k = 0; k < N2; ++k) x[k] = add2(x[k], d[k]);
                     }
-#pragma unroll
-                    for (int k = 0; k < VN; ++k) o.v[k] = from_f<T>(v[k]);
-                    store_vec<T, VN>(static_cast<T *>(a.dx) + row * a.H + c, o);
+                    *reinterpret_cast<uint4 *>(dx + i * ring.hop) = pack<T>(x);
                 }
             }
         }
-        stage = stage == Ring::D - 1 ? 0 : stage + 1;
+        ring.done();
+        dx += out;
         r = r_next;
     }
     if constexpr (DW) {
         float *part = a.part + (int64_t)blockIdx.x * a.H, *fold = reinterpret_cast<float *>(dyn);
-        float *to = groups > 1 ? fold + (int64_t)group * a.H : part;
+        float *to = (groups > 1 ? fold + group * a.H : part) + t * 2 * N2;
         asm volatile("cp.async.wait_all;" ::: "memory");
         __syncthreads();                     // the ring is read; its space takes the sums
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (i * tpr + t) * VN;
-            if (c < a.H)
+        for (int i = 0; i < NV; ++i)
+            if (ring.has >> i & 1)
 #pragma unroll
-                for (int k = 0; k < VN; ++k) to[c + k] = acc[i][k];
-        }
+                for (int k = 0; k < N2; ++k) reinterpret_cast<float2 *>(to + i * tpr * 2 * N2)[k] = halves(acc[i][k]);
         if (groups > 1) {
             __syncthreads();
             for (int c = threadIdx.x; c < a.H; c += blockDim.x) {
@@ -405,23 +475,19 @@ __global__ void __launch_bounds__(1024) norm_dw_kernel(const float *__restrict__
     if (lane == 0 && blockIdx.x * 32 + k < H) dw[blockIdx.x * 32 + k] = from_f<W>(v);
 }
 
-// How the rows are cut: vectors of 16 bytes where every row starts on a 16-byte
-// boundary, else single values; NV vectors a thread, threads a row, threads a CTA.
+// How rows of n 16-byte vectors are cut: vectors a thread, threads a row, threads
+// a CTA.  Two vectors a thread let the work of a turn (addresses, the sum over
+// the threads) serve 32 bytes; four only where two would take more than a CTA.
 struct RowPlan {
-    int vn, nv, tpr, block;
+    int nv, tpr, block;
 };
 
-template <typename T> static RowPlan plan_rows(int H, bool aligned) {
-    RowPlan p{aligned ? 16 / (int)sizeof(T) : 1, 8, 0, 0};
-    const int n = (H + p.vn - 1) / p.vn;     // vectors of a row
-    if (aligned) p.nv = n <= 4 ? 1 : n <= 2 * kNormMaxBlock ? 2 : 4;
+static RowPlan plan_rows(int n) {
+    RowPlan p{n <= 4 ? 1 : n <= 2 * kNormMaxBlock ? 2 : 4, 1, 0};
     const int t = (n + p.nv - 1) / p.nv;
-    if (t > 32) {
-        p.tpr = (t + 31) / 32 * 32;
-    } else {
-        p.tpr = 1;
+    if (t > 32) p.tpr = (t + 31) / 32 * 32;
+    else
         while (p.tpr < t) p.tpr *= 2;
-    }
     p.block = p.tpr >= 256 ? p.tpr : 256 / p.tpr * p.tpr;
     if (p.tpr > kNormMaxBlock) p.nv = 0;     // too wide for a CTA's registers
     return p;
@@ -432,48 +498,41 @@ static bool on16(const void *p, int64_t ld_bytes) { return ((uintptr_t)p | (uint
 // CTAs that fit the SMs at once by shared memory and `regs` registers a thread,
 // or fewer where the rows are fewer
 static int row_grid(const RowPlan &p, int smem, int regs, int64_t rows, int most) {
-    const int per_sm = std::max(1, std::min({227 * 1024 / (smem + 1024 + 256), 65536 / (regs * p.block),
-                                             2048 / p.block}));
+    const int per_sm = std::max(1, std::min({227 * 1024 / (smem + 2048), 65536 / (regs * p.block), 2048 / p.block}));
     const int groups = p.block / p.tpr;
     return (int)std::min<int64_t>((rows + groups - 1) / groups, std::min(148 * per_sm, most));
 }
 
 template <typename K> static bool allow_smem(K kernel, int smem) {
-    if (smem + 256 <= 48 * 1024 ||       // 256 bytes are the reduction's
+    if (smem + 1024 <= 48 * 1024 ||          // the reductions take up to 1024 bytes more
         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess)
         return true;
     (void)cudaGetLastError();
     return false;
 }
 
-template <typename T, typename W, int VN, int NV, bool RES>
+template <typename T, typename W, int NV, bool RES>
 static int fwd_launch(const NormFwd &a, const RowPlan &p, cudaStream_t st) {
-    constexpr int NT = RES ? 2 : 1;
-    const int smem = VN > 1 ? NV * NT * ring_depth(NV, NT) * 16 * p.block : 0;
-    if (!allow_smem(norm_fwd_rows<T, W, VN, NV, RES>, smem)) return USAF_ECUDA;
+    const int smem = ring_slots(NV, RES ? 2 : 1) * 16 * p.block;
+    if (!allow_smem(norm_fwd_rows<T, W, NV, RES>, smem)) return USAF_ECUDA;
     const int grid = row_grid(p, smem, NV == 4 ? 128 : 64, a.rows, 1 << 30);
-    norm_fwd_rows<T, W, VN, NV, RES><<<grid, p.block, smem, st>>>(a, p.tpr);
+    norm_fwd_rows<T, W, NV, RES><<<grid, p.block, smem, st>>>(a, p.tpr);
     USAF_CHECK_LAUNCH();
     return USAF_OK;
 }
 
-template <typename T, typename W, int VN, int NV>
-static int fwd_launch(const NormFwd &a, const RowPlan &p, cudaStream_t st) {
-    return a.res ? fwd_launch<T, W, VN, NV, true>(a, p, st) : fwd_launch<T, W, VN, NV, false>(a, p, st);
+template <typename T, typename W, int NV> static int fwd_launch(const NormFwd &a, const RowPlan &p, cudaStream_t st) {
+    return a.res ? fwd_launch<T, W, NV, true>(a, p, st) : fwd_launch<T, W, NV, false>(a, p, st);
 }
 
 template <typename T, typename W> static int norm_fwd(const NormFwd &a, cudaStream_t st) {
-    constexpr int N = 16 / (int)sizeof(T);
-    const int64_t row = (int64_t)a.H * sizeof(T);
-    const bool aligned = on16(a.x, a.ldx * sizeof(T)) && on16(a.y, row) && on16(a.w, 0) &&
-                         (!a.res || (on16(a.res, a.ldr * sizeof(T)) && on16(a.sum, row)));
-    const RowPlan p = plan_rows<T>(a.H, aligned);
-    if (p.vn > 1) {
-        if (p.nv == 1) return fwd_launch<T, W, N, 1>(a, p, st);
-        if (p.nv == 2) return fwd_launch<T, W, N, 2>(a, p, st);
-        if (p.nv == 4) return fwd_launch<T, W, N, 4>(a, p, st);
-    } else if (p.nv) {
-        return fwd_launch<T, W, 1, 8>(a, p, st);
+    const int64_t bytes = (int64_t)a.H * sizeof(T);
+    if (on16(a.x, a.ldx * sizeof(T)) && on16(a.y, bytes) && on16(a.w, 0) &&
+        (!a.res || (on16(a.res, a.ldr * sizeof(T)) && on16(a.sum, 0)))) {
+        const RowPlan p = plan_rows((int)(bytes / 16));
+        if (p.nv == 1) return fwd_launch<T, W, 1>(a, p, st);
+        if (p.nv == 2) return fwd_launch<T, W, 2>(a, p, st);
+        if (p.nv == 4) return fwd_launch<T, W, 4>(a, p, st);
     }
     const unsigned grid = (unsigned)std::min<int64_t>(a.rows, 148 * 8);
     norm_fwd_any<T, W><<<grid, 256, 0, st>>>((const T *)a.x, a.ldx, (const T *)a.res, a.ldr, (const W *)a.w, a.rows,
@@ -482,45 +541,36 @@ template <typename T, typename W> static int norm_fwd(const NormFwd &a, cudaStre
     return USAF_OK;
 }
 
-// the partial rows of a launch: P of them
-template <typename T, typename W, int VN, int NV, bool DSUM, bool DW>
+// the launches write P partial rows of dw
+template <typename T, typename W, int NV, bool DSUM, bool DW>
 static int bwd_launch(const NormBwd &a, const RowPlan &p, int *P, cudaStream_t st) {
-    constexpr int NT = DSUM ? 3 : 2;
     const int groups = p.block / p.tpr, fold = DW && groups > 1 ? groups * a.H * 4 : 0;
-    const int smem = std::max(VN > 1 ? NV * NT * ring_depth(NV, NT) * 16 * p.block : 0, fold);
-    if (!allow_smem(norm_bwd_rows<T, W, VN, NV, DSUM, DW>, smem)) return USAF_ECUDA;
-    const int grid = row_grid(p, smem, NV == 4 ? 128 : 64, a.rows, DW ? kNormMaxPartials : 1 << 30);
-    norm_bwd_rows<T, W, VN, NV, DSUM, DW><<<grid, p.block, smem, st>>>(a, p.tpr);
+    const int smem = std::max(ring_slots(NV, DSUM ? 3 : 2) * 16 * p.block, fold);
+    if (!allow_smem(norm_bwd_rows<T, W, NV, DSUM, DW>, smem)) return USAF_ECUDA;
+    const int grid = row_grid(p, smem, NV == 4 ? 128 : 80, a.rows, DW ? kNormMaxPartials : 1 << 30);
+    norm_bwd_rows<T, W, NV, DSUM, DW><<<grid, p.block, smem, st>>>(a, p.tpr);
     USAF_CHECK_LAUNCH();
     *P = grid;
     return USAF_OK;
 }
 
-template <typename T, typename W, int VN, int NV>
+template <typename T, typename W, int NV>
 static int bwd_launch(const NormBwd &a, const RowPlan &p, int *P, cudaStream_t st) {
-    if (a.dw)
-        return a.dsum ? bwd_launch<T, W, VN, NV, true, true>(a, p, P, st) : bwd_launch<T, W, VN, NV, false, true>(a, p, P, st);
-    return a.dsum ? bwd_launch<T, W, VN, NV, true, false>(a, p, P, st) : bwd_launch<T, W, VN, NV, false, false>(a, p, P, st);
+    if (a.dw) return a.dsum ? bwd_launch<T, W, NV, true, true>(a, p, P, st) : bwd_launch<T, W, NV, false, true>(a, p, P, st);
+    return a.dsum ? bwd_launch<T, W, NV, true, false>(a, p, P, st) : bwd_launch<T, W, NV, false, false>(a, p, P, st);
 }
 
 template <typename T, typename W> static int bwd_rows(const NormBwd &a, int *P, cudaStream_t st) {
-    constexpr int N = 16 / (int)sizeof(T);
-    const bool aligned = on16(a.x, a.ldx * sizeof(T)) && on16(a.dy, a.lddy * sizeof(T)) && on16(a.w, 0) &&
-                         on16(a.dx, (int64_t)a.H * sizeof(T)) && (!a.dsum || on16(a.dsum, a.ldds * sizeof(T)));
-    const RowPlan p = plan_rows<T>(a.H, aligned);
-    if (p.vn > 1) {
-        if (p.nv == 1) return bwd_launch<T, W, N, 1>(a, p, P, st);
-        if (p.nv == 2) return bwd_launch<T, W, N, 2>(a, p, P, st);
-        if (p.nv == 4) return bwd_launch<T, W, N, 4>(a, p, P, st);
-    } else if (p.nv) {
-        return bwd_launch<T, W, 1, 8>(a, p, P, st);
+    const int64_t bytes = (int64_t)a.H * sizeof(T);
+    if (on16(a.x, a.ldx * sizeof(T)) && on16(a.dy, a.lddy * sizeof(T)) && on16(a.w, 0) && on16(a.dx, bytes) &&
+        on16(a.dw ? a.part : nullptr, 0) && (!a.dsum || on16(a.dsum, a.ldds * sizeof(T)))) {
+        const RowPlan p = plan_rows((int)(bytes / 16));
+        if (p.nv == 1) return bwd_launch<T, W, 1>(a, p, P, st);
+        if (p.nv == 2) return bwd_launch<T, W, 2>(a, p, P, st);
+        if (p.nv == 4) return bwd_launch<T, W, 4>(a, p, P, st);
     }
     const int smem = a.dw ? a.H * 4 : 0;
-    if (smem + 256 > 48 * 1024 && cudaFuncSetAttribute(norm_bwd_any<T, W>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 kNormMaxH * 4) != cudaSuccess) {
-        (void)cudaGetLastError();
-        return USAF_ECUDA;
-    }
+    if (!allow_smem(norm_bwd_any<T, W>, smem)) return USAF_ECUDA;
     *P = (int)std::min<int64_t>(a.rows, kNormMaxPartials);
     norm_bwd_any<T, W><<<*P, 256, smem, st>>>((const T *)a.dy, a.lddy, (const T *)a.x, a.ldx, (const W *)a.w, a.rstd,
                                               (const T *)a.dsum, a.ldds, a.rows, a.H, (T *)a.dx, a.dw ? a.part : nullptr);
