@@ -410,25 +410,20 @@ int usaf_embedding_bwd(const void *dy, const void *ids, int32_t ids_bits, int64_
  * of one dtype, gradients of the same dtype or fp32:
  *   g = grad / grad_div; m = b1 m + (1-b1) g; v = b2 v + (1-b2) g^2;
  *   p = p (1 - lr wd) - lr/(1-b1^step) * m / (sqrt(v)/sqrt(1-b2^step) + eps)
- * `tensors` is a HOST array, read before the call returns.  m, v (and master,
- * the fp32 weights that p is rounded from, or NULL) are flat buffers that all
- * tensors share; tensor i takes numel values from `start`, a multiple of 256.
+ * p, g, numel, start and weight_decay (wd) are HOST arrays, read before the
+ * call returns; the tensors must not share memory.  m, v (and master,
+ * the fp32 weights that p is rounded from, or NULL) are flat buffers, 16-byte
+ * aligned, that all tensors share; tensor i takes numel values from `start`, a multiple of 256.
  * bits 32: m, v fp32.  bits 8: m and sqrt(v) as e4m3 bytes, each group of 256
  * values times m_scale / v_scale [values / 256] (fp32; the group's largest
  * magnitude / 448, 0 for a group below 1e-30); a sqrt(v) above zero is stored
  * as the lowest code at least.  The values between a tensor's end and the next
  * multiple of 256 stay what they are in 32 bits and are written as zeros in 8. */
-typedef struct {
-    void *p;
-    const void *g;
-    int64_t numel;
-    int64_t start;
-    double weight_decay;
-} usaf_adamw_tensor;
-int usaf_adamw(const usaf_adamw_tensor *tensors, int32_t n_tensors, int32_t p_dtype,
-               int32_t g_dtype, float *master, int32_t bits, void *m, void *v, float *m_scale,
-               float *v_scale, double grad_div, int32_t step, double lr, double beta1,
-               double beta2, double eps, void *stream);
+int usaf_adamw(int32_t n_tensors, void *const *p, const void *const *g, const int64_t *numel,
+               const int64_t *start, const double *weight_decay, int32_t p_dtype, int32_t g_dtype,
+               float *master, int32_t bits, void *m, void *v, float *m_scale, float *v_scale,
+               double grad_div, int32_t step, double lr, double beta1, double beta2, double eps,
+               void *stream);
 
 /* ---- expert parallelism ------------------------------------------------------
  * No counterpart in the reference (it runs in a single process).  Plan:

@@ -83,7 +83,7 @@ _SIGS = {
     "usaf_embedding_fwd": (I32, [P, I32, I64, P, I32, I64, I32, F64, P, P, P]),
     "usaf_embedding_workspace_bytes": (I64, [I64, I64, I32]),
     "usaf_embedding_bwd": (I32, [P, P, I32, I64, I32, I64, I32, F64, I64, I32, P, I32, P, P, P]),
-    "usaf_adamw": (I32, [P, I32, I32, I32, P, I32, P, P, P, P, F64, I32, F64, F64, F64, F64, P]),
+    "usaf_adamw": (I32, [I32, P, P, P, P, P, I32, I32, P, I32, P, P, P, P, F64, I32, F64, F64, F64, F64, P]),
     "usaf_version": (C.c_char_p, []),
 }
 

@@ -75,6 +75,31 @@ __device__ __forceinline__ float warp_max(float v) {
     return v;
 }
 
+// A kernel launched with launch_early may be set up while the one before it in
+// the stream still runs (once every CTA of that one has called let_next_start
+// or ended); wait_for_previous returns when the one before has ended and its
+// writes are visible, and comes before the first access to them.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename... Args, typename... Given>
+static inline bool launch_early(void (*kernel)(Args...), dim3 grid, int block, int smem, cudaStream_t st,
+                                Given... given) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, kernel, static_cast<Args>(given)...) == cudaSuccess) return true;
+    (void)cudaGetLastError();
+    return false;
+}
+
 // Effective weight of storage element (e, r, c) of a projection, looked up
 // through the CSR overlay when the coordinate is trained.  Used by the
 // generic (SIMT) paths; the tensor-core kernels patch tiles instead.

@@ -8,6 +8,7 @@
 // partial sums, and a second kernel adds those rows in a fixed order: the
 // result does not depend on timing.
 #include "common.cuh"
+#include "f32x2.cuh"
 
 namespace usaf {
 
@@ -37,71 +38,6 @@ template <int NT> __device__ __forceinline__ float block_sum(float v, float *red
 // products run in pairs (f32x2), 16-bit values are taken apart by a shift and a
 // mask and put together two at a time, and addresses are carried along.
 
-// two fp32 values in one register pair
-__device__ __forceinline__ uint64_t pair(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float2 halves(uint64_t p) {
-    float2 f;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
-    return f;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-
-// 16 bytes of T as pairs, and back (rounded to the nearest)
-template <typename T> constexpr int kPairs = 8 / (int)sizeof(T);
-
-__device__ __forceinline__ uint64_t unpack_word(uint32_t u, __nv_bfloat16) {
-    return pair(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
-}
-__device__ __forceinline__ uint64_t unpack_word(uint32_t u, __half) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u));
-    return pair(f.x, f.y);
-}
-__device__ __forceinline__ uint32_t pack_word(float2 f, __nv_bfloat16) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-__device__ __forceinline__ uint32_t pack_word(float2 f, __half) {
-    const __half2 h = __floats2half2_rn(f.x, f.y);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-template <typename T> __device__ __forceinline__ void unpack(const uint4 &u, uint64_t *p) {
-    if constexpr (sizeof(T) == 4) {
-        p[0] = pair(__uint_as_float(u.x), __uint_as_float(u.y));
-        p[1] = pair(__uint_as_float(u.z), __uint_as_float(u.w));
-    } else {
-        p[0] = unpack_word(u.x, T());
-        p[1] = unpack_word(u.y, T());
-        p[2] = unpack_word(u.z, T());
-        p[3] = unpack_word(u.w, T());
-    }
-}
-template <typename T> __device__ __forceinline__ uint4 pack(const uint64_t *p) {
-    if constexpr (sizeof(T) == 4) {
-        const float2 a = halves(p[0]), b = halves(p[1]);
-        return make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y));
-    } else {
-        return make_uint4(pack_word(halves(p[0]), T()), pack_word(halves(p[1]), T()), pack_word(halves(p[2]), T()),
-                          pack_word(halves(p[3]), T()));
-    }
-}
 // the weight of the columns of one vector of rows
 template <typename T, typename W> __device__ __forceinline__ void load_weight(const W *w, uint64_t *p) {
     constexpr int N = 2 * kPairs<T>;
@@ -138,14 +74,15 @@ __device__ __forceinline__ float row_sum(float v, int tpr, int group, float (*re
 // SM's shared memory.  A slot's 16 bytes of neighbouring threads lie side by side:
 // with each thread's slots together instead, the copies' scattered writes made the
 // forward pass of 8192 x 2048 rows take 28 us instead of 21.
-constexpr int ring_depth(int nv, int tensors) {
-    const int d = 12 / (nv * tensors);
+constexpr int ring_depth(int nv, int tensors, int slots) {
+    const int d = slots / (nv * tensors);
     return d > 6 ? 6 : d < 2 ? 2 : d;
 }
-constexpr int ring_slots(int nv, int tensors) { return ring_depth(nv, tensors) * nv * tensors; }
+constexpr int kFwdSlots = 12, kBwdSlots = 16;   // the backward pass's registers leave 3 CTAs of 256 an SM
+constexpr int ring_slots(int nv, int tensors, int slots) { return ring_depth(nv, tensors, slots) * nv * tensors; }
 
-template <typename T, int NV, int NT> struct RowRing {
-    static constexpr int D = ring_depth(NV, NT);
+template <typename T, int NV, int NT, int SLOTS> struct RowRing {
+    static constexpr int D = ring_depth(NV, NT, SLOTS);
     const char *p[NT];           // this thread's first vector of the next row to fetch
     int64_t ahead[NT];           // bytes from a turn's row to the next turn's
     int64_t row, step, rows;     // the next row to fetch
@@ -235,7 +172,7 @@ __global__ void __launch_bounds__(kNormMaxBlock) norm_fwd_rows(const NormFwd a, 
     __syncthreads();
     const int64_t step = (int64_t)gridDim.x * groups;
     int64_t row = (int64_t)blockIdx.x * groups + group;
-    RowRing<T, NV, RES ? 2 : 1> ring;
+    RowRing<T, NV, RES ? 2 : 1, kFwdSlots> ring;
     ring.open(dyn, tpr, t, a.H, row, step, a.rows);
     ring.tensor(0, a.x, a.ldx, t);
     if constexpr (RES) ring.tensor(1, a.res, a.ldr, t);
@@ -308,9 +245,10 @@ __global__ void __launch_bounds__(kNormMaxBlock) norm_bwd_rows(const NormBwd a, 
     const int group = threadIdx.x / tpr, t = threadIdx.x - group * tpr, groups = blockDim.x / tpr;
     for (int i = threadIdx.x; i < 256; i += blockDim.x) (&red[0][0][0])[i] = 0.0f;
     __syncthreads();
+    if constexpr (DW) let_next_start();
     const int64_t step = (int64_t)gridDim.x * groups;
     int64_t row = (int64_t)blockIdx.x * groups + group;
-    RowRing<T, NV, DSUM ? 3 : 2> ring;
+    RowRing<T, NV, DSUM ? 3 : 2, kBwdSlots> ring;
     ring.open(dyn, tpr, t, a.H, row, step, a.rows);
     ring.tensor(0, a.x, a.ldx, t);
     ring.tensor(1, a.dy, a.lddy, t);
@@ -465,6 +403,7 @@ __global__ void __launch_bounds__(1024) norm_dw_kernel(const float *__restrict__
     __shared__ float s[32][33];
     const int lane = threadIdx.x & 31, k = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     float v = 0.0f;
+    wait_for_previous();
     if (c < H) {
 #pragma unroll 10
         for (int p = k; p < P; p += 32) v += part[(int64_t)p * H + c];
@@ -513,7 +452,7 @@ template <typename K> static bool allow_smem(K kernel, int smem) {
 
 template <typename T, typename W, int NV, bool RES>
 static int fwd_launch(const NormFwd &a, const RowPlan &p, cudaStream_t st) {
-    const int smem = ring_slots(NV, RES ? 2 : 1) * 16 * p.block;
+    const int smem = ring_slots(NV, RES ? 2 : 1, kFwdSlots) * 16 * p.block;
     if (!allow_smem(norm_fwd_rows<T, W, NV, RES>, smem)) return USAF_ECUDA;
     const int grid = row_grid(p, smem, NV == 4 ? 128 : 64, a.rows, 1 << 30);
     norm_fwd_rows<T, W, NV, RES><<<grid, p.block, smem, st>>>(a, p.tpr);
@@ -545,7 +484,7 @@ template <typename T, typename W> static int norm_fwd(const NormFwd &a, cudaStre
 template <typename T, typename W, int NV, bool DSUM, bool DW>
 static int bwd_launch(const NormBwd &a, const RowPlan &p, int *P, cudaStream_t st) {
     const int groups = p.block / p.tpr, fold = DW && groups > 1 ? groups * a.H * 4 : 0;
-    const int smem = std::max(ring_slots(NV, DSUM ? 3 : 2) * 16 * p.block, fold);
+    const int smem = std::max(ring_slots(NV, DSUM ? 3 : 2, kBwdSlots) * 16 * p.block, fold);
     if (!allow_smem(norm_bwd_rows<T, W, NV, DSUM, DW>, smem)) return USAF_ECUDA;
     const int grid = row_grid(p, smem, NV == 4 ? 128 : 80, a.rows, DW ? kNormMaxPartials : 1 << 30);
     norm_bwd_rows<T, W, NV, DSUM, DW><<<grid, p.block, smem, st>>>(a, p.tpr);
@@ -585,8 +524,9 @@ template <typename T, typename W> static int norm_bwd(const NormBwd &a, cudaStre
         if (rc) return rc;
     }
     if (a.dw) {
-        norm_dw_kernel<W><<<cdiv(a.H, 32), 1024, 0, st>>>(a.part, P, a.H, (W *)a.dw);
-        USAF_CHECK_LAUNCH();
+        if (!launch_early(norm_dw_kernel<W>, dim3(cdiv(a.H, 32)), 1024, 0, st, (const float *)a.part, P, a.H,
+                          (W *)a.dw))
+            return USAF_ECUDA;
     }
     return USAF_OK;
 }

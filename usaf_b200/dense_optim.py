@@ -14,19 +14,15 @@ rounded by itself in fp32, in a fixed order.
 """
 from __future__ import annotations
 
-import ctypes
+from array import array
 from typing import Dict, Iterable, List, Optional, Sequence, Tuple, Union
 
-import numpy as np
 import torch
 
 from . import _lib
 from ._lib import call_on, ptr
 
 BLOCK = 256
-
-_TENSOR = np.dtype([("p", np.uint64), ("g", np.uint64), ("numel", np.int64), ("start", np.int64),
-                    ("weight_decay", np.float64)])
 
 Packed = Tuple[torch.Tensor, torch.Tensor]
 
@@ -45,6 +41,8 @@ def _check_flat(name: str, t: torch.Tensor, n: int, dtype: torch.dtype, device: 
     if t.numel() != n or t.dtype != dtype or t.device != device or not t.is_contiguous():
         raise ValueError(f"{name}: expected {n} contiguous {dtype} values on {device}, got {t.numel()} {t.dtype} "
                          f"on {t.device}")
+    if t.data_ptr() % 16:
+        raise ValueError(f"{name}: must start on a 16-byte boundary")
 
 
 def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m: Union[torch.Tensor, Packed],
@@ -62,7 +60,6 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m:
     rounded from.  ``weight_decay``: one value, or one for each tensor.
     ``grad_div`` divides the gradients first.  ``starts`` gives the tensors'
     places when they are not all that the buffers hold."""
-    params, grads = list(params), list(grads)
     n = len(params)
     if len(grads) != n:
         raise ValueError(f"{len(grads)} gradients for {n} parameters")
@@ -76,37 +73,46 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m:
     if n == 0:
         return
     dev, dtype, g_dtype = params[0].device, params[0].dtype, grads[0].dtype
-    if g_dtype not in (dtype, torch.float32):
+    if g_dtype is not dtype and g_dtype is not torch.float32:
         raise TypeError(f"gradients: expected {dtype} or torch.float32, got {g_dtype}")
-    tab = np.zeros(n, dtype=_TENSOR)
-    numels = [p.numel() for p in params]
-    for i, (p, g) in enumerate(zip(params, grads)):
-        if p.dtype != dtype or g.dtype != g_dtype:
+    ptr(params[0])      # on a CUDA device, and so are the others
+    index = dev.index
+    for i, p in enumerate(params):
+        g = grads[i]
+        if p.dtype is not dtype or g.dtype is not g_dtype:
             raise TypeError(f"tensor {i}: {p.dtype} with a gradient of {g.dtype}, the first has {dtype} and {g_dtype}")
-        if p.device != dev or g.device != dev:
+        if p.get_device() != index or g.get_device() != index:
             raise ValueError(f"tensor {i}: expected on {dev}")
-        if g.shape != p.shape or not p.is_contiguous() or not g.is_contiguous():
+        if not (p.is_same_size(g) and p.is_contiguous() and g.is_contiguous()):
             raise ValueError(f"tensor {i}: the parameter and a gradient of its shape must be contiguous")
-    tab["p"] = [ptr(p) for p in params]
-    tab["g"] = [g.data_ptr() for g in grads]
-    tab["numel"] = numels
-    tab["weight_decay"] = weight_decay
-    by_address = tab[tab["numel"] > 0]
-    by_address = by_address[np.argsort(by_address["p"])]
-    ends = by_address["p"] + (by_address["numel"] * params[0].element_size()).astype(np.uint64)
-    if (ends[:-1] > by_address["p"][1:]).any():
-        raise ValueError("a parameter is listed twice, or two share memory")
+    numels = [p.numel() for p in params]
+    at = [p.data_ptr() for p in params]
+    size = params[0].element_size()
+    end = 0
+    for a, k in sorted(zip(at, numels)):
+        if k:
+            if a < end:
+                raise ValueError("a parameter is listed twice, or two share memory")
+            end = a + k * size
     if starts is None:
         places, total = state_layout(numels)
     else:
         places = [int(a) for a in starts]
         total = (m[0] if eight else m).numel()
-        order = sorted(range(n), key=places.__getitem__) if len(places) == n else []
-        ends = [-(-(places[i] + numels[i]) // BLOCK) * BLOCK for i in order]
-        if (not order or places[order[0]] < 0 or ends[-1] > total or any(a % BLOCK for a in places)
-                or any(e > places[i] for e, i in zip(ends, order[1:]))):
+        end = 0
+        for a, k in sorted(zip(places, numels)):
+            if a % BLOCK or a < end:
+                end = -1
+                break
+            end = a + -(-k // BLOCK) * BLOCK
+        if len(places) != n or not 0 <= end <= total:
             raise ValueError("starts: one multiple of 256 for each tensor, within the states, none overlapping")
-    tab["start"] = places
+    decays = [float(weight_decay)] * n if isinstance(weight_decay, (int, float)) else [float(d) for d in weight_decay]
+    if len(decays) != n:
+        raise ValueError(f"{len(decays)} weight decays for {n} parameters")
+    # one host array of each, read before the call returns
+    tab = (array("Q", at), array("Q", [g.data_ptr() for g in grads]), array("q", numels), array("q", places),
+           array("d", decays))
     ms = vs = None
     if eight:
         (m, ms), (v, vs) = m, v
@@ -118,7 +124,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m:
         _check_flat("v", v, total, torch.float32, dev)
     if masters is not None:
         _check_flat("masters", masters, total, torch.float32, dev)
-    call_on(dev, "usaf_adamw", tab.ctypes.data_as(ctypes.c_void_p), n, _lib.dtype_code(dtype),
+    call_on(dev, "usaf_adamw", n, *[a.buffer_info()[0] for a in tab], _lib.dtype_code(dtype),
             _lib.dtype_code(g_dtype), ptr(masters), 8 if eight else 32, ptr(m), ptr(v), ptr(ms), ptr(vs),
             float(grad_div), int(step), float(lr), float(betas[0]), float(betas[1]), float(eps))
 
