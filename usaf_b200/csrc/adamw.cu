@@ -20,13 +20,13 @@ namespace usaf {
 constexpr int kAdamBlock = 256;      // values per scale, and the unit of the tensors' places
 
 struct AdamwConsts {
-    float b1, omb1, b2, omb2, inv_root2, eps, step_size, gmul;
+    float b1, omb1, b2, omb2, inv_root2, eps, step_size, gmul, one;
 };
 
 // the tensors of one launch, passed by value: nothing on the device to keep or to update
 template <int N> struct AdamwTable {
     int32_t n;
-    int32_t first[N + 1];            // first 256-value block of each tensor in this launch
+    int32_t first[N + 1];            // first run of blocks of each tensor in this launch
     void *p[N];
     const void *g[N];
     int64_t numel[N];
@@ -89,92 +89,88 @@ template <typename T> __device__ __forceinline__ void store8(T *p, bool whole, i
     }
 }
 
-// a + b by scalar additions: an f32x2 addition of f32x2 products was fused with
-// them (observed: the weights came out as a fused multiply-add's)
-__device__ __forceinline__ uint64_t sum2(uint64_t a, uint64_t b) {
-    const float2 x = halves(a), y = halves(b);
-    return pair(__fadd_rn(x.x, y.x), __fadd_rn(x.y, y.y));
+// a + b by a multiply-add with a 1 that comes with the launch: f32x2 additions of
+// f32x2 products, and multiply-adds with a known 1, were fused with the products
+// (observed: the weights came out as a fused multiply-add's)
+__device__ __forceinline__ uint64_t sum2(uint64_t a, uint64_t b, float one) { return fma2(a, pair(one, one), b); }
+
+// Root and quotient by an approximation and one corrected step (Markstein's
+// method: the residual of the first result by a fused multiply-add, times the
+// approximate reciprocal), two at a time.  Equal to the correctly rounded ones
+// for every significand (2^24 of each of eleven exponents compared) down to a
+// radicand of 2^-125, below which the residual is too small for a number; with a
+// third of the instructions, which bound the step with 8-bit states.
+__device__ __forceinline__ uint64_t neg2(uint64_t a) { return mul2(a, pair(-1.0f, -1.0f)); }
+__device__ __forceinline__ float rsqrt_approx(float v) {
+    float r;
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return fminf(r, 9.3e18f);        // 2^-126 has 9.2e18; a root of zero is zero times this
+}
+__device__ __forceinline__ float rcp_approx(float v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t root2(uint64_t v) {
+    const float2 w = halves(v);
+    const uint64_t y = pair(rsqrt_approx(w.x), rsqrt_approx(w.y));
+    const uint64_t s = mul2(v, y);
+    return fma2(fma2(neg2(s), s, v), mul2(y, pair(0.5f, 0.5f)), s);
+}
+__device__ __forceinline__ uint64_t quot2(uint64_t a, uint64_t b) {
+    const float2 w = halves(b);
+    const uint64_t y = pair(rcp_approx(w.x), rcp_approx(w.y));
+    const uint64_t q = mul2(a, y);
+    return fma2(fma2(neg2(q), b, a), y, q);
+}
+__device__ __forceinline__ float warp_top(float v) {     // largest magnitude of the warp
+    float r;
+    asm("redux.sync.max.abs.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
 }
 
-// A warp steps one block of 256 values, 8 a lane: every load of a warp is of
-// whole sectors, all of a block's loads are on their way at once, and a block's
-// scales are its lanes' maximum.
-template <int N, typename P, typename G, bool EIGHT, bool MASTER>
-__global__ void __launch_bounds__(256)
-adamw_kernel(const __grid_constant__ AdamwTable<N> tab, const AdamwState s, const AdamwConsts c) {
-    const int b = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (b >= tab.first[tab.n]) return;
-    int lo = 0, hi = tab.n;          // the last tensor that starts at or before this block
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (tab.first[mid] <= b) lo = mid;
-        else hi = mid;
-    }
-    const int64_t rel = b - tab.first[lo], i = rel * kAdamBlock + lane * 8;
-    const int64_t blk = tab.start[lo] + rel, f = blk * kAdamBlock + lane * 8;
-    P *pp = static_cast<P *>(tab.p[lo]) + i;
-    const G *gg = static_cast<const G *>(tab.g[lo]) + i;
-    const int n = (int)max((int64_t)0, min((int64_t)8, tab.numel[lo] - i));
-    const bool whole = n == 8 && (((uintptr_t)pp | (uintptr_t)gg) & 15) == 0;
-    uint64_t p[4], g[4], m[4], v[4];
-    load8<G>(gg, whole, n, g);
-    if (MASTER) load8<float>(s.master + f, true, 8, p);
-    else load8<P>(pp, whole, n, p);
-    if (EIGHT) {
-        const uint2 qm = *reinterpret_cast<const uint2 *>(static_cast<uint8_t *>(s.m) + f);
-        const uint2 qv = *reinterpret_cast<const uint2 *>(static_cast<uint8_t *>(s.v) + f);
-        const float sm = s.m_scale[blk], sv = s.v_scale[blk];
-        unpack_e4m3(qm.x, m);
-        unpack_e4m3(qm.y, m + 2);
-        unpack_e4m3(qv.x, v);
-        unpack_e4m3(qv.y, v + 2);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            m[k] = mul2(m[k], pair(sm, sm));
-            v[k] = mul2(v[k], pair(sv, sv));
-            v[k] = mul2(v[k], v[k]);
-        }
-    } else {
-        load8<float>(static_cast<float *>(s.m) + f, true, 8, m);
-        load8<float>(static_cast<float *>(s.v) + f, true, 8, v);
-    }
-    if (n < 8) {                     // what lies behind a tensor's end takes no part
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float2 a = halves(m[k]), b2 = halves(v[k]);
-            m[k] = pair(2 * k < n ? a.x : 0.0f, 2 * k + 1 < n ? a.y : 0.0f);
-            v[k] = pair(2 * k < n ? b2.x : 0.0f, 2 * k + 1 < n ? b2.y : 0.0f);
-        }
-    }
-    const float keep = tab.keep[lo];
-    uint64_t root[4];
+// the step of 8 values: p, m and v are replaced, root is the new sqrt(v)
+template <bool EIGHT>
+__device__ __forceinline__ void step8(const AdamwConsts &c, float keep, uint64_t *g, uint64_t *p, uint64_t *m,
+                                      uint64_t *v, uint64_t *root) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        g[k] = mul2(g[k], pair(c.gmul, c.gmul));
-        m[k] = sum2(mul2(m[k], pair(c.b1, c.b1)), mul2(g[k], pair(c.omb1, c.omb1)));
-        v[k] = sum2(mul2(v[k], pair(c.b2, c.b2)), mul2(mul2(g[k], pair(c.omb2, c.omb2)), g[k]));
-        const float2 w = halves(v[k]);
-        root[k] = pair(__fsqrt_rn(w.x), __fsqrt_rn(w.y));
-        const float2 den = halves(sum2(mul2(root[k], pair(c.inv_root2, c.inv_root2)), pair(c.eps, c.eps)));
-        const float2 h = halves(m[k]);
-        const uint64_t up = pair(__fdiv_rn(h.x, den.x), __fdiv_rn(h.y, den.y));
-        p[k] = sum2(mul2(p[k], pair(keep, keep)), mul2(up, pair(-c.step_size, -c.step_size)));
-    }
-    store8<P>(pp, whole, n, p);
-    if (n == 8) {
-        if (MASTER) store8<float>(s.master + f, true, 8, p);
-        if (!EIGHT) {
-            store8<float>(static_cast<float *>(s.m) + f, true, 8, m);
-            store8<float>(static_cast<float *>(s.v) + f, true, 8, v);
+        const uint64_t gk = mul2(g[k], pair(c.gmul, c.gmul));
+        m[k] = sum2(mul2(m[k], pair(c.b1, c.b1)), mul2(gk, pair(c.omb1, c.omb1)), c.one);
+        v[k] = sum2(mul2(v[k], pair(c.b2, c.b2)), mul2(mul2(gk, pair(c.omb2, c.omb2)), gk), c.one);
+        uint64_t up;
+        if (EIGHT) {
+            root[k] = root2(v[k]);
+            up = quot2(m[k], sum2(mul2(root[k], pair(c.inv_root2, c.inv_root2)), pair(c.eps, c.eps), c.one));
+        } else {
+            const float2 w = halves(v[k]), h = halves(m[k]);
+            root[k] = pair(__fsqrt_rn(w.x), __fsqrt_rn(w.y));
+            const float2 den = halves(sum2(mul2(root[k], pair(c.inv_root2, c.inv_root2)), pair(c.eps, c.eps), c.one));
+            up = pair(__fdiv_rn(h.x, den.x), __fdiv_rn(h.y, den.y));
         }
-    } else {                         // the values behind a tensor's end stay as they are
-        if (MASTER) store8<float>(s.master + f, false, n, p);
-        if (!EIGHT) {
-            store8<float>(static_cast<float *>(s.m) + f, false, n, m);
-            store8<float>(static_cast<float *>(s.v) + f, false, n, v);
-        }
+        p[k] = sum2(mul2(p[k], pair(keep, keep)), mul2(up, pair(-c.step_size, -c.step_size)), c.one);
     }
-    if (!EIGHT) return;
+}
+
+// m and v of a lane's 8 values from their e4m3 codes and the block's scales, and
+// back: the scales are the warp's largest magnitudes / 448
+struct Codes {
+    uint2 m, v;
+    float m_scale, v_scale;
+};
+__device__ __forceinline__ void decode(const Codes &q, uint64_t *m, uint64_t *v) {
+    unpack_e4m3(q.m.x, m);
+    unpack_e4m3(q.m.y, m + 2);
+    unpack_e4m3(q.v.x, v);
+    unpack_e4m3(q.v.y, v + 2);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        m[k] = mul2(m[k], pair(q.m_scale, q.m_scale));
+        v[k] = mul2(v[k], pair(q.v_scale, q.v_scale));
+        v[k] = mul2(v[k], v[k]);
+    }
+}
+__device__ __forceinline__ Codes encode(const uint64_t *m, const uint64_t *root) {
     float am = 0.0f, av = 0.0f;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -182,49 +178,230 @@ adamw_kernel(const __grid_constant__ AdamwTable<N> tab, const AdamwState s, cons
         am = fmaxf(am, fmaxf(fabsf(h.x), fabsf(h.y)));
         av = fmaxf(av, fmaxf(w.x, w.y));
     }
-    am = warp_max(am);
-    av = warp_max(av);
+    am = warp_top(am);
+    av = warp_top(av);
     const float mm = am >= 1e-30f ? __fmul_rn(__frcp_rn(am), 448.0f) : 0.0f;
     const float mv = av >= 1e-30f ? __fmul_rn(__frcp_rn(av), 448.0f) : 0.0f;
-    // below the lowest code 2^-9 a root above zero becomes that
+    // a root above zero (3e-23 at least, of the smallest fp32 value) becomes no
+    // less than the lowest code, 2^-9
     const float least = mv > 0.0f ? 0.001953125f : 0.0f;
+    uint64_t a[4], b[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        m[k] = mul2(m[k], pair(mm, mm));
-        const float2 w = halves(root[k]), q = halves(mul2(root[k], pair(mv, mv)));
-        root[k] = pair(w.x > 0.0f ? fmaxf(q.x, least) : q.x, w.y > 0.0f ? fmaxf(q.y, least) : q.y);
+        a[k] = mul2(m[k], pair(mm, mm));
+        const float2 q = halves(mul2(root[k], pair(mv, mv))), any = halves(mul2(root[k], pair(1e30f, 1e30f)));
+        b[k] = pair(fmaxf(q.x, fminf(any.x, least)), fmaxf(q.y, fminf(any.y, least)));
     }
-    *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(s.m) + f) = make_uint2(pack_e4m3(m), pack_e4m3(m + 2));
-    *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(s.v) + f) = make_uint2(pack_e4m3(root), pack_e4m3(root + 2));
+    Codes q;
+    q.m = make_uint2(pack_e4m3(a), pack_e4m3(a + 2));
+    q.v = make_uint2(pack_e4m3(b), pack_e4m3(b + 2));
+    q.m_scale = mm > 0.0f ? __fmul_rn(am, (float)(1.0 / 448.0)) : 0.0f;
+    q.v_scale = mv > 0.0f ? __fmul_rn(av, (float)(1.0 / 448.0)) : 0.0f;
+    return q;
+}
+
+// A lane's values of the blocks ahead, on their way into its own slots of shared
+// memory (16 bytes a slot, neighbouring threads' side by side): weights, gradients,
+// and the codes of m and v in one slot.
+template <typename P, typename G> struct AdamRing {
+    static constexpr int SP = sizeof(P) / 2, SG = sizeof(G) / 2, S = SP + SG + 1;
+    static constexpr int D = S <= 3 ? 4 : 3;             // 192 to 240 bytes a thread
+    static constexpr int kBytes = D * S * 16 * 256;
+    uint32_t base;
+    __device__ __forceinline__ static void copy(uint32_t to, const void *from, bool half) {
+        if (half) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from) : "memory");
+        else asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+    }
+    __device__ __forceinline__ static uint4 read(uint32_t at) {
+        uint4 u;
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+                     : "r"(at));
+        return u;
+    }
+    __device__ __forceinline__ void fetch(int stage, bool any, const P *p, const G *g, const void *m, const void *v) const {
+        const uint32_t at = base + stage * (S * 16 * 256);
+        if (any) {
+#pragma unroll
+            for (int i = 0; i < SP; ++i) copy(at + i * 4096, reinterpret_cast<const uint4 *>(p) + i, false);
+#pragma unroll
+            for (int i = 0; i < SG; ++i) copy(at + (SP + i) * 4096, reinterpret_cast<const uint4 *>(g) + i, false);
+            copy(at + (SP + SG) * 4096, m, true);
+            copy(at + (SP + SG) * 4096 + 8, v, true);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    __device__ __forceinline__ static void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(D - 1) : "memory"); }
+    __device__ __forceinline__ void get(int stage, uint64_t *p, uint64_t *g, Codes &q) const {
+        const uint32_t at = base + stage * (S * 16 * 256);
+#pragma unroll
+        for (int i = 0; i < SP; ++i) unpack<P>(read(at + i * 4096), p + i * kPairs<P>);
+#pragma unroll
+        for (int i = 0; i < SG; ++i) unpack<G>(read(at + (SP + i) * 4096), g + i * kPairs<G>);
+        const uint4 u = read(at + (SP + SG) * 4096);
+        q.m = make_uint2(u.x, u.y);
+        q.v = make_uint2(u.z, u.w);
+    }
+};
+__device__ __forceinline__ void store_codes(const AdamwState &s, const Codes &q, int64_t f, int64_t blk, int lane) {
+    *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(s.m) + f) = q.m;
+    *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(s.v) + f) = q.v;
     if (lane == 0) {
-        s.m_scale[blk] = mm > 0.0f ? __fmul_rn(am, (float)(1.0 / 448.0)) : 0.0f;
-        s.v_scale[blk] = mv > 0.0f ? __fmul_rn(av, (float)(1.0 / 448.0)) : 0.0f;
+        s.m_scale[blk] = q.m_scale;
+        s.v_scale[blk] = q.v_scale;
     }
+}
+
+// A warp steps a run of up to `run` blocks of 256 values one after another, 8
+// values a lane: every load of a warp is of whole sectors and a block's scales are
+// its lanes' maximum.  With 8-bit states a block takes as long to compute as its
+// few bytes take to arrive, so they are fetched D - 1 blocks ahead (loaded where
+// they are used, the warps waited for half of the time), and the scales of the
+// run's 16 blocks at most lie in its lanes.
+template <int N, typename P, typename G, bool EIGHT, bool MASTER>
+__global__ void __launch_bounds__(256, 3)
+adamw_kernel(const __grid_constant__ AdamwTable<N> tab, const AdamwState s, const AdamwConsts c, const int run) {
+    extern __shared__ uint4 dyn[];
+    const int u = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (u >= tab.first[tab.n]) return;
+    int lo = 0, hi = tab.n;          // the last tensor that starts at or before this run
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (tab.first[mid] <= u) lo = mid;
+        else hi = mid;
+    }
+    using PM = std::conditional_t<MASTER, float, P>;     // where the exact weight is
+    const int64_t rel = (int64_t)(u - tab.first[lo]) * run, numel = tab.numel[lo];
+    int64_t i = rel * kAdamBlock + lane * 8;
+    int64_t blk = tab.start[lo] + rel, f = blk * kAdamBlock + lane * 8;
+    P *pp = static_cast<P *>(tab.p[lo]) + i;
+    const G *gg = static_cast<const G *>(tab.g[lo]) + i;
+    const float keep = tab.keep[lo];
+    const bool aligned = (((uintptr_t)pp | (uintptr_t)gg) & 15) == 0;
+    const int64_t left = (numel + kAdamBlock - 1) / kAdamBlock - rel;
+    const int blocks = (int)(left < run ? left : run);
+    if (EIGHT && aligned && numel - rel * kAdamBlock >= (int64_t)blocks * kAdamBlock) {
+        using Ring = AdamRing<PM, G>;
+        Ring ring;
+        ring.base = (uint32_t)__cvta_generic_to_shared(dyn + threadIdx.x);
+        const PM *from;
+        if constexpr (MASTER) from = s.master + f;
+        else from = pp;
+        const uint8_t *m8 = static_cast<const uint8_t *>(s.m) + f, *v8 = static_cast<const uint8_t *>(s.v) + f;
+        auto fetch = [&](int stage, int r) {
+            const int64_t at = (int64_t)r * kAdamBlock;
+            ring.fetch(stage, r < blocks, from + at, gg + at, m8 + at, v8 + at);
+        };
+#pragma unroll
+        for (int d = 0; d < Ring::D - 1; ++d) fetch(d, d);
+        float scale = 0.0f;          // lanes 0-15: of m, 16-31: of v
+        if ((lane & 15) < blocks) scale = (lane < 16 ? s.m_scale : s.v_scale)[blk + (lane & 15)];
+        int stage = 0;
+        for (int r = 0; r < blocks; ++r) {
+            fetch(stage == 0 ? Ring::D - 1 : stage - 1, r + Ring::D - 1);
+            Ring::wait();
+            uint64_t p[4], g[4], m[4], v[4], root[4];
+            Codes q;
+            ring.get(stage, p, g, q);
+            q.m_scale = __shfl_sync(0xffffffffu, scale, r);
+            q.v_scale = __shfl_sync(0xffffffffu, scale, 16 + r);
+            decode(q, m, v);
+            step8<true>(c, keep, g, p, m, v, root);
+            store8<P>(pp, true, 8, p);
+            if (MASTER) store8<float>(s.master + f, true, 8, p);
+            store_codes(s, encode(m, root), f, blk, lane);
+            stage = stage == Ring::D - 1 ? 0 : stage + 1;
+            pp += kAdamBlock;
+            f += kAdamBlock;
+            ++blk;
+        }
+        return;
+    }
+    for (int r = 0; r < blocks; ++r) {
+        const int n = numel - i >= 8 ? 8 : numel - i > 0 ? (int)(numel - i) : 0;
+        const bool whole = aligned && n == 8;
+        float *m32 = static_cast<float *>(s.m) + f, *v32 = static_cast<float *>(s.v) + f;
+        uint64_t p[4], g[4], m[4], v[4], root[4];
+        load8<G>(gg, whole, n, g);
+        if (MASTER) load8<float>(s.master + f, true, 8, p);
+        else load8<P>(pp, whole, n, p);
+        if (EIGHT) {
+            Codes q;
+            q.m = *reinterpret_cast<const uint2 *>(static_cast<uint8_t *>(s.m) + f);
+            q.v = *reinterpret_cast<const uint2 *>(static_cast<uint8_t *>(s.v) + f);
+            q.m_scale = s.m_scale[blk];
+            q.v_scale = s.v_scale[blk];
+            decode(q, m, v);
+        } else {
+            load8<float>(m32, true, 8, m);
+            load8<float>(v32, true, 8, v);
+        }
+        if (n < 8) {                 // what lies behind a tensor's end takes no part
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float2 x = halves(m[k]), y = halves(v[k]);
+                m[k] = pair(2 * k < n ? x.x : 0.0f, 2 * k + 1 < n ? x.y : 0.0f);
+                v[k] = pair(2 * k < n ? y.x : 0.0f, 2 * k + 1 < n ? y.y : 0.0f);
+            }
+        }
+        step8<EIGHT>(c, keep, g, p, m, v, root);
+        store8<P>(pp, whole, n, p);
+        // the values behind a tensor's end stay as they are
+        if (MASTER) store8<float>(s.master + f, n == 8, n, p);
+        if (EIGHT) {
+            store_codes(s, encode(m, root), f, blk, lane);
+        } else {
+            store8<float>(m32, n == 8, n, m);
+            store8<float>(v32, n == 8, n, v);
+        }
+        pp += kAdamBlock;
+        gg += kAdamBlock;
+        f += kAdamBlock;
+        i += kAdamBlock;
+        ++blk;
+    }
+}
+
+template <int N, typename P, typename G, bool EIGHT, bool MASTER>
+static int adamw_start(const AdamwTable<N> &tab, const AdamwState &s, const AdamwConsts &c, int run, cudaStream_t st) {
+    auto kernel = adamw_kernel<N, P, G, EIGHT, MASTER>;
+    const int smem = EIGHT ? AdamRing<std::conditional_t<MASTER, float, P>, G>::kBytes : 0;
+    if (smem > 48 * 1024 &&
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return USAF_ECUDA;
+    }
+    kernel<<<cdiv(tab.first[tab.n], 8), 256, smem, st>>>(tab, s, c, run);
+    USAF_CHECK_LAUNCH();
+    return USAF_OK;
 }
 
 template <int N, typename P, typename G, bool EIGHT>
 static int adamw_launch(const AdamwList &t, int at, int n, double lr, const AdamwState &s, const AdamwConsts &c,
                         cudaStream_t st) {
     AdamwTable<N> tab;
-    int64_t blocks = 0;
+    int64_t values = 0, runs = 0;
+    for (int i = 0; i < n; ++i) values += t.numel[at + i];
+    // A warp looks its place up once for a run of up to 16 blocks (4 with 32-bit
+    // states, which have no ring to fill), where that leaves the GPU (148 SMs of 24
+    // warps) eight runs for each of its warps
+    int run = 1;
+    while (run < (EIGHT ? 16 : 4) && values >= (int64_t)kAdamBlock * 2 * run * 148 * 24 * 8) run *= 2;
     tab.n = n;
     for (int i = 0; i < n; ++i) {
-        tab.first[i] = (int32_t)blocks;
+        tab.first[i] = (int32_t)runs;
         tab.p[i] = t.p[at + i];
         tab.g[i] = t.g[at + i];
         tab.numel[i] = t.numel[at + i];
         tab.start[i] = t.start[at + i] / kAdamBlock;
         tab.keep[i] = (float)(1.0 - lr * t.decay[at + i]);
-        blocks += (t.numel[at + i] + kAdamBlock - 1) / kAdamBlock;
-        if (blocks > 0x7fffffff) return USAF_EUNSUPPORTED;
+        runs += (t.numel[at + i] + kAdamBlock * run - 1) / (kAdamBlock * run);
+        if (runs > 0x7fffffff) return USAF_EUNSUPPORTED;
     }
-    tab.first[n] = (int32_t)blocks;
-    if (blocks == 0) return USAF_OK;
-    const unsigned grid = cdiv(blocks, 8);
-    if (s.master) adamw_kernel<N, P, G, EIGHT, true><<<grid, 256, 0, st>>>(tab, s, c);
-    else adamw_kernel<N, P, G, EIGHT, false><<<grid, 256, 0, st>>>(tab, s, c);
-    USAF_CHECK_LAUNCH();
-    return USAF_OK;
+    tab.first[n] = (int32_t)runs;
+    if (runs == 0) return USAF_OK;
+    return s.master ? adamw_start<N, P, G, EIGHT, true>(tab, s, c, run, st)
+                    : adamw_start<N, P, G, EIGHT, false>(tab, s, c, run, st);
 }
 
 template <typename P, typename G>
@@ -270,6 +447,7 @@ extern "C" int usaf_adamw(int32_t n_tensors, void *const *p, const void *const *
     c.eps = (float)eps;
     c.step_size = (float)(lr / (1.0 - std::pow(beta1, (double)step)));
     c.gmul = (float)(1.0 / grad_div);
+    c.one = 1.0f;
     const AdamwState s{master, m, v, m_scale, v_scale};
     const bool eight = bits == 8;
     cudaStream_t st = as_stream(stream);

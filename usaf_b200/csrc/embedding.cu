@@ -17,6 +17,7 @@
 #include <cooperative_groups.h>
 
 #include "common.cuh"
+#include "f32x2.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -143,6 +144,7 @@ __device__ __forceinline__ uint32_t sort_key(const SortArgs &a, uint32_t j) {
 __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads)
 embed_sort_kernel(const SortArgs a) {
     extern __shared__ uint32_t hist[];                 // [32 warps][bins], then total [bins], base [bins]
+    let_next_start();
     if (blockIdx.x >= kSortCtas) {
         zero_fill(a.zero, a.zero_bytes, (int64_t)(blockIdx.x - kSortCtas) * kSortThreads + threadIdx.x,
                   (int64_t)(gridDim.x - kSortCtas) * kSortThreads);
@@ -235,6 +237,26 @@ __device__ __forceinline__ void put_row(G *__restrict__ grad, int64_t row, int c
                                         float scale, int add) {
     constexpr int N = kLaneN<T>;
     G *g = grad + row * H;
+    if constexpr (VEC) {             // the lane's values are one or two vectors of the gradient's row
+        const int c = c0 + lane * N;
+        if (c < H) {
+            uint4 *to = reinterpret_cast<uint4 *>(g + c);
+#pragma unroll
+            for (int i = 0; i < N * (int)sizeof(G) / 16; ++i) {
+                uint64_t v[kPairs<G>];
+                if (add) unpack<G>(to[i], v);
+#pragma unroll
+                for (int k = 0; k < kPairs<G>; ++k) {
+                    const int j = (i * kPairs<G> + k) * 2;
+                    const float2 h = add ? halves(v[k]) : make_float2(0.0f, 0.0f);
+                    v[k] = pair(add ? fmaf(acc[j], scale, h.x) : acc[j] * scale,
+                                add ? fmaf(acc[j + 1], scale, h.y) : acc[j + 1] * scale);
+                }
+                to[i] = pack<G>(v);
+            }
+        }
+        return;
+    }
 #pragma unroll
     for (int k = 0; k < N; ++k) {
         const int c = lane_col<T, VEC>(c0, lane, k);
@@ -248,6 +270,8 @@ embed_sum_kernel(const T *__restrict__ dy, const uint32_t *__restrict__ key, con
                  uint32_t tokens, uint32_t V, int H, float scale, int add, G *__restrict__ grad,
                  float *__restrict__ part) {
     constexpr int N = kLaneN<T>, B = 8;
+    wait_for_previous();
+    let_next_start();
     const int slabs = (H + 32 * N - 1) / (32 * N);
     const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5;
     const int lane = threadIdx.x & 31;
@@ -271,10 +295,18 @@ embed_sum_kernel(const T *__restrict__ dy, const uint32_t *__restrict__ key, con
             put_row<T, G, VEC>(grad, cur, c0, lane, H, acc, scale, add);
         } else {                                       // slot 0: begun before this chunk, 1: begins in it
             float *p = part + (chunk * 2 + (from ? 0 : 1)) * H;
+            if constexpr (VEC) {
+                if (c0 + lane * N < H)
 #pragma unroll
-            for (int k = 0; k < N; ++k) {
-                const int c = lane_col<T, VEC>(c0, lane, k);
-                if (c < H) p[c] = acc[k];
+                    for (int k = 0; k < N; k += 4)
+                        *reinterpret_cast<float4 *>(p + c0 + lane * N + k) =
+                            make_float4(acc[k], acc[k + 1], acc[k + 2], acc[k + 3]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < N; ++k) {
+                    const int c = lane_col<T, VEC>(c0, lane, k);
+                    if (c < H) p[c] = acc[k];
+                }
             }
         }
     };
@@ -303,42 +335,76 @@ embed_sum_kernel(const T *__restrict__ dy, const uint32_t *__restrict__ key, con
     flush(live == n);
 }
 
-// one CTA per chunk and 32 columns: where the chunk's last token begins in it
-// and goes on, the 8 warps add contiguous parts of its partial sums, which are
-// then added in order
+// A CTA looks at 8 chunks, one a warp: where a chunk's last token begins in it and
+// goes on, the chunks that it runs through are counted.  A token of few chunks is
+// joined by its warp, 32 columns at a time; of many (a run of hundreds of partial
+// sums) by all 8 warps, each a contiguous part, which are then added in order.
 template <typename G>
 __global__ void __launch_bounds__(256)
 embed_join_kernel(const uint32_t *__restrict__ key, uint32_t tokens, uint32_t V, int H, float scale, int add,
-                  G *__restrict__ grad, const float *__restrict__ part) {
+                  G *__restrict__ grad, const float *__restrict__ part, int64_t chunks) {
     __shared__ float s[8][32];
-    const int64_t chunk = blockIdx.x;
-    const uint32_t b = (uint32_t)(chunk * kChunk), e = b + kChunk;     // never the last chunk
-    const uint32_t k = key[e - 1];
-    if (k >= V || key[e] != k || (key[b] == k && b > 0 && key[b - 1] == k)) return;
-    int follow = 0;                                    // chunks that begin with this token
-    for (;;) {
-        const uint64_t p = (uint64_t)e + (uint64_t)(follow + threadIdx.x) * kChunk;
-        const int got = __syncthreads_count(p < tokens && key[p] == k);
-        follow += got;
-        if (got < 256) break;
-    }
+    __shared__ int follow[8];
+    __shared__ uint32_t token[8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int each = (follow + 1 + 7) / 8;
-    for (int c = blockIdx.y * 32 + lane; c - lane < H; c += gridDim.y * 32) {
-        float v = 0.0f;
-        if (c < H)
-            for (int i = warp * each; i < min(follow + 1, (warp + 1) * each); ++i)
-                v += part[((chunk + i) * 2 + (i == 0 ? 1 : 0)) * H + c];
-        s[warp][lane] = v;
-        __syncthreads();
-        if (warp == 0 && c < H) {
-            float t = 0.0f;
-#pragma unroll
-            for (int w = 0; w < 8; ++w) t += s[w][lane];
-            G *g = grad + (int64_t)k * H + c;
-            *g = from_f<G>(add ? fmaf(t, scale, to_f(*g)) : t * scale);
+    constexpr int kFew = 12;
+    auto put = [&](uint32_t k, int c, float v) {
+        G *g = grad + (int64_t)k * H + c;
+        *g = from_f<G>(add ? fmaf(v, scale, to_f(*g)) : v * scale);
+    };
+    wait_for_previous();
+    const int64_t mine = (int64_t)blockIdx.x * 8 + warp;
+    int n = 0;
+    if (mine < chunks - 1) {
+        const uint32_t b = (uint32_t)(mine * kChunk), e = b + kChunk;
+        const uint32_t k = key[e - 1];
+        if (k < V && key[e] == k && !(key[b] == k && b > 0 && key[b - 1] == k)) {
+            for (;;) {               // chunks that begin with this token
+                const uint64_t p = (uint64_t)e + (uint64_t)(n + lane) * kChunk;
+                const int got = __popc(__ballot_sync(0xffffffffu, p < tokens && key[p] == k));
+                n += got;
+                if (got < 32) break;
+            }
         }
-        __syncthreads();
+        if (n > 0 && n <= kFew) {
+            for (int c = blockIdx.y * 32 + lane; c < H; c += gridDim.y * 32) {
+                float v[kFew + 1];
+#pragma unroll
+                for (int i = 0; i <= kFew; ++i)
+                    v[i] = i <= n ? part[((mine + i) * 2 + (i == 0 ? 1 : 0)) * H + c] : 0.0f;
+                float t = v[0];
+#pragma unroll
+                for (int i = 1; i <= kFew; ++i)
+                    if (i <= n) t += v[i];
+                put(k, c, t);
+            }
+            n = 0;
+        }
+        if (lane == 0) token[warp] = k;
+    }
+    if (lane == 0) follow[warp] = n;
+    __syncthreads();
+    for (int w = 0; w < 8; ++w) {
+        const int m = follow[w] + 1, each = (m + 7) / 8;
+        if (m == 1) continue;
+        const int64_t chunk = (int64_t)blockIdx.x * 8 + w;
+        for (int c = blockIdx.y * 32 + lane; c - lane < H; c += gridDim.y * 32) {
+            float v = 0.0f;
+            if (c < H) {
+#pragma unroll 8
+                for (int i = warp * each; i < min(m, (warp + 1) * each); ++i)
+                    v += part[((chunk + i) * 2 + (i == 0 ? 1 : 0)) * H + c];
+            }
+            s[warp][lane] = v;
+            __syncthreads();
+            if (warp == 0 && c < H) {
+                float t = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) t += s[i][lane];
+                put(token[w], c, t);
+            }
+            __syncthreads();
+        }
     }
 }
 
@@ -390,19 +456,17 @@ template <typename T, typename G> static int embed_bwd(const EmbedBwd &a, cudaSt
     const int64_t chunks = (a.tokens + kChunk - 1) / kChunk;
     const int slabs = (a.H + 32 * kLaneN<T> - 1) / (32 * kLaneN<T>);
     const unsigned grid = cdiv(chunks * slabs, 8);
-    const bool vec = (uintptr_t)a.dy % 16 == 0 && (int64_t)a.H * sizeof(T) % 16 == 0;
-    if (vec)
-        embed_sum_kernel<T, G, true><<<grid, 256, 0, st>>>((const T *)a.dy, key, pos, (uint32_t)a.tokens, (uint32_t)a.V,
-                                                           a.H, a.scale, a.add, (G *)a.grad, part);
-    else
-        embed_sum_kernel<T, G, false><<<grid, 256, 0, st>>>((const T *)a.dy, key, pos, (uint32_t)a.tokens, (uint32_t)a.V,
-                                                            a.H, a.scale, a.add, (G *)a.grad, part);
-    USAF_CHECK_LAUNCH();
+    // 16-byte vectors of dy's rows, of the gradient's and of the partial sums
+    const bool vec = ((uintptr_t)a.dy | (uintptr_t)a.grad | (uintptr_t)a.ws) % 16 == 0 && (int64_t)a.H * sizeof(T) % 16 == 0;
+    if (!launch_early(vec ? embed_sum_kernel<T, G, true> : embed_sum_kernel<T, G, false>, dim3(grid), 256, 0, st,
+                      (const T *)a.dy, key, pos, (uint32_t)a.tokens, (uint32_t)a.V, a.H, a.scale, a.add, (G *)a.grad,
+                      part))
+        return USAF_ECUDA;
     if (chunks > 1) {
-        const dim3 jgrid((unsigned)(chunks - 1), (unsigned)std::min((a.H + 31) / 32, 64));
-        embed_join_kernel<G><<<jgrid, 256, 0, st>>>(key, (uint32_t)a.tokens, (uint32_t)a.V, a.H, a.scale, a.add,
-                                                    (G *)a.grad, part);
-        USAF_CHECK_LAUNCH();
+        const dim3 jgrid(cdiv(chunks - 1, 8), (unsigned)std::min((a.H + 31) / 32, 64));
+        if (!launch_early(embed_join_kernel<G>, jgrid, 256, 0, st, key, (uint32_t)a.tokens, (uint32_t)a.V, a.H, a.scale,
+                          a.add, (G *)a.grad, (const float *)part, chunks))
+            return USAF_ECUDA;
     }
     return USAF_OK;
 }
