@@ -232,44 +232,52 @@ embed_sort_kernel(const SortArgs a) {
 }
 
 // ---- backward: sums -----------------------------------------------------------
+// the lane's 16 / sizeof(T) sums into its columns of a row of the gradient
 template <typename T, typename G, bool VEC>
-__device__ __forceinline__ void put_row(G *__restrict__ grad, int64_t row, int c0, int lane, int H, const float *acc,
-                                        float scale, int add) {
-    constexpr int N = kLaneN<T>;
-    G *g = grad + row * H;
-    if constexpr (VEC) {             // the lane's values are one or two vectors of the gradient's row
-        const int c = c0 + lane * N;
-        if (c < H) {
-            uint4 *to = reinterpret_cast<uint4 *>(g + c);
+__device__ __forceinline__ void put_row(G *__restrict__ g, int c0, int lane, int H, const uint64_t *acc, float scale,
+                                        int add) {
+    constexpr int N2 = kPairs<T>;
+    const uint64_t by = pair(scale, scale);
+    if constexpr (VEC) {             // one or two vectors
+        const int c = c0 + lane * 2 * N2;
+        if (c >= H) return;
+        uint4 *to = reinterpret_cast<uint4 *>(g + c);
 #pragma unroll
-            for (int i = 0; i < N * (int)sizeof(G) / 16; ++i) {
-                uint64_t v[kPairs<G>];
-                if (add) unpack<G>(to[i], v);
+        for (int i = 0; i < N2 / kPairs<G>; ++i) {
+            uint64_t v[kPairs<G>];
+            if (add) unpack<G>(to[i], v);
 #pragma unroll
-                for (int k = 0; k < kPairs<G>; ++k) {
-                    const int j = (i * kPairs<G> + k) * 2;
-                    const float2 h = add ? halves(v[k]) : make_float2(0.0f, 0.0f);
-                    v[k] = pair(add ? fmaf(acc[j], scale, h.x) : acc[j] * scale,
-                                add ? fmaf(acc[j + 1], scale, h.y) : acc[j + 1] * scale);
-                }
-                to[i] = pack<G>(v);
+            for (int k = 0; k < kPairs<G>; ++k) {
+                const uint64_t s = acc[i * kPairs<G> + k];
+                v[k] = add ? fma2(s, by, v[k]) : mul2(s, by);
             }
+            to[i] = pack<G>(v);
         }
-        return;
-    }
+    } else {
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-        const int c = lane_col<T, VEC>(c0, lane, k);
-        if (c < H) g[c] = from_f<G>(add ? fmaf(acc[k], scale, to_f(g[c])) : acc[k] * scale);
+        for (int k = 0; k < N2; ++k) {
+            const float2 h = halves(acc[k]);
+            const int c = c0 + lane + 64 * k;
+            if (c < H) g[c] = from_f<G>(add ? fmaf(h.x, scale, to_f(g[c])) : h.x * scale);
+            if (c + 32 < H) g[c + 32] = from_f<G>(add ? fmaf(h.y, scale, to_f(g[c + 32])) : h.y * scale);
+        }
     }
 }
+
+// One warp per chunk and slab.  The chunk's rows come through a ring of kAhead
+// slots of 16 bytes a lane in shared memory, filled by asynchronous copies (of 16
+// bytes, or of 4 where fp32 rows are not aligned), so that 15 rows are on their
+// way whatever the tokens are; 16-bit rows that are not aligned are loaded eight at
+// a time.
+constexpr int kAhead = 16;
 
 template <typename T, typename G, bool VEC>
 __global__ void __launch_bounds__(256)
 embed_sum_kernel(const T *__restrict__ dy, const uint32_t *__restrict__ key, const uint32_t *__restrict__ pos,
                  uint32_t tokens, uint32_t V, int H, float scale, int add, G *__restrict__ grad,
                  float *__restrict__ part) {
-    constexpr int N = kLaneN<T>, B = 8;
+    extern __shared__ uint4 dyn[];   // [kAhead][256 threads]
+    constexpr int N = kLaneN<T>, N2 = N / 2;
     wait_for_previous();
     let_next_start();
     const int slabs = (H + 32 * N - 1) / (32 * N);
@@ -284,55 +292,78 @@ embed_sum_kernel(const T *__restrict__ dy, const uint32_t *__restrict__ key, con
     const uint32_t before = b ? key[b - 1] : V, after = b + n < tokens ? key[b + n] : V;
     const int live = __popc(__ballot_sync(0xffffffffu, k_l < V));     // row V sorts behind the others
     if (!live) return;
-    const uint32_t first = __shfl_sync(0xffffffffu, k_l, 0);
-    float acc[N];
-    uint32_t cur = first;
+    uint4 *ring = dyn + threadIdx.x;
+    const uint32_t at = (uint32_t)__cvta_generic_to_shared(ring);
+    auto fetch = [&](int i) {        // row i of the chunk into slot i % kAhead
+        if constexpr (VEC || sizeof(T) == 4) {
+            const uint32_t p = __shfl_sync(0xffffffffu, p_l, i & 31), to = at + (i % kAhead) * 4096;
+            if (i < live) {
+                const T *row = dy + (int64_t)p * H + c0;
+                if constexpr (VEC) {
+                    if (c0 + lane * N < H)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(row + lane * N) : "memory");
+                } else {
 #pragma unroll
-    for (int k = 0; k < N; ++k) acc[k] = 0.0f;
-    auto flush = [&](bool last) {
-        const bool from = cur == before && cur == first, on = last && cur == after;
-        if (!from && !on) {
-            put_row<T, G, VEC>(grad, cur, c0, lane, H, acc, scale, add);
-        } else {                                       // slot 0: begun before this chunk, 1: begins in it
-            float *p = part + (chunk * 2 + (from ? 0 : 1)) * H;
-            if constexpr (VEC) {
-                if (c0 + lane * N < H)
-#pragma unroll
-                    for (int k = 0; k < N; k += 4)
-                        *reinterpret_cast<float4 *>(p + c0 + lane * N + k) =
-                            make_float4(acc[k], acc[k + 1], acc[k + 2], acc[k + 3]);
-            } else {
-#pragma unroll
-                for (int k = 0; k < N; ++k) {
-                    const int c = lane_col<T, VEC>(c0, lane, k);
-                    if (c < H) p[c] = acc[k];
+                    for (int k = 0; k < N; ++k)
+                        if (c0 + lane + 32 * k < H)
+                            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + 4 * k),
+                                         "l"(row + lane + 32 * k)
+                                         : "memory");
                 }
             }
+            asm volatile("cp.async.commit_group;" ::: "memory");
         }
     };
-    for (int i0 = 0; i0 < live; i0 += B) {
-        float v[B][N];
+    for (int i = 0; i < kAhead - 1; ++i) fetch(i);
+    uint64_t acc[N2];
+    uint32_t cur = V, first = V;
+    for (int i = 0; i <= live; ++i) {
+        const uint32_t k_i = __shfl_sync(0xffffffffu, k_l, i & 31);
+        if (i == live || k_i != cur) {
+            if (i > 0) {             // the row of `cur` is complete in this chunk
+                const bool from = cur == before && cur == first, on = i == live && live == n && cur == after;
+                if (!from && !on) {
+                    put_row<T, G, VEC>(grad + (int64_t)cur * H, c0, lane, H, acc, scale, add);
+                } else {             // slot 0: begun before this chunk, 1: begins in it
+                    put_row<T, float, VEC>(part + (chunk * 2 + (from ? 0 : 1)) * H, c0, lane, H, acc, 1.0f, 0);
+                }
+            } else {
+                first = k_i;
+            }
+            if (i == live) break;
+            cur = k_i;
 #pragma unroll
-        for (int i = 0; i < B; ++i) {
-            const uint32_t p = __shfl_sync(0xffffffffu, p_l, i0 + i);
-            if (i0 + i < live) load_lane<T, VEC>(dy + (int64_t)p * H, c0, lane, H, v[i]);
+            for (int k = 0; k < N2; ++k) acc[k] = 0;
         }
+        if constexpr (!VEC && sizeof(T) == 2) {
+            if (i % 8 == 0) {
+                T v[8][N];
 #pragma unroll
-        for (int i = 0; i < B; ++i) {
-            if (i0 + i < live) {
-                const uint32_t k_i = __shfl_sync(0xffffffffu, k_l, i0 + i);
-                if (k_i != cur) {
-                    flush(false);
-                    cur = k_i;
+                for (int j = 0; j < 8; ++j) {
+                    const uint32_t p = __shfl_sync(0xffffffffu, p_l, i + j);
+                    if (i + j < live)
 #pragma unroll
-                    for (int k = 0; k < N; ++k) acc[k] = 0.0f;
+                        for (int k = 0; k < N; ++k)
+                            v[j][k] = c0 + lane + 32 * k < H ? dy[(int64_t)p * H + c0 + lane + 32 * k] : T();
                 }
 #pragma unroll
-                for (int k = 0; k < N; ++k) acc[k] += v[i][k];
+                for (int j = 0; j < 8; ++j)
+                    if (i + j < live) {
+                        uint4 u;
+#pragma unroll
+                        for (int k = 0; k < N; ++k) reinterpret_cast<T *>(&u)[k] = v[j][k];
+                        ring[((i + j) % kAhead) * 256] = u;
+                    }
             }
+        } else {
+            fetch(i + kAhead - 1);
+            asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
         }
+        uint64_t v[N2];
+        unpack<T>(ring[(i % kAhead) * 256], v);
+#pragma unroll
+        for (int k = 0; k < N2; ++k) acc[k] = add2(acc[k], v[k]);
     }
-    flush(live == n);
 }
 
 // A CTA looks at 8 chunks, one a warp: where a chunk's last token begins in it and
@@ -458,9 +489,14 @@ template <typename T, typename G> static int embed_bwd(const EmbedBwd &a, cudaSt
     const unsigned grid = cdiv(chunks * slabs, 8);
     // 16-byte vectors of dy's rows, of the gradient's and of the partial sums
     const bool vec = ((uintptr_t)a.dy | (uintptr_t)a.grad | (uintptr_t)a.ws) % 16 == 0 && (int64_t)a.H * sizeof(T) % 16 == 0;
-    if (!launch_early(vec ? embed_sum_kernel<T, G, true> : embed_sum_kernel<T, G, false>, dim3(grid), 256, 0, st,
-                      (const T *)a.dy, key, pos, (uint32_t)a.tokens, (uint32_t)a.V, a.H, a.scale, a.add, (G *)a.grad,
-                      part))
+    auto sum = vec ? embed_sum_kernel<T, G, true> : embed_sum_kernel<T, G, false>;
+    const int ring = kAhead * 256 * 16;
+    if (cudaFuncSetAttribute(sum, cudaFuncAttributeMaxDynamicSharedMemorySize, ring) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return USAF_ECUDA;
+    }
+    if (!launch_early(sum, dim3(grid), 256, ring, st, (const T *)a.dy, key, pos, (uint32_t)a.tokens, (uint32_t)a.V, a.H,
+                      a.scale, a.add, (G *)a.grad, part))
         return USAF_ECUDA;
     if (chunks > 1) {
         const dim3 jgrid(cdiv(chunks - 1, 8), (unsigned)std::min((a.H + 31) / 32, 64));
