@@ -1,10 +1,11 @@
 // Embedding lookup y[t] = scale W[id_t] and the gradient of the table,
 // dW[v] = scale * (sum of dy[t] over the tokens t with id_t = v, ascending t).
 //
-// The gradient takes three launches:
+// The gradient takes four launches, each set up while the one before runs:
 //   1. sort: one cluster of 8 CTAs sorts the (token, position) pairs by a stable
 //      radix sort (digits of up to 9 bits, so two passes for a table of up to
-//      2^18 rows); the other clusters of the same launch write the table's zeros,
+//      2^18 rows);
+//      zeros: on the other SMs at the same time, the table's gradient is cleared,
 //      which is where the time goes (V x H values against tokens x H);
 //   2. sum: the sorted positions are cut into chunks of 32, whatever tokens they
 //      hold, so that a frequent token spreads over many warps; a warp adds the
@@ -27,44 +28,19 @@ __device__ __forceinline__ int64_t token_id(const void *ids, int ids64, int64_t 
     return ids64 ? static_cast<const int64_t *>(ids)[t] : (int64_t) static_cast<const int32_t *>(ids)[t];
 }
 
-// ---- rows in registers ------------------------------------------------------
+// ---- forward ------------------------------------------------------------------
 // A lane holds N = 16 / sizeof(T) values of a slab of 32 N columns: 16
 // consecutive bytes where the rows are 16-byte aligned (VEC), else every 32nd
-// column.
+// column.  One warp takes a token and up to 8 slabs, all loaded before the first
+// is stored; a token outside the table reads as zeros and sets the error word.
 template <typename T> constexpr int kLaneN = 16 / (int)sizeof(T);
+constexpr int kFwdSlabs = 8;
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void load_lane(const T *__restrict__ row, int c0, int lane, int H, float *v) {
-    constexpr int N = kLaneN<T>;
-    if (VEC) {
-        const int c = c0 + lane * N;
-        uint4 u = make_uint4(0, 0, 0, 0);
-        if (c < H) u = *reinterpret_cast<const uint4 *>(row + c);
-        const T *t = reinterpret_cast<const T *>(&u);
-#pragma unroll
-        for (int k = 0; k < N; ++k) v[k] = to_f(t[k]);
-    } else {
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-            const int c = c0 + lane + 32 * k;
-            v[k] = c < H ? to_f(row[c]) : 0.0f;
-        }
-    }
-}
-
-// the lane's columns: c0 + lane * N + k (VEC) or c0 + lane + 32 k
-template <typename T, bool VEC> __device__ __forceinline__ int lane_col(int c0, int lane, int k) {
-    return VEC ? c0 + lane * kLaneN<T> + k : c0 + lane + 32 * k;
-}
-
-// ---- forward ------------------------------------------------------------------
-// one warp per token and up to 4 slabs; a token outside the table reads as
-// zeros and sets the error word
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
 embed_fwd_kernel(const void *__restrict__ ids, int ids64, int64_t tokens, const T *__restrict__ table, int64_t V,
                  int H, float scale, T *__restrict__ out, int32_t *__restrict__ err) {
-    constexpr int N = kLaneN<T>, S = 4;
+    constexpr int N = kLaneN<T>, S = kFwdSlabs;
     const int groups = (H + 32 * N * S - 1) / (32 * N * S);
     const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5;
     const int lane = threadIdx.x & 31;
@@ -74,36 +50,39 @@ embed_fwd_kernel(const void *__restrict__ ids, int ids64, int64_t tokens, const 
     const int64_t id = token_id(ids, ids64, t);
     const bool ok = id >= 0 && id < V;
     if (!ok && lane == 0 && c0 == 0 && err) atomicOr(err, USAF_ERR_BAD_INDEX);
-    float v[S][N];
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-        if (ok) load_lane<T, VEC>(table + id * H, c0 + s * 32 * N, lane, H, v[s]);
-        else
-#pragma unroll
-            for (int k = 0; k < N; ++k) v[s][k] = 0.0f;
-    }
+    const T *row = table + (ok ? id * H : 0);
     T *o = out + t * H;
+    if constexpr (VEC) {
+        uint4 u[S];
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-        if (VEC) {
-            uint4 u;
-            T *w = reinterpret_cast<T *>(&u);
-#pragma unroll
-            for (int k = 0; k < N; ++k) w[k] = from_f<T>(v[s][k] * scale);
+        for (int s = 0; s < S; ++s) {
             const int c = c0 + s * 32 * N + lane * N;
-            if (c < H) *reinterpret_cast<uint4 *>(o + c) = u;
-        } else {
-#pragma unroll
-            for (int k = 0; k < N; ++k) {
-                const int c = c0 + s * 32 * N + lane + 32 * k;
-                if (c < H) o[c] = from_f<T>(v[s][k] * scale);
-            }
+            u[s] = make_uint4(0, 0, 0, 0);
+            if (ok && c < H) u[s] = *reinterpret_cast<const uint4 *>(row + c);
         }
+        const uint64_t by = pair(scale, scale);
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            const int c = c0 + s * 32 * N + lane * N;
+            uint64_t v[kPairs<T>];
+            unpack<T>(u[s], v);
+#pragma unroll
+            for (int k = 0; k < kPairs<T>; ++k) v[k] = mul2(v[k], by);
+            if (c < H) *reinterpret_cast<uint4 *>(o + c) = pack<T>(v);
+        }
+    } else {
+        T v[S * N];
+#pragma unroll
+        for (int k = 0; k < S * N; ++k) v[k] = ok && c0 + lane + 32 * k < H ? row[c0 + lane + 32 * k] : from_f<T>(0.0f);
+#pragma unroll
+        for (int k = 0; k < S * N; ++k)
+            if (c0 + lane + 32 * k < H) o[c0 + lane + 32 * k] = from_f<T>(to_f(v[k]) * scale);
     }
 }
 
 // ---- backward: sort and zeros ---------------------------------------------------
 constexpr int kSortCtas = 8, kSortThreads = 1024, kSortWarps = 32, kMaxBins = 512;
+constexpr int kRound = 8;       // pairs a lane loads at once
 constexpr int kChunk = 32;      // sorted positions a warp adds up
 
 struct SortArgs {
@@ -113,17 +92,29 @@ struct SortArgs {
     int passes, width;          // digits of `width` bits
     uint32_t *key[2], *pos[2];  // pass i writes buffer i & 1
     int32_t *err;
-    char *zero; int64_t zero_bytes;   // the gradient to clear, or none
 };
 
-__device__ __forceinline__ void zero_fill(char *p, int64_t n, int64_t tid, int64_t threads) {
-    const int64_t head = min(n, (int64_t)(-(uintptr_t)p & 15));
-    for (int64_t i = tid; i < head; i += threads) p[i] = 0;
+// A CTA clears its 32 KB of the gradient, so many CTAs one after another: 86 us
+// for 622 MB, as the runtime's memset; CTAs that walk through all of it, one or two
+// an SM, took 103 us, and whole clusters of the sort's launch 240.  It runs beside
+// the sort, which it does not need; its last CTAs wait for the sort, so that what
+// waits for the zeros has both.
+constexpr int kZeroTile = 32768, kZeroThreads = 512;
+
+__global__ void __launch_bounds__(kZeroThreads) embed_zero_kernel(char *p, int64_t n) {
+    const int64_t head = min(n, (int64_t)(-(uintptr_t)p & 15)), tile = blockIdx.x;
+    let_next_start();
+    if (tile == 0 && threadIdx.x < head) p[threadIdx.x] = 0;
     p += head;
     n -= head;
-    const uint4 z = make_uint4(0, 0, 0, 0);
-    for (int64_t i = tid; i < n / 16; i += threads) reinterpret_cast<uint4 *>(p)[i] = z;
-    for (int64_t i = n / 16 * 16 + tid; i < n; i += threads) p[i] = 0;
+    uint4 *v = reinterpret_cast<uint4 *>(p);
+#pragma unroll
+    for (int i = 0; i < kZeroTile / 16 / kZeroThreads; ++i) {
+        const int64_t at = tile * (kZeroTile / 16) + i * kZeroThreads + threadIdx.x;
+        if (at < n / 16) v[at] = make_uint4(0, 0, 0, 0);
+    }
+    if (tile == n / kZeroTile && threadIdx.x < (n & 15)) p[n - 1 - threadIdx.x] = 0;
+    if (blockIdx.x + 1 == gridDim.x) wait_for_previous();
 }
 
 // padding and tokens outside the table sort behind the table's rows, as row V
@@ -136,62 +127,99 @@ __device__ __forceinline__ uint32_t sort_key(const SortArgs &a, uint32_t j) {
     return id == a.pad ? (uint32_t)a.V : (uint32_t)id;
 }
 
-// Each CTA of the first cluster owns a contiguous eighth of the pairs, each of
-// its warps a contiguous part of that.  A pass counts the digits per warp
-// (equal digits of 32 pairs found by match), scans the counts over warps, CTAs
-// (distributed shared memory) and digits, and moves every pair to its place:
-// stable, since a warp walks its pairs in order.
+// the lanes of the warp with this lane's digit: a vote per bit (match_any, which
+// does the same, took 4.5 us for 4 digits a lane of 32 warps, the votes under 1)
+__device__ __forceinline__ uint32_t same_digit(uint32_t d, int bits) {
+    uint32_t same = 0xffffffffu;
+    for (int i = 0; i < bits; ++i) {
+        const uint32_t set = __ballot_sync(0xffffffffu, d >> i & 1);
+        same &= d >> i & 1 ? set : ~set;
+    }
+    return same;
+}
+
+// Each CTA of the cluster owns a contiguous eighth of the pairs, each of
+// its warps a contiguous part of that.  A pass counts the digits per warp, scans
+// the counts over warps, CTAs (distributed shared memory) and digits, and moves
+// every pair to its place: stable, since a warp walks its pairs in order.
 __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads)
 embed_sort_kernel(const SortArgs a) {
-    extern __shared__ uint32_t hist[];                 // [32 warps][bins], then total [bins], base [bins]
+    extern __shared__ uint32_t hist[];                 // [32 warps][bins]; total, base [bins]; sums [4][bins]
     let_next_start();
-    if (blockIdx.x >= kSortCtas) {
-        zero_fill(a.zero, a.zero_bytes, (int64_t)(blockIdx.x - kSortCtas) * kSortThreads + threadIdx.x,
-                  (int64_t)(gridDim.x - kSortCtas) * kSortThreads);
-        return;
-    }
     cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int bins = 1 << a.width;
-    uint32_t *total = hist + kSortWarps * bins, *base = total + bins;
+    uint32_t *total = hist + kSortWarps * bins, *base = total + bins, *sums = base + bins;
     __shared__ uint32_t scan[16];
     const uint32_t part = (a.tokens + kSortCtas * kSortWarps * 32 - 1) / (kSortCtas * kSortWarps * 32) * 32;
     const uint64_t first = (uint64_t)(blockIdx.x * kSortWarps + warp) * part;
     const uint32_t b = (uint32_t)min(first, (uint64_t)a.tokens), e = (uint32_t)min(first + part, (uint64_t)a.tokens);
     uint32_t *mine = hist + warp * bins;
+    const bool once = part <= 32 * kRound;              // a warp's pairs stay in its registers for a pass
+    const int split = min(4, kSortThreads / bins);      // threads that scan a digit's counts of the warps
     for (int pass = 0; pass < a.passes; ++pass) {
         const uint32_t *ksrc = a.key[(pass + 1) & 1], *psrc = a.pos[(pass + 1) & 1];
         uint32_t *kdst = a.key[pass & 1], *pdst = a.pos[pass & 1];
         const int shift = pass * a.width;
+        uint32_t key[kRound], pos[kRound];
+        auto load = [&](uint32_t j0) {
+#pragma unroll
+            for (int r = 0; r < kRound; ++r) {
+                const uint32_t j = j0 + 32 * r + lane;
+                if (j < e) {
+                    key[r] = pass ? ksrc[j] : sort_key(a, j);
+                    pos[r] = pass ? psrc[j] : j;
+                }
+            }
+        };
         for (int i = tid; i < kSortWarps * bins; i += kSortThreads) hist[i] = 0;
+        if (once) load(b);
         __syncthreads();
-        for (uint32_t j0 = b; j0 < e; j0 += 32) {
-            const uint32_t j = j0 + lane;
-            uint32_t d = bins;
-            if (j < e) d = ((pass ? ksrc[j] : sort_key(a, j)) >> shift) & (bins - 1);
-            const uint32_t same = __match_any_sync(0xffffffffu, d);
-            if (j < e && lane == __ffs(same) - 1) mine[d] += __popc(same);
-            __syncwarp();
+        for (uint32_t j0 = b; j0 < e; j0 += 32 * kRound) {
+            if (!once) load(j0);
+#pragma unroll
+            for (int r = 0; r < kRound; ++r) {
+                if (j0 + 32 * r >= e) break;
+                const bool in = j0 + 32 * r + lane < e;
+                const uint32_t d = in ? (key[r] >> shift) & (bins - 1) : bins;
+                const uint32_t same = same_digit(d, a.width + 1);
+                if (in && lane == __ffs(same) - 1) mine[d] += __popc(same);
+                __syncwarp();
+            }
         }
         __syncthreads();
-        if (tid < bins) {
+        {                                               // a digit's counts: `split` threads, in whole warps
+            const int d = tid & (bins - 1), q = tid >> a.width, each = kSortWarps / split;
             uint32_t run = 0;
-            for (int w = 0; w < kSortWarps; ++w) {
-                const uint32_t t = hist[w * bins + tid];
-                hist[w * bins + tid] = run;
-                run += t;
+            if (q < split) {
+#pragma unroll 8
+                for (int w = q * each; w < (q + 1) * each; ++w) run += hist[w * bins + d];
+                sums[q * bins + d] = run;
             }
-            total[tid] = run;
+            __syncthreads();
+            if (q < split) {
+                uint32_t at = 0;
+                for (int k = 0; k < q; ++k) at += sums[k * bins + d];
+                if (q == split - 1) total[d] = at + run;
+#pragma unroll 8
+                for (int w = q * each; w < (q + 1) * each; ++w) {
+                    const uint32_t t = hist[w * bins + d];
+                    hist[w * bins + d] = at;
+                    at += t;
+                }
+            }
         }
         cluster.sync();
         uint32_t all = 0, before = 0, inc = 0;
         if (tid < kMaxBins) {                          // whole warps; bins <= kMaxBins
             if (tid < bins) {
+                uint32_t t[kSortCtas];
+#pragma unroll
+                for (int c = 0; c < kSortCtas; ++c) t[c] = cluster.map_shared_rank(total, c)[tid];
 #pragma unroll
                 for (int c = 0; c < kSortCtas; ++c) {
-                    const uint32_t t = cluster.map_shared_rank(total, c)[tid];
-                    if (c < (int)blockIdx.x) before += t;
-                    all += t;
+                    if (c < (int)blockIdx.x) before += t[c];
+                    all += t[c];
                 }
             }
             inc = all;
@@ -209,66 +237,75 @@ embed_sort_kernel(const SortArgs a) {
             base[tid] = add + inc - all + before;
         }
         __syncthreads();
-        for (uint32_t j0 = b; j0 < e; j0 += 32) {
-            const uint32_t j = j0 + lane;
-            uint32_t d = bins, key = 0;
-            if (j < e) {
-                key = pass ? ksrc[j] : sort_key(a, j);
-                d = (key >> shift) & (bins - 1);
+        for (uint32_t j0 = b; j0 < e; j0 += 32 * kRound) {
+            if (!once) load(j0);
+#pragma unroll
+            for (int r = 0; r < kRound; ++r) {
+                if (j0 + 32 * r >= e) break;
+                const bool in = j0 + 32 * r + lane < e;
+                const uint32_t d = in ? (key[r] >> shift) & (bins - 1) : bins;
+                const uint32_t same = same_digit(d, a.width + 1);
+                const uint32_t to = in ? base[d] + mine[d] + __popc(same & ((1u << lane) - 1)) : 0;
+                __syncwarp();
+                if (in) {
+                    if (lane == __ffs(same) - 1) mine[d] += __popc(same);
+                    kdst[to] = key[r];
+                    pdst[to] = pos[r];
+                }
+                __syncwarp();
             }
-            const uint32_t same = __match_any_sync(0xffffffffu, d);
-            uint32_t to = 0;
-            if (j < e) to = base[d] + mine[d] + __popc(same & ((1u << lane) - 1));
-            __syncwarp();
-            if (j < e) {
-                if (lane == __ffs(same) - 1) mine[d] += __popc(same);
-                kdst[to] = key;
-                pdst[to] = pass ? psrc[j] : j;
-            }
-            __syncwarp();
         }
         cluster.sync();                                // the pass's pairs are in place, `total` is read
     }
 }
 
 // ---- backward: sums -----------------------------------------------------------
-// the lane's 16 / sizeof(T) sums into its columns of a row of the gradient
-template <typename T, typename G, bool VEC>
-__device__ __forceinline__ void put_row(G *__restrict__ g, int c0, int lane, int H, const uint64_t *acc, float scale,
-                                        int add) {
+// a lane's columns of a row of T or of the gradient, from a slot of the ring that
+// holds the aligned vectors around them (VEC: the vectors themselves)
+template <typename T, typename X, bool VEC>
+__device__ __forceinline__ void read_slot(const char *slot, const X *row, int c0, int lane, int H, uint64_t *v) {
     constexpr int N2 = kPairs<T>;
-    const uint64_t by = pair(scale, scale);
+    if constexpr (VEC) {
+#pragma unroll
+        for (int i = 0; i < N2 / kPairs<X>; ++i)
+            unpack<X>(reinterpret_cast<const uint4 *>(slot)[lane * (N2 / kPairs<X>) + i], v + i * kPairs<X>);
+    } else {
+        const X *t = reinterpret_cast<const X *>(slot + ((uintptr_t)(row + c0) & 15)) + lane;
+#pragma unroll
+        for (int k = 0; k < N2; ++k) {
+            const int c = c0 + lane + 64 * k;
+            v[k] = pair(c < H ? to_f(t[64 * k]) : 0.0f, c + 32 < H ? to_f(t[64 * k + 32]) : 0.0f);
+        }
+    }
+}
+
+// the lane's sums into its columns of a row
+template <typename T, typename X, bool VEC>
+__device__ __forceinline__ void put_row(X *__restrict__ row, int c0, int lane, int H, const uint64_t *v) {
+    constexpr int N2 = kPairs<T>;
     if constexpr (VEC) {             // one or two vectors
         const int c = c0 + lane * 2 * N2;
         if (c >= H) return;
-        uint4 *to = reinterpret_cast<uint4 *>(g + c);
 #pragma unroll
-        for (int i = 0; i < N2 / kPairs<G>; ++i) {
-            uint64_t v[kPairs<G>];
-            if (add) unpack<G>(to[i], v);
-#pragma unroll
-            for (int k = 0; k < kPairs<G>; ++k) {
-                const uint64_t s = acc[i * kPairs<G> + k];
-                v[k] = add ? fma2(s, by, v[k]) : mul2(s, by);
-            }
-            to[i] = pack<G>(v);
-        }
+        for (int i = 0; i < N2 / kPairs<X>; ++i) reinterpret_cast<uint4 *>(row + c)[i] = pack<X>(v + i * kPairs<X>);
     } else {
 #pragma unroll
         for (int k = 0; k < N2; ++k) {
-            const float2 h = halves(acc[k]);
+            const float2 h = halves(v[k]);
             const int c = c0 + lane + 64 * k;
-            if (c < H) g[c] = from_f<G>(add ? fmaf(h.x, scale, to_f(g[c])) : h.x * scale);
-            if (c + 32 < H) g[c + 32] = from_f<G>(add ? fmaf(h.y, scale, to_f(g[c + 32])) : h.y * scale);
+            if (c < H) row[c] = from_f<X>(h.x);
+            if (c + 32 < H) row[c + 32] = from_f<X>(h.y);
         }
     }
 }
 
 // One warp per chunk and slab.  The chunk's rows come through a ring of kAhead
-// slots of 16 bytes a lane in shared memory, filled by asynchronous copies (of 16
-// bytes, or of 4 where fp32 rows are not aligned), so that 15 rows are on their
-// way whatever the tokens are; 16-bit rows that are not aligned are loaded eight at
-// a time.
+// slots in shared memory, filled by asynchronous copies of 16 bytes, so that many
+// rows are on their way whatever the tokens are; where the sums are added to a
+// gradient, its row follows a token's last row through the same ring (loaded where
+// it was needed, its latency once a token took two thirds of the time).  Of a row
+// that is not aligned the 16-byte vectors around the slab are fetched: each holds
+// a value of the row, so it lies in the tensor's memory.
 constexpr int kAhead = 16;
 
 template <typename T, typename G, bool VEC>
@@ -276,8 +313,8 @@ __global__ void __launch_bounds__(256)
 embed_sum_kernel(const T *__restrict__ dy, const uint32_t *__restrict__ key, const uint32_t *__restrict__ pos,
                  uint32_t tokens, uint32_t V, int H, float scale, int add, G *__restrict__ grad,
                  float *__restrict__ part) {
-    extern __shared__ uint4 dyn[];   // [kAhead][256 threads]
-    constexpr int N = kLaneN<T>, N2 = N / 2;
+    constexpr int N = kLaneN<T>, N2 = N / 2, kSlot = 32 * N * (int)sizeof(G) + (VEC ? 0 : 16);
+    extern __shared__ uint4 dyn[];   // [8 warps][kAhead][kSlot bytes]
     wait_for_previous();
     let_next_start();
     const int slabs = (H + 32 * N - 1) / (32 * N);
@@ -292,123 +329,129 @@ embed_sum_kernel(const T *__restrict__ dy, const uint32_t *__restrict__ key, con
     const uint32_t before = b ? key[b - 1] : V, after = b + n < tokens ? key[b + n] : V;
     const int live = __popc(__ballot_sync(0xffffffffu, k_l < V));     // row V sorts behind the others
     if (!live) return;
-    uint4 *ring = dyn + threadIdx.x;
+    // bit i: position i is its token's last in this chunk; begun before it, going on behind it
+    const uint32_t follows = __shfl_down_sync(0xffffffffu, k_l, 1), first = __shfl_sync(0xffffffffu, k_l, 0);
+    const uint32_t last = __ballot_sync(0xffffffffu, lane < live && (lane == live - 1 || follows != k_l));
+    const uint32_t from = __ballot_sync(0xffffffffu, k_l == first && first == before);
+    const uint32_t on = __ballot_sync(0xffffffffu, live == n && k_l == after);
+    const uint32_t whole = last & ~from & ~on, with = add ? whole : 0;    // rows to write; gradient rows to read first
+    char *ring = reinterpret_cast<char *>(dyn) + (threadIdx.x >> 5) * (kAhead * kSlot);
     const uint32_t at = (uint32_t)__cvta_generic_to_shared(ring);
-    auto fetch = [&](int i) {        // row i of the chunk into slot i % kAhead
-        if constexpr (VEC || sizeof(T) == 4) {
-            const uint32_t p = __shfl_sync(0xffffffffu, p_l, i & 31), to = at + (i % kAhead) * 4096;
-            if (i < live) {
-                const T *row = dy + (int64_t)p * H + c0;
-                if constexpr (VEC) {
-                    if (c0 + lane * N < H)
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(row + lane * N) : "memory");
+    auto copy_row = [&](int slot, const char *row, int bytes) {
+        const int shift = VEC ? 0 : (int)((uintptr_t)row & 15);
+        for (int i = lane * 16; i < bytes + shift; i += 512)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + slot * kSlot + i), "l"(row - shift + i)
+                         : "memory");
+    };
+    const int width = min(32 * N, H - c0);
+    int f_row = 0, f_slot = 0;       // next to fetch: the row of position f_row, or the gradient row behind it
+    bool f_grad = false;
+    auto fetch = [&] {
+        const uint32_t p = __shfl_sync(0xffffffffu, p_l, f_row & 31), k = __shfl_sync(0xffffffffu, k_l, f_row & 31);
+        if (f_row < live) {
+            if (f_grad) copy_row(f_slot, reinterpret_cast<const char *>(grad + (int64_t)k * H + c0), width * (int)sizeof(G));
+            else copy_row(f_slot, reinterpret_cast<const char *>(dy + (int64_t)p * H + c0), width * (int)sizeof(T));
+            f_grad = !f_grad && (with >> f_row & 1);
+            f_row += !f_grad;
+            f_slot = f_slot == kAhead - 1 ? 0 : f_slot + 1;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    int slot = 0;
+    // the next slot is there, and every lane has read the one that is filled now
+    auto next = [&] {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 2) : "memory");
+        __syncwarp();
+        fetch();
+        const char *s = ring + slot * kSlot;
+        slot = slot == kAhead - 1 ? 0 : slot + 1;
+        return s;
+    };
+    for (int i = 0; i < kAhead - 1; ++i) fetch();
+    uint64_t acc[N2], v[N2];
+#pragma unroll
+    for (int k = 0; k < N2; ++k) acc[k] = 0;
+    for (int i = 0; i < live; ++i) {
+        const uint32_t p = __shfl_sync(0xffffffffu, p_l, i), token = __shfl_sync(0xffffffffu, k_l, i);
+        read_slot<T, T, VEC>(next(), dy + (int64_t)p * H, c0, lane, H, v);
+#pragma unroll
+        for (int k = 0; k < N2; ++k) acc[k] = add2(acc[k], v[k]);
+        if (last >> i & 1) {
+            if (whole >> i & 1) {
+                G *row = grad + (int64_t)token * H;
+                const uint64_t by = pair(scale, scale);
+                if (add) {
+                    read_slot<T, G, VEC>(next(), row, c0, lane, H, v);
+#pragma unroll
+                    for (int k = 0; k < N2; ++k) acc[k] = fma2(acc[k], by, v[k]);
                 } else {
 #pragma unroll
-                    for (int k = 0; k < N; ++k)
-                        if (c0 + lane + 32 * k < H)
-                            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + 4 * k),
-                                         "l"(row + lane + 32 * k)
-                                         : "memory");
+                    for (int k = 0; k < N2; ++k) acc[k] = mul2(acc[k], by);
                 }
+                put_row<T, G, VEC>(row, c0, lane, H, acc);
+            } else {                 // slot 0: begun before this chunk, 1: begins in it
+                put_row<T, float, VEC>(part + (chunk * 2 + (from >> i & 1 ? 0 : 1)) * H, c0, lane, H, acc);
             }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        }
-    };
-    for (int i = 0; i < kAhead - 1; ++i) fetch(i);
-    uint64_t acc[N2];
-    uint32_t cur = V, first = V;
-    for (int i = 0; i <= live; ++i) {
-        const uint32_t k_i = __shfl_sync(0xffffffffu, k_l, i & 31);
-        if (i == live || k_i != cur) {
-            if (i > 0) {             // the row of `cur` is complete in this chunk
-                const bool from = cur == before && cur == first, on = i == live && live == n && cur == after;
-                if (!from && !on) {
-                    put_row<T, G, VEC>(grad + (int64_t)cur * H, c0, lane, H, acc, scale, add);
-                } else {             // slot 0: begun before this chunk, 1: begins in it
-                    put_row<T, float, VEC>(part + (chunk * 2 + (from ? 0 : 1)) * H, c0, lane, H, acc, 1.0f, 0);
-                }
-            } else {
-                first = k_i;
-            }
-            if (i == live) break;
-            cur = k_i;
 #pragma unroll
             for (int k = 0; k < N2; ++k) acc[k] = 0;
         }
-        if constexpr (!VEC && sizeof(T) == 2) {
-            if (i % 8 == 0) {
-                T v[8][N];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const uint32_t p = __shfl_sync(0xffffffffu, p_l, i + j);
-                    if (i + j < live)
-#pragma unroll
-                        for (int k = 0; k < N; ++k)
-                            v[j][k] = c0 + lane + 32 * k < H ? dy[(int64_t)p * H + c0 + lane + 32 * k] : T();
-                }
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (i + j < live) {
-                        uint4 u;
-#pragma unroll
-                        for (int k = 0; k < N; ++k) reinterpret_cast<T *>(&u)[k] = v[j][k];
-                        ring[((i + j) % kAhead) * 256] = u;
-                    }
-            }
-        } else {
-            fetch(i + kAhead - 1);
-            asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
-        }
-        uint64_t v[N2];
-        unpack<T>(ring[(i % kAhead) * 256], v);
-#pragma unroll
-        for (int k = 0; k < N2; ++k) acc[k] = add2(acc[k], v[k]);
     }
 }
 
 // A CTA looks at 8 chunks, one a warp: where a chunk's last token begins in it and
 // goes on, the chunks that it runs through are counted.  A token of few chunks is
-// joined by its warp, 32 columns at a time; of many (a run of hundreds of partial
+// joined by its warp, 128 columns a CTA; of many (a run of hundreds of partial
 // sums) by all 8 warps, each a contiguous part, which are then added in order.
 template <typename G>
 __global__ void __launch_bounds__(256)
 embed_join_kernel(const uint32_t *__restrict__ key, uint32_t tokens, uint32_t V, int H, float scale, int add,
                   G *__restrict__ grad, const float *__restrict__ part, int64_t chunks) {
-    __shared__ float s[8][32];
+    __shared__ float s[8][128];
     __shared__ int follow[8];
     __shared__ uint32_t token[8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    constexpr int kFew = 12;
+    constexpr int kFew = 16;
+    const int c0 = blockIdx.y * 128 + lane;             // columns c0, c0 + 32, c0 + 64, c0 + 96
     auto put = [&](uint32_t k, int c, float v) {
         G *g = grad + (int64_t)k * H + c;
         *g = from_f<G>(add ? fmaf(v, scale, to_f(*g)) : v * scale);
     };
+    // partial sums [i0, i1) of a token that begins in `chunk`, in order
+    auto sums = [&](int64_t chunk, int i0, int i1, float *t) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) t[j] = 0.0f;
+#pragma unroll 4
+        for (int i = i0; i < i1; ++i) {
+            const float *p = part + ((chunk + i) * 2 + (i == 0 ? 1 : 0)) * H;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (c0 + 32 * j < H) t[j] += p[c0 + 32 * j];
+        }
+    };
+    float t[4];
     wait_for_previous();
     const int64_t mine = (int64_t)blockIdx.x * 8 + warp;
     int n = 0;
     if (mine < chunks - 1) {
         const uint32_t b = (uint32_t)(mine * kChunk), e = b + kChunk;
-        const uint32_t k = key[e - 1];
-        if (k < V && key[e] == k && !(key[b] == k && b > 0 && key[b - 1] == k)) {
-            for (;;) {               // chunks that begin with this token
-                const uint64_t p = (uint64_t)e + (uint64_t)(n + lane) * kChunk;
-                const int got = __popc(__ballot_sync(0xffffffffu, p < tokens && key[p] == k));
+        // the keys around, and those that the chunks behind begin with
+        const uint32_t k = key[e - 1], front = key[b], before = b ? key[b - 1] : V;
+        uint64_t p = (uint64_t)e + (uint64_t)lane * kChunk;
+        uint32_t ahead = p < tokens ? key[p] : V;
+        if (k < V && !(front == k && before == k)) {
+            for (;;) {
+                const int got = __popc(__ballot_sync(0xffffffffu, ahead == k));
                 n += got;
                 if (got < 32) break;
+                p += 32 * kChunk;
+                ahead = p < tokens ? key[p] : V;
             }
         }
         if (n > 0 && n <= kFew) {
-            for (int c = blockIdx.y * 32 + lane; c < H; c += gridDim.y * 32) {
-                float v[kFew + 1];
+            sums(mine, 0, n + 1, t);
 #pragma unroll
-                for (int i = 0; i <= kFew; ++i)
-                    v[i] = i <= n ? part[((mine + i) * 2 + (i == 0 ? 1 : 0)) * H + c] : 0.0f;
-                float t = v[0];
-#pragma unroll
-                for (int i = 1; i <= kFew; ++i)
-                    if (i <= n) t += v[i];
-                put(k, c, t);
-            }
+            for (int j = 0; j < 4; ++j)
+                if (c0 + 32 * j < H) put(k, c0 + 32 * j, t[j]);
             n = 0;
         }
         if (lane == 0) token[warp] = k;
@@ -418,24 +461,17 @@ embed_join_kernel(const uint32_t *__restrict__ key, uint32_t tokens, uint32_t V,
     for (int w = 0; w < 8; ++w) {
         const int m = follow[w] + 1, each = (m + 7) / 8;
         if (m == 1) continue;
-        const int64_t chunk = (int64_t)blockIdx.x * 8 + w;
-        for (int c = blockIdx.y * 32 + lane; c - lane < H; c += gridDim.y * 32) {
-            float v = 0.0f;
-            if (c < H) {
-#pragma unroll 8
-                for (int i = warp * each; i < min(m, (warp + 1) * each); ++i)
-                    v += part[((chunk + i) * 2 + (i == 0 ? 1 : 0)) * H + c];
-            }
-            s[warp][lane] = v;
-            __syncthreads();
-            if (warp == 0 && c < H) {
-                float t = 0.0f;
+        sums((int64_t)blockIdx.x * 8 + w, min(m, warp * each), min(m, (warp + 1) * each), t);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) t += s[i][lane];
-                put(token[w], c, t);
-            }
-            __syncthreads();
+        for (int j = 0; j < 4; ++j) s[warp][lane + 32 * j] = t[j];
+        __syncthreads();
+        if (threadIdx.x < 128 && blockIdx.y * 128 + threadIdx.x < H) {
+            float v = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v += s[i][threadIdx.x];
+            put(token[w], blockIdx.y * 128 + threadIdx.x, v);
         }
+        __syncthreads();
     }
 }
 
@@ -470,18 +506,19 @@ template <typename T, typename G> static int embed_bwd(const EmbedBwd &a, cudaSt
     s.passes = (bits + 8) / 9;
     s.width = (bits + s.passes - 1) / s.passes;
     s.err = a.err;
-    s.zero = static_cast<char *>(a.grad);
-    s.zero_bytes = a.add ? 0 : a.V * (int64_t)a.H * (int64_t)sizeof(G);
-    // two CTAs per SM write zeros, fewer where that is less than 16 KB each
-    const int64_t fill = std::min<int64_t>(36, (s.zero_bytes + kSortCtas * 16384 - 1) / (kSortCtas * 16384));
-    const int bins = 1 << s.width, smem = (kSortWarps + 2) * bins * 4;
-    if (smem > 48 * 1024 && cudaFuncSetAttribute(embed_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 (kSortWarps + 2) * kMaxBins * 4) != cudaSuccess) {
+    const int bins = 1 << s.width, smem = (kSortWarps + 6) * bins * 4;
+    if (smem > 47 * 1024 && cudaFuncSetAttribute(embed_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 (kSortWarps + 6) * kMaxBins * 4) != cudaSuccess) {
         (void)cudaGetLastError();
         return USAF_ECUDA;
     }
-    embed_sort_kernel<<<(unsigned)(kSortCtas * (1 + fill)), kSortThreads, smem, st>>>(s);
-    USAF_CHECK_LAUNCH();
+    if (a.tokens) {
+        embed_sort_kernel<<<kSortCtas, kSortThreads, smem, st>>>(s);
+        USAF_CHECK_LAUNCH();
+    }
+    const int64_t zero = a.add ? 0 : a.V * (int64_t)a.H * (int64_t)sizeof(G);
+    if (zero && !launch_early(embed_zero_kernel, dim3(cdiv(zero + 1, kZeroTile)), kZeroThreads, 0, st, (char *)a.grad, zero))
+        return USAF_ECUDA;
     if (a.tokens == 0) return USAF_OK;
     const uint32_t *key = s.key[(s.passes - 1) & 1], *pos = s.pos[(s.passes - 1) & 1];
     const int64_t chunks = (a.tokens + kChunk - 1) / kChunk;
@@ -490,7 +527,7 @@ template <typename T, typename G> static int embed_bwd(const EmbedBwd &a, cudaSt
     // 16-byte vectors of dy's rows, of the gradient's and of the partial sums
     const bool vec = ((uintptr_t)a.dy | (uintptr_t)a.grad | (uintptr_t)a.ws) % 16 == 0 && (int64_t)a.H * sizeof(T) % 16 == 0;
     auto sum = vec ? embed_sum_kernel<T, G, true> : embed_sum_kernel<T, G, false>;
-    const int ring = kAhead * 256 * 16;
+    const int ring = 8 * kAhead * (32 * kLaneN<T> * (int)sizeof(G) + (vec ? 0 : 16));
     if (cudaFuncSetAttribute(sum, cudaFuncAttributeMaxDynamicSharedMemorySize, ring) != cudaSuccess) {
         (void)cudaGetLastError();
         return USAF_ECUDA;
@@ -499,7 +536,7 @@ template <typename T, typename G> static int embed_bwd(const EmbedBwd &a, cudaSt
                       a.scale, a.add, (G *)a.grad, part))
         return USAF_ECUDA;
     if (chunks > 1) {
-        const dim3 jgrid(cdiv(chunks - 1, 8), (unsigned)std::min((a.H + 31) / 32, 64));
+        const dim3 jgrid(cdiv(chunks - 1, 8), cdiv(a.H, 128));
         if (!launch_early(embed_join_kernel<G>, jgrid, 256, 0, st, key, (uint32_t)a.tokens, (uint32_t)a.V, a.H, a.scale,
                           a.add, (G *)a.grad, (const float *)part, chunks))
             return USAF_ECUDA;
@@ -510,7 +547,7 @@ template <typename T, typename G> static int embed_bwd(const EmbedBwd &a, cudaSt
 template <typename T>
 static void embed_fwd(const void *ids, int ids64, int64_t tokens, const void *table, int64_t V, int H, float scale,
                       void *out, int32_t *err, cudaStream_t st) {
-    const int group = 32 * kLaneN<T> * 4;
+    const int group = 32 * kLaneN<T> * kFwdSlabs;
     const unsigned grid = cdiv(tokens * ((H + group - 1) / group), 8);
     const bool vec = ((uintptr_t)table | (uintptr_t)out) % 16 == 0 && (int64_t)H * sizeof(T) % 16 == 0;
     if (vec)
@@ -554,7 +591,8 @@ extern "C" int usaf_embedding_bwd(const void *dy, const void *ids, int32_t ids_b
                                   void *grad, int32_t grad_dtype, void *ws, int32_t *err, void *stream) {
     USAF_REQUIRE(tokens >= 0 && V >= 0 && H >= 1 && (ids_bits == 32 || ids_bits == 64));
     USAF_REQUIRE((grad || V == 0) && (tokens == 0 || (dy && ids && ws)));
-    if (tokens > kMostTokens || V > kMostRows || (tokens / kChunk + 1) * ((H + 127) / 128) > ((int64_t)1 << 33))
+    if (tokens > kMostTokens || V > kMostRows || H > (1 << 22) ||
+        (tokens / kChunk + 1) * ((H + 127) / 128) > ((int64_t)1 << 33))
         return USAF_EUNSUPPORTED;
     cudaStream_t st = as_stream(stream);
     const EmbedBwd a{dy, ids, ids_bits == 64, tokens, V, H, (float)scale, padding_idx, accumulate, grad, ws, err};
