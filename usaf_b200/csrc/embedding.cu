@@ -90,7 +90,7 @@ struct SortArgs {
     int64_t V, pad;
     uint32_t tokens;
     int passes, width;          // digits of `width` bits
-    uint32_t *key[2], *pos[2];  // pass i writes buffer i & 1
+    uint2 *pairs[2];            // (key, position); pass i writes buffer i & 1
     int32_t *err;
 };
 
@@ -158,18 +158,18 @@ embed_sort_kernel(const SortArgs a) {
     const bool once = part <= 32 * kRound;              // a warp's pairs stay in its registers for a pass
     const int split = min(4, kSortThreads / bins);      // threads that scan a digit's counts of the warps
     for (int pass = 0; pass < a.passes; ++pass) {
-        const uint32_t *ksrc = a.key[(pass + 1) & 1], *psrc = a.pos[(pass + 1) & 1];
-        uint32_t *kdst = a.key[pass & 1], *pdst = a.pos[pass & 1];
+        const uint2 *src = a.pairs[(pass + 1) & 1];
+        uint2 *dst = a.pairs[pass & 1];
         const int shift = pass * a.width;
-        uint32_t key[kRound], pos[kRound];
+        uint2 item[kRound];                             // and the lanes with the same digit
+        uint32_t same[kRound];
+#pragma unroll
+        for (int r = 0; r < kRound; ++r) item[r] = make_uint2(0, 0);
         auto load = [&](uint32_t j0) {
 #pragma unroll
             for (int r = 0; r < kRound; ++r) {
                 const uint32_t j = j0 + 32 * r + lane;
-                if (j < e) {
-                    key[r] = pass ? ksrc[j] : sort_key(a, j);
-                    pos[r] = pass ? psrc[j] : j;
-                }
+                if (j < e) item[r] = pass ? src[j] : make_uint2(sort_key(a, j), j);
             }
         };
         for (int i = tid; i < kSortWarps * bins; i += kSortThreads) hist[i] = 0;
@@ -181,9 +181,9 @@ embed_sort_kernel(const SortArgs a) {
             for (int r = 0; r < kRound; ++r) {
                 if (j0 + 32 * r >= e) break;
                 const bool in = j0 + 32 * r + lane < e;
-                const uint32_t d = in ? (key[r] >> shift) & (bins - 1) : bins;
-                const uint32_t same = same_digit(d, a.width + 1);
-                if (in && lane == __ffs(same) - 1) mine[d] += __popc(same);
+                const uint32_t d = (item[r].x >> shift) & (bins - 1);
+                same[r] = same_digit(d, a.width) & __ballot_sync(0xffffffffu, in);
+                if (in && lane == __ffs(same[r]) - 1) mine[d] += __popc(same[r]);
                 __syncwarp();
             }
         }
@@ -243,14 +243,13 @@ embed_sort_kernel(const SortArgs a) {
             for (int r = 0; r < kRound; ++r) {
                 if (j0 + 32 * r >= e) break;
                 const bool in = j0 + 32 * r + lane < e;
-                const uint32_t d = in ? (key[r] >> shift) & (bins - 1) : bins;
-                const uint32_t same = same_digit(d, a.width + 1);
-                const uint32_t to = in ? base[d] + mine[d] + __popc(same & ((1u << lane) - 1)) : 0;
+                const uint32_t d = (item[r].x >> shift) & (bins - 1);
+                if (!once) same[r] = same_digit(d, a.width) & __ballot_sync(0xffffffffu, in);
+                const uint32_t to = base[d] + mine[d] + __popc(same[r] & ((1u << lane) - 1));
                 __syncwarp();
                 if (in) {
-                    if (lane == __ffs(same) - 1) mine[d] += __popc(same);
-                    kdst[to] = key[r];
-                    pdst[to] = pos[r];
+                    if (lane == __ffs(same[r]) - 1) mine[d] += __popc(same[r]);
+                    dst[to] = item[r];
                 }
                 __syncwarp();
             }
@@ -310,9 +309,8 @@ constexpr int kAhead = 16;
 
 template <typename T, typename G, bool VEC>
 __global__ void __launch_bounds__(256)
-embed_sum_kernel(const T *__restrict__ dy, const uint32_t *__restrict__ key, const uint32_t *__restrict__ pos,
-                 uint32_t tokens, uint32_t V, int H, float scale, int add, G *__restrict__ grad,
-                 float *__restrict__ part) {
+embed_sum_kernel(const T *__restrict__ dy, const uint2 *__restrict__ sorted, uint32_t tokens, uint32_t V, int H,
+                 float scale, int add, G *__restrict__ grad, float *__restrict__ part) {
     constexpr int N = kLaneN<T>, N2 = N / 2, kSlot = 32 * N * (int)sizeof(G) + (VEC ? 0 : 16);
     extern __shared__ uint4 dyn[];   // [8 warps][kAhead][kSlot bytes]
     wait_for_previous();
@@ -325,8 +323,9 @@ embed_sum_kernel(const T *__restrict__ dy, const uint32_t *__restrict__ key, con
     const uint32_t b = (uint32_t)min((uint64_t)chunk * kChunk, (uint64_t)tokens);
     const int n = (int)min((uint32_t)kChunk, tokens - b);
     if (n <= 0) return;
-    const uint32_t k_l = lane < n ? key[b + lane] : V, p_l = lane < n ? pos[b + lane] : 0;
-    const uint32_t before = b ? key[b - 1] : V, after = b + n < tokens ? key[b + n] : V;
+    const uint2 own = lane < n ? sorted[b + lane] : make_uint2(V, 0);
+    const uint32_t k_l = own.x, p_l = own.y;
+    const uint32_t before = b ? sorted[b - 1].x : V, after = b + n < tokens ? sorted[b + n].x : V;
     const int live = __popc(__ballot_sync(0xffffffffu, k_l < V));     // row V sorts behind the others
     if (!live) return;
     // bit i: position i is its token's last in this chunk; begun before it, going on behind it
@@ -404,7 +403,7 @@ embed_sum_kernel(const T *__restrict__ dy, const uint32_t *__restrict__ key, con
 // sums) by all 8 warps, each a contiguous part, which are then added in order.
 template <typename G>
 __global__ void __launch_bounds__(256)
-embed_join_kernel(const uint32_t *__restrict__ key, uint32_t tokens, uint32_t V, int H, float scale, int add,
+embed_join_kernel(const uint2 *__restrict__ sorted, uint32_t tokens, uint32_t V, int H, float scale, int add,
                   G *__restrict__ grad, const float *__restrict__ part, int64_t chunks) {
     __shared__ float s[8][128];
     __shared__ int follow[8];
@@ -435,16 +434,16 @@ embed_join_kernel(const uint32_t *__restrict__ key, uint32_t tokens, uint32_t V,
     if (mine < chunks - 1) {
         const uint32_t b = (uint32_t)(mine * kChunk), e = b + kChunk;
         // the keys around, and those that the chunks behind begin with
-        const uint32_t k = key[e - 1], front = key[b], before = b ? key[b - 1] : V;
+        const uint32_t k = sorted[e - 1].x, front = sorted[b].x, before = b ? sorted[b - 1].x : V;
         uint64_t p = (uint64_t)e + (uint64_t)lane * kChunk;
-        uint32_t ahead = p < tokens ? key[p] : V;
+        uint32_t ahead = p < tokens ? sorted[p].x : V;
         if (k < V && !(front == k && before == k)) {
             for (;;) {
                 const int got = __popc(__ballot_sync(0xffffffffu, ahead == k));
                 n += got;
                 if (got < 32) break;
                 p += 32 * kChunk;
-                ahead = p < tokens ? key[p] : V;
+                ahead = p < tokens ? sorted[p].x : V;
             }
         }
         if (n > 0 && n <= kFew) {
@@ -485,7 +484,7 @@ static inline int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
 
 static int64_t embed_ws_bytes(int64_t tokens, int H) {
     const int64_t chunks = (tokens + kChunk - 1) / kChunk;
-    return 4 * up256(tokens * 4) + (chunks > 1 ? chunks * 2 * H * 4 : 0);
+    return 2 * up256(tokens * 8) + (chunks > 1 ? chunks * 2 * H * 4 : 0);
 }
 
 template <typename T, typename G> static int embed_bwd(const EmbedBwd &a, cudaStream_t st) {
@@ -496,11 +495,8 @@ template <typename T, typename G> static int embed_bwd(const EmbedBwd &a, cudaSt
     s.pad = a.pad;
     s.tokens = (uint32_t)a.tokens;
     char *w = static_cast<char *>(a.ws);
-    for (int i = 0; i < 2; ++i) {
-        s.key[i] = reinterpret_cast<uint32_t *>(w + (2 * i) * up256(a.tokens * 4));
-        s.pos[i] = reinterpret_cast<uint32_t *>(w + (2 * i + 1) * up256(a.tokens * 4));
-    }
-    float *part = reinterpret_cast<float *>(w + 4 * up256(a.tokens * 4));
+    for (int i = 0; i < 2; ++i) s.pairs[i] = reinterpret_cast<uint2 *>(w + i * up256(a.tokens * 8));
+    float *part = reinterpret_cast<float *>(w + 2 * up256(a.tokens * 8));
     int bits = 1;                                      // of row V, the last key
     while ((a.V >> bits) != 0) ++bits;
     s.passes = (bits + 8) / 9;
@@ -520,7 +516,7 @@ template <typename T, typename G> static int embed_bwd(const EmbedBwd &a, cudaSt
     if (zero && !launch_early(embed_zero_kernel, dim3(cdiv(zero + 1, kZeroTile)), kZeroThreads, 0, st, (char *)a.grad, zero))
         return USAF_ECUDA;
     if (a.tokens == 0) return USAF_OK;
-    const uint32_t *key = s.key[(s.passes - 1) & 1], *pos = s.pos[(s.passes - 1) & 1];
+    const uint2 *sorted = s.pairs[(s.passes - 1) & 1];
     const int64_t chunks = (a.tokens + kChunk - 1) / kChunk;
     const int slabs = (a.H + 32 * kLaneN<T> - 1) / (32 * kLaneN<T>);
     const unsigned grid = cdiv(chunks * slabs, 8);
@@ -532,12 +528,12 @@ template <typename T, typename G> static int embed_bwd(const EmbedBwd &a, cudaSt
         (void)cudaGetLastError();
         return USAF_ECUDA;
     }
-    if (!launch_early(sum, dim3(grid), 256, ring, st, (const T *)a.dy, key, pos, (uint32_t)a.tokens, (uint32_t)a.V, a.H,
+    if (!launch_early(sum, dim3(grid), 256, ring, st, (const T *)a.dy, sorted, (uint32_t)a.tokens, (uint32_t)a.V, a.H,
                       a.scale, a.add, (G *)a.grad, part))
         return USAF_ECUDA;
     if (chunks > 1) {
         const dim3 jgrid(cdiv(chunks - 1, 8), cdiv(a.H, 128));
-        if (!launch_early(embed_join_kernel<G>, jgrid, 256, 0, st, key, (uint32_t)a.tokens, (uint32_t)a.V, a.H, a.scale,
+        if (!launch_early(embed_join_kernel<G>, jgrid, 256, 0, st, sorted, (uint32_t)a.tokens, (uint32_t)a.V, a.H, a.scale,
                           a.add, (G *)a.grad, (const float *)part, chunks))
             return USAF_ECUDA;
     }
