@@ -747,7 +747,7 @@ def run_c5(steps: int = 10, warmup: int = 3):
                       "steps": steps, "warmup": warmup, "data": "synthetic"}), flush=True)
 
 
-def run_c3(n_layers: int = 2, steps: int = 5, warmup: int = 2, recompute: bool = True):
+def run_c3(n_layers: int = 2, steps: int = 5, warmup: int = 2, recompute: bool = True, dense: str = ""):
     """BASELINE configs[2] (C3), on one GPU or, under torchrun, with the experts
     sharded over the ranks (each rank its own micro-batch): a random-init Qwen3MoeForCausalLM
     with the C3 shapes (H 2048, 32/4 heads, head dim 128, E 128, top-8, I 768,
@@ -760,7 +760,11 @@ def run_c3(n_layers: int = 2, steps: int = 5, warmup: int = 2, recompute: bool =
     share their backward-only buffers, the pair buffers hold 1.25 x top_k
     pairs per token, and (``recompute``, as the reference's loader enables,
     usaf/moe_loader.py:758-760) each decoder layer's activations are
-    recomputed in the backward.  One JSON line with the whole-model tokens/s."""
+    recomputed in the backward.  ``dense``: "kernels" runs the norms, residual
+    additions and embedding on the device kernels (qwen3moe.use_dense_kernels);
+    "train" also trains them and the gates whole (SparseTrainer's dense_names, 8-bit
+    AdamW states); "torch-train" trains the same tensors on torch's operations
+    (torch.optim.AdamW).  One JSON line with the whole-model tokens/s."""
     from transformers.models.qwen3_moe.configuration_qwen3_moe import Qwen3MoeConfig
     from transformers.models.qwen3_moe.modeling_qwen3_moe import Qwen3MoeForCausalLM
     from usaf_b200 import qwen3moe
@@ -811,8 +815,27 @@ def run_c3(n_layers: int = 2, steps: int = 5, warmup: int = 2, recompute: bool =
     gt = torch.Generator(device=dev).manual_seed(4 + rank)
     batches = [torch.randint(0, V, (MB, S), device=dev, generator=gt) for _ in range(2)]
     lm = lambda m, ids: m(input_ids=ids, labels=ids).loss  # noqa: E731
-    tr = SparseTrainer(model, steps=1000, lr_peak=2e-4, accum=1, frac=0.005, reselect_every=10 ** 9)
+    names = [n for n, _ in model.named_parameters() if "norm" in n or "embed_tokens" in n or n.endswith("gate.weight")]
+    if dense in ("kernels", "train"):
+        qwen3moe.use_dense_kernels(model)
+    tr = SparseTrainer(model, steps=1000, lr_peak=2e-4, accum=1, frac=0.005, reselect_every=10 ** 9,
+                       train_router=dense != "torch-train", dense_names=names if dense == "train" else None,
+                       dense_state_bits=8)
     tr.init_selection(tr.importance(batches[0], lm))
+    if dense == "torch-train":
+        ps = [p_ for n, p_ in model.named_parameters() if n in set(names)]
+        for p_ in ps:
+            p_.requires_grad_(True)
+        adamw = torch.optim.AdamW(ps, lr=2e-4, weight_decay=0.005)
+        own = tr.train_step
+
+        def train_step(mbs, fn):
+            out = own(mbs, fn)
+            adamw.step()
+            adamw.zero_grad()
+            return out
+
+        tr.train_step = train_step
     for i in range(warmup):
         tr.train_step([batches[i % 2]], lm)
     torch.cuda.synchronize()
@@ -836,7 +859,7 @@ def run_c3(n_layers: int = 2, steps: int = 5, warmup: int = 2, recompute: bool =
                       "parallelism": f"ep{world}" if world > 1 else "single",
                       "tokens_per_step": world * MB * S,
                       "step_ms": ms, "tokens_per_s": world * MB * S / (ms * 1e-3),
-                      "ms_per_layer_incl_head": ms / n_layers, "activation_recompute": recompute,
+                      "ms_per_layer_incl_head": ms / n_layers, "activation_recompute": recompute, "dense": dense or "torch, frozen",
                       "max_memory_gb": torch.cuda.max_memory_allocated(dev) / 1e9,
                       "losses": [round(l_["loss"], 4) for l_ in logs],
                       "all_finite": all(l_["finite"] for l_ in logs), "steps": steps, "warmup": warmup,
@@ -872,6 +895,8 @@ def main():
                     help="Mixtral-8x22B-shaped layer: importance pass + sparse steps (1 GPU)")
     ap.add_argument("--c3", type=int, default=0, metavar="LAYERS",
                     help="C3-shaped causal LM with this many layers through SparseTrainer (1 GPU)")
+    ap.add_argument("--c3-dense", default="", choices=["", "kernels", "train", "torch-train"],
+                    help="norms and embedding of --c3: on the device kernels, trained too, or trained on torch's operations")
     ap.add_argument("--c3-no-recompute", action="store_true",
                     help="keep every decoder layer's activations instead of recomputing them")
     args = ap.parse_args()
@@ -887,7 +912,7 @@ def main():
         run_c5()
         return
     if args.c3:
-        run_c3(args.c3, recompute=not args.c3_no_recompute)
+        run_c3(args.c3, recompute=not args.c3_no_recompute, dense=args.c3_dense)
         return
     world = int(os.environ.get("WORLD_SIZE", "1"))
     rank = int(os.environ.get("RANK", "0"))

@@ -259,19 +259,23 @@ embed_sort_kernel(const SortArgs a) {
 }
 
 // ---- backward: sums -----------------------------------------------------------
-// a lane's columns of a row of T or of the gradient, from a slot of the ring that
-// holds the aligned vectors around them (VEC: the vectors themselves)
-template <typename T, typename X, bool VEC>
-__device__ __forceinline__ void read_slot(const char *slot, const X *row, int c0, int lane, int H, uint64_t *v) {
-    constexpr int N2 = kPairs<T>;
+// A slab is 32 lanes times NV vectors of 16 bytes of T; a lane's values are those
+// of vectors lane, 32 + lane, ... (VEC), else every 32nd column.  From a slot of the
+// ring that holds a row of X (T, or the gradient's fp32) of the slab, `shift` bytes
+// behind the slot's beginning:
+template <typename T, typename X, int NV, bool VEC>
+__device__ __forceinline__ void read_slot(const char *slot, int shift, int c0, int lane, int H, uint64_t *v) {
+    constexpr int N2 = kPairs<T>, R = N2 / kPairs<X>;
     if constexpr (VEC) {
 #pragma unroll
-        for (int i = 0; i < N2 / kPairs<X>; ++i)
-            unpack<X>(reinterpret_cast<const uint4 *>(slot)[lane * (N2 / kPairs<X>) + i], v + i * kPairs<X>);
-    } else {
-        const X *t = reinterpret_cast<const X *>(slot + ((uintptr_t)(row + c0) & 15)) + lane;
+        for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int k = 0; k < N2; ++k) {
+            for (int i = 0; i < R; ++i)
+                unpack<X>(reinterpret_cast<const uint4 *>(slot)[(j * 32 + lane) * R + i], v + j * N2 + i * kPairs<X>);
+    } else {
+        const X *t = reinterpret_cast<const X *>(slot + shift) + lane;
+#pragma unroll
+        for (int k = 0; k < NV * N2; ++k) {
             const int c = c0 + lane + 64 * k;
             v[k] = pair(c < H ? to_f(t[64 * k]) : 0.0f, c + 32 < H ? to_f(t[64 * k + 32]) : 0.0f);
         }
@@ -279,17 +283,21 @@ __device__ __forceinline__ void read_slot(const char *slot, const X *row, int c0
 }
 
 // the lane's sums into its columns of a row
-template <typename T, typename X, bool VEC>
+template <typename T, typename X, int NV, bool VEC>
 __device__ __forceinline__ void put_row(X *__restrict__ row, int c0, int lane, int H, const uint64_t *v) {
     constexpr int N2 = kPairs<T>;
-    if constexpr (VEC) {             // one or two vectors
-        const int c = c0 + lane * 2 * N2;
-        if (c >= H) return;
+    if constexpr (VEC) {
 #pragma unroll
-        for (int i = 0; i < N2 / kPairs<X>; ++i) reinterpret_cast<uint4 *>(row + c)[i] = pack<X>(v + i * kPairs<X>);
+        for (int j = 0; j < NV; ++j) {
+            const int c = c0 + (j * 32 + lane) * 2 * N2;
+            if (c < H)
+#pragma unroll
+                for (int i = 0; i < N2 / kPairs<X>; ++i)
+                    reinterpret_cast<uint4 *>(row + c)[i] = pack<X>(v + j * N2 + i * kPairs<X>);
+        }
     } else {
 #pragma unroll
-        for (int k = 0; k < N2; ++k) {
+        for (int k = 0; k < NV * N2; ++k) {
             const float2 h = halves(v[k]);
             const int c = c0 + lane + 64 * k;
             if (c < H) row[c] = from_f<X>(h.x);
@@ -305,14 +313,16 @@ __device__ __forceinline__ void put_row(X *__restrict__ row, int c0, int lane, i
 // it was needed, its latency once a token took two thirds of the time).  Of a row
 // that is not aligned the 16-byte vectors around the slab are fetched: each holds
 // a value of the row, so it lies in the tensor's memory.
-constexpr int kAhead = 16;
+template <int NV> constexpr int kAhead = NV == 1 ? 16 : 8;
+template <typename T, typename G, int NV, bool VEC>
+constexpr int kSlot = 512 * NV * (int)(sizeof(G) / sizeof(T)) + (VEC ? 0 : 16);
 
-template <typename T, typename G, bool VEC>
+template <typename T, typename G, int NV, bool VEC>
 __global__ void __launch_bounds__(256)
 embed_sum_kernel(const T *__restrict__ dy, const uint2 *__restrict__ sorted, uint32_t tokens, uint32_t V, int H,
                  float scale, int add, G *__restrict__ grad, float *__restrict__ part) {
-    constexpr int N = kLaneN<T>, N2 = N / 2, kSlot = 32 * N * (int)sizeof(G) + (VEC ? 0 : 16);
-    extern __shared__ uint4 dyn[];   // [8 warps][kAhead][kSlot bytes]
+    constexpr int N = kLaneN<T> * NV, N2 = N / 2, D = kAhead<NV>, S = kSlot<T, G, NV, VEC>;
+    extern __shared__ uint4 dyn[];   // [8 warps][D][S bytes]
     wait_for_previous();
     let_next_start();
     const int slabs = (H + 32 * N - 1) / (32 * N);
@@ -334,62 +344,70 @@ embed_sum_kernel(const T *__restrict__ dy, const uint2 *__restrict__ sorted, uin
     const uint32_t from = __ballot_sync(0xffffffffu, k_l == first && first == before);
     const uint32_t on = __ballot_sync(0xffffffffu, live == n && k_l == after);
     const uint32_t whole = last & ~from & ~on, with = add ? whole : 0;    // rows to write; gradient rows to read first
-    char *ring = reinterpret_cast<char *>(dyn) + (threadIdx.x >> 5) * (kAhead * kSlot);
-    const uint32_t at = (uint32_t)__cvta_generic_to_shared(ring);
-    auto copy_row = [&](int slot, const char *row, int bytes) {
-        const int shift = VEC ? 0 : (int)((uintptr_t)row & 15);
-        for (int i = lane * 16; i < bytes + shift; i += 512)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + slot * kSlot + i), "l"(row - shift + i)
-                         : "memory");
-    };
+    char *ring = reinterpret_cast<char *>(dyn) + (threadIdx.x >> 5) * (D * S);
+    const uint32_t at = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
     const int width = min(32 * N, H - c0);
+    const char *dy0 = reinterpret_cast<const char *>(dy + c0), *grad0 = reinterpret_cast<const char *>(grad + c0);
+    // bytes that a row begins behind a 16-byte boundary (32 bits hold what matters)
+    auto shift_of = [&](const char *base, uint32_t row, int size) {
+        return VEC ? 0 : (int)(((uint32_t)(uintptr_t)base + row * (uint32_t)H * (uint32_t)size) & 15);
+    };
+    auto copy_row = [&](int slot, const char *base, uint32_t row, int size, int most) {
+        const int shift = shift_of(base, row, size), bytes = width * size + shift;
+        const char *src = base + (int64_t)row * H * size - shift + lane * 16;
+#pragma unroll
+        for (int i = 0; i <= most; ++i)
+            if (lane * 16 + 512 * i < bytes && (i < most || !VEC))
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + slot * S + 512 * i), "l"(src + 512 * i)
+                             : "memory");
+    };
     int f_row = 0, f_slot = 0;       // next to fetch: the row of position f_row, or the gradient row behind it
     bool f_grad = false;
     auto fetch = [&] {
-        const uint32_t p = __shfl_sync(0xffffffffu, p_l, f_row & 31), k = __shfl_sync(0xffffffffu, k_l, f_row & 31);
         if (f_row < live) {
-            if (f_grad) copy_row(f_slot, reinterpret_cast<const char *>(grad + (int64_t)k * H + c0), width * (int)sizeof(G));
-            else copy_row(f_slot, reinterpret_cast<const char *>(dy + (int64_t)p * H + c0), width * (int)sizeof(T));
+            const uint32_t r = __shfl_sync(0xffffffffu, f_grad ? k_l : p_l, f_row);
+            if (f_grad) copy_row(f_slot, grad0, r, sizeof(G), NV * (int)(sizeof(G) / sizeof(T)));
+            else copy_row(f_slot, dy0, r, sizeof(T), NV);
             f_grad = !f_grad && (with >> f_row & 1);
             f_row += !f_grad;
-            f_slot = f_slot == kAhead - 1 ? 0 : f_slot + 1;
+            f_slot = (f_slot + 1) % D;
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     int slot = 0;
     // the next slot is there, and every lane has read the one that is filled now
     auto next = [&] {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 2) : "memory");
+        asm volatile("cp.async.wait_group %0;" ::"n"(D - 2) : "memory");
         __syncwarp();
         fetch();
-        const char *s = ring + slot * kSlot;
-        slot = slot == kAhead - 1 ? 0 : slot + 1;
+        const char *s = ring + slot * S;
+        slot = (slot + 1) % D;
         return s;
     };
-    for (int i = 0; i < kAhead - 1; ++i) fetch();
+    for (int i = 0; i < D - 1; ++i) fetch();
     uint64_t acc[N2], v[N2];
 #pragma unroll
     for (int k = 0; k < N2; ++k) acc[k] = 0;
     for (int i = 0; i < live; ++i) {
-        const uint32_t p = __shfl_sync(0xffffffffu, p_l, i), token = __shfl_sync(0xffffffffu, k_l, i);
-        read_slot<T, T, VEC>(next(), dy + (int64_t)p * H, c0, lane, H, v);
+        const int shift = VEC ? 0 : shift_of(dy0, __shfl_sync(0xffffffffu, p_l, i), sizeof(T));
+        read_slot<T, T, NV, VEC>(next(), shift, c0, lane, H, v);
 #pragma unroll
         for (int k = 0; k < N2; ++k) acc[k] = add2(acc[k], v[k]);
         if (last >> i & 1) {
             if (whole >> i & 1) {
-                G *row = grad + (int64_t)token * H;
+                const uint32_t token = __shfl_sync(0xffffffffu, k_l, i);
                 const uint64_t by = pair(scale, scale);
                 if (add) {
-                    read_slot<T, G, VEC>(next(), row, c0, lane, H, v);
+                    read_slot<T, G, NV, VEC>(next(), shift_of(grad0, token, sizeof(G)), c0, lane, H, v);
 #pragma unroll
                     for (int k = 0; k < N2; ++k) acc[k] = fma2(acc[k], by, v[k]);
                 } else {
 #pragma unroll
                     for (int k = 0; k < N2; ++k) acc[k] = mul2(acc[k], by);
                 }
-                put_row<T, G, VEC>(row, c0, lane, H, acc);
+                put_row<T, G, NV, VEC>(grad + (int64_t)token * H, c0, lane, H, acc);
             } else {                 // slot 0: begun before this chunk, 1: begins in it
-                put_row<T, float, VEC>(part + (chunk * 2 + (from >> i & 1 ? 0 : 1)) * H, c0, lane, H, acc);
+                put_row<T, float, NV, VEC>(part + (chunk * 2 + (from >> i & 1 ? 0 : 1)) * H, c0, lane, H, acc);
             }
 #pragma unroll
             for (int k = 0; k < N2; ++k) acc[k] = 0;
@@ -487,6 +505,21 @@ static int64_t embed_ws_bytes(int64_t tokens, int H) {
     return 2 * up256(tokens * 8) + (chunks > 1 ? chunks * 2 * H * 4 : 0);
 }
 
+template <typename T, typename G, int NV, bool VEC>
+static int sum_launch(const EmbedBwd &a, const uint2 *sorted, int64_t chunks, float *part, cudaStream_t st) {
+    constexpr int smem = 8 * kAhead<NV> * kSlot<T, G, NV, VEC>, slab = 32 * NV * kLaneN<T>;
+    auto kernel = embed_sum_kernel<T, G, NV, VEC>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return USAF_ECUDA;
+    }
+    const unsigned grid = cdiv(chunks * ((a.H + slab - 1) / slab), 8);
+    return launch_early(kernel, dim3(grid), 256, smem, st, (const T *)a.dy, sorted, (uint32_t)a.tokens, (uint32_t)a.V, a.H,
+                        a.scale, a.add, (G *)a.grad, part)
+               ? USAF_OK
+               : USAF_ECUDA;
+}
+
 template <typename T, typename G> static int embed_bwd(const EmbedBwd &a, cudaStream_t st) {
     SortArgs s;
     s.ids = a.ids;
@@ -518,19 +551,16 @@ template <typename T, typename G> static int embed_bwd(const EmbedBwd &a, cudaSt
     if (a.tokens == 0) return USAF_OK;
     const uint2 *sorted = s.pairs[(s.passes - 1) & 1];
     const int64_t chunks = (a.tokens + kChunk - 1) / kChunk;
-    const int slabs = (a.H + 32 * kLaneN<T> - 1) / (32 * kLaneN<T>);
-    const unsigned grid = cdiv(chunks * slabs, 8);
-    // 16-byte vectors of dy's rows, of the gradient's and of the partial sums
     const bool vec = ((uintptr_t)a.dy | (uintptr_t)a.grad | (uintptr_t)a.ws) % 16 == 0 && (int64_t)a.H * sizeof(T) % 16 == 0;
-    auto sum = vec ? embed_sum_kernel<T, G, true> : embed_sum_kernel<T, G, false>;
-    const int ring = 8 * kAhead * (32 * kLaneN<T> * (int)sizeof(G) + (vec ? 0 : 16));
-    if (cudaFuncSetAttribute(sum, cudaFuncAttributeMaxDynamicSharedMemorySize, ring) != cudaSuccess) {
-        (void)cudaGetLastError();
-        return USAF_ECUDA;
-    }
-    if (!launch_early(sum, dim3(grid), 256, ring, st, (const T *)a.dy, sorted, (uint32_t)a.tokens, (uint32_t)a.V, a.H,
-                      a.scale, a.add, (G *)a.grad, part))
-        return USAF_ECUDA;
+    // Two vectors a lane halve what a row costs beside its bytes (16384 rows of 1001
+    // fp32 values added to a gradient: 28 us against 37); one where that would leave an
+    // SM fewer than 16 warps to have rows on their way (8192 rows of 2048 bf16: the
+    // pass 123 us against 129)
+    const int wide = 64 * kLaneN<T>;
+    const bool two = a.H > wide / 2 && chunks * ((a.H + wide - 1) / wide) >= 148 * 16;
+    auto sum = two ? (vec ? sum_launch<T, G, 2, true> : sum_launch<T, G, 2, false>)
+                   : (vec ? sum_launch<T, G, 1, true> : sum_launch<T, G, 1, false>);
+    if (const int rc = sum(a, sorted, chunks, part, st)) return rc;
     if (chunks > 1) {
         const dim3 jgrid(cdiv(chunks - 1, 8), cdiv(a.H, 128));
         if (!launch_early(embed_join_kernel<G>, jgrid, 256, 0, st, sorted, (uint32_t)a.tokens, (uint32_t)a.V, a.H, a.scale,

@@ -97,22 +97,34 @@ def embedding_backward(dout: torch.Tensor, ids: torch.Tensor, num_embeddings: in
 
 class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, ids, table, scale, padding_idx, err):
+    def forward(ctx, ids, table, scale, padding_idx, err, into_grad):
         ctx.save_for_backward(ids)
         ctx.args = (table.shape[0], scale, padding_idx)
+        ctx.into = table if into_grad else None
         return embedding_forward(ids, table, scale, err)
 
     @staticmethod
     def backward(ctx, dout):
         (ids,) = ctx.saved_tensors
-        return None, embedding_backward(dout, ids, *ctx.args), None, None, None
+        held = ctx.into.grad if ctx.into is not None else None
+        if held is not None and held.is_contiguous() and held.dtype in (dout.dtype, torch.float32):
+            embedding_backward(dout, ids, *ctx.args, grad=held)
+            return None, None, None, None, None, None
+        return None, embedding_backward(dout, ids, *ctx.args), None, None, None, None
 
 
 def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, padding_idx: Optional[int] = None,
-              err: Optional[torch.Tensor] = None) -> torch.Tensor:
+              err: Optional[torch.Tensor] = None, into_grad: bool = False) -> torch.Tensor:
     """``scale * table[ids]`` (any shape of ``ids``), differentiable in the
-    table; ``padding_idx``'s row gets no gradient."""
+    table; ``padding_idx``'s row gets no gradient.
+
+    ``into_grad``: the backward pass adds to ``table.grad``, where the table
+    (a leaf) has one, and gives autograd nothing: for loops that accumulate
+    micro-batches with ``backward()``.  Not for ``torch.autograd.grad``, which
+    would find no gradient."""
     _padding(padding_idx, table.shape[0])
     if torch.is_grad_enabled() and table.requires_grad:
-        return _EmbeddingFn.apply(ids, table, scale, padding_idx, err)
+        if into_grad and not table.is_leaf:
+            raise ValueError("into_grad: the table must be a leaf")
+        return _EmbeddingFn.apply(ids, table, scale, padding_idx, err, into_grad)
     return embedding_forward(ids, table, scale, err)

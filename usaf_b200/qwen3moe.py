@@ -30,10 +30,13 @@ The router weight receives its gradient through autograd.
 from __future__ import annotations
 
 import contextlib
+import types
 from typing import Dict, List, Optional, Tuple
 
 import torch
 
+from . import embedding as _embedding
+from . import norms
 from .engine import BackwardScratch, BlockDims, MoEBlock, Projection, pair_capacity
 from .moe_loader import DenseAbsGradStore, SparseGradStore, TopKImportanceStore
 
@@ -319,6 +322,65 @@ def patch_qwen3moe_for_b200():
     modeling_qwen3_moe.Qwen3MoeExperts.forward = b200_qwen3_experts_forward
     modeling_qwen3_moe.Qwen3MoeSparseMoeBlock.forward = b200_qwen3_moe_block_forward
     return modeling_qwen3_moe
+
+
+# ------------------------------------------------- around the experts ---
+def b200_rms_norm_forward(self, hidden_states: torch.Tensor) -> torch.Tensor:
+    """A norm module of the model (weight, variance_epsilon)."""
+    return norms.rms_norm(hidden_states, self.weight, self.variance_epsilon)
+
+
+def b200_decoder_layer_forward(self, hidden_states: torch.Tensor, **kwargs) -> torch.Tensor:
+    """A pre-norm decoder layer; the residual addition behind the attention is
+    part of the norm in front of the MoE block."""
+    attn = self.self_attn(hidden_states=self.input_layernorm(hidden_states), **kwargs)[0]
+    post = self.post_attention_layernorm
+    normed, total = norms.rms_norm(attn, post.weight, post.variance_epsilon, residual=hidden_states)
+    return total + self.mlp(normed)
+
+
+def b200_embedding_forward(self, input: torch.Tensor) -> torch.Tensor:
+    """The token embedding; tokens outside the table set the module's error
+    word (:func:`error_words`) and read as zeros."""
+    if self._usaf_err is None or self._usaf_err.device != self.weight.device:
+        self._usaf_err = torch.zeros(1, dtype=torch.int32, device=self.weight.device)
+    return _embedding.embedding(input, self.weight, padding_idx=self.padding_idx, err=self._usaf_err,
+                                into_grad=self._usaf_into_grad)
+
+
+def use_dense_kernels(model: torch.nn.Module) -> torch.nn.Module:
+    """Run the norms, the residual additions between attention and MoE block and
+    the token embedding of this Qwen3-MoE model on the device kernels
+    (:mod:`usaf_b200.norms`, :mod:`usaf_b200.embedding`), forward and backward.
+
+    Unlike the patch of the MoE blocks this is per model, since the embedding
+    is torch's own class.  The norms round once where the modules' chains of
+    operations round the normed row before they multiply by the weight, so
+    16-bit activations differ by that rounding."""
+    from transformers.models.qwen3_moe import modeling_qwen3_moe as mq
+    for m in model.modules():
+        if isinstance(m, mq.Qwen3MoeRMSNorm):
+            m.forward = types.MethodType(b200_rms_norm_forward, m)
+        elif isinstance(m, mq.Qwen3MoeDecoderLayer):
+            m.forward = types.MethodType(b200_decoder_layer_forward, m)
+        elif isinstance(m, mq.Qwen3MoeModel):
+            e = m.embed_tokens
+            if e.max_norm is not None or e.scale_grad_by_freq or e.sparse:
+                raise ValueError("the token embedding's max_norm, scale_grad_by_freq and sparse are not handled")
+            e._usaf_err, e._usaf_into_grad = None, False
+            e.forward = types.MethodType(b200_embedding_forward, e)
+    return model
+
+
+def embeddings(model: torch.nn.Module) -> List[torch.nn.Module]:
+    """The token embeddings of ``model`` that run on the device kernels."""
+    return [m for m in model.modules() if "_usaf_into_grad" in m.__dict__]
+
+
+def error_words(model: torch.nn.Module) -> List[torch.Tensor]:
+    """The embeddings' device error words: nonzero after a token outside the
+    table (reading one waits for the device)."""
+    return [m._usaf_err for m in embeddings(model) if m._usaf_err is not None]
 
 
 @contextlib.contextmanager

@@ -32,6 +32,12 @@ weights from :func:`usaf_b200.qwen3moe.attach_int4_experts`):
   micro-batches each is one process accumulating ``accum * W`` micro-batches:
   the summed gradients are divided by ``loss_scale * accum * W``.
 
+* dense tensors around the experts (``dense_names``, no counterpart in train.py,
+  which trains experts and routers only): trained whole by AdamW
+  (:class:`usaf_b200.dense_optim.AdamW`), all in one launch a step, with the same
+  learning rate, loss scale and skips; a step is skipped too when one of their
+  gradients is not finite.
+
 Everything stays on the device; one host read per step carries the
 finiteness flag, the loss and the error words of the block workspaces (a
 batch whose routed pairs exceed a workspace raises ``UsafError`` there,
@@ -48,6 +54,7 @@ import torch.distributed as dist
 from . import checkpoint as ckpt
 from . import qwen3moe, rigl
 from ._lib import UsafError
+from .dense_optim import AdamW
 from .engine import Projection
 from .expert_parallel import global_select
 from .moe_loader import SparseGradStore, TopKImportanceStore
@@ -109,9 +116,14 @@ class SparseTrainer:
                  weight_decay: float = 0.005, accum: int = 1, frac: float = 0.005,
                  reselect_every: int = 50, loss_scale_init: float = LOSS_SCALE_INIT,
                  scale_up_every: int = SCALE_UP_EVERY, train_router: bool = True,
-                 expert_names: Optional[Iterable[str]] = None):
+                 expert_names: Optional[Iterable[str]] = None,
+                 dense_names: Optional[Iterable[str]] = None, dense_state_bits: int = 32):
         """``expert_names``: the ``*.mlp.experts`` modules to train (default:
-        every one with int4 weights attached); the others run frozen."""
+        every one with int4 weights attached); the others run frozen.
+        ``dense_names``: parameters of ``model`` (embedding, norms, gates) to
+        train whole by AdamW, states in ``dense_state_bits`` (32 or 8), weight
+        decay on those of two dimensions; a gate among them leaves the router
+        optimizer."""
         self.model = model
         self.steps, self.lr_peak, self.weight_decay = int(steps), float(lr_peak), float(weight_decay)
         self.accum, self.frac, self.reselect_every = int(accum), float(frac), int(reselect_every)
@@ -145,6 +157,9 @@ class SparseTrainer:
             for n in self.experts:
                 blk = model.get_submodule(n.rsplit(".", 1)[0])
                 self.router_params[f"{n.rsplit('.', 1)[0]}.gate.weight"] = blk.gate.weight
+        self.dense_params, self.dense_opt = self._dense(dense_names, dense_state_bits)
+        for n in self.dense_params:
+            self.router_params.pop(n, None)
         self.router_opt = (torch.optim.SGD(list(self.router_params.values()), lr=self.lr_peak,
                                            momentum=0.9, weight_decay=self.weight_decay)
                            if self.router_params else None)
@@ -155,6 +170,23 @@ class SparseTrainer:
         self.masters: Dict[str, torch.nn.Parameter] = {}
         self.store: Optional[SparseGradStore] = None
         self.opt: Optional[SparseAdam] = None
+
+    def _dense(self, names: Optional[Iterable[str]], state_bits: int):
+        named = dict(self.model.named_parameters())
+        names = list(names or ())
+        unknown = [n for n in names if n not in named]
+        if unknown:
+            raise ValueError(f"dense_names: the model has no parameter {unknown}")
+        if not names:
+            return {}, None
+        if self.expert_parallel:
+            raise NotImplementedError("dense tensors with experts sharded over ranks: their gradients are not "
+                                      "summed over the ranks")
+        params = {n: named[n] for n in names}
+        for p in params.values():
+            p.requires_grad_(True)
+        return params, AdamW(params, lr=self.lr_peak, weight_decay=self.weight_decay, state_bits=state_bits,
+                             no_decay=[n for n, p in params.items() if p.dim() < 2])
 
     # ---------------------------------------------------------------- capture
     def _set_capture(self, store) -> None:
@@ -177,7 +209,7 @@ class SparseTrainer:
             self._backward(loss_fn, batch)
         finally:
             self._set_capture(self.store) if self.store is not None else self._clear_capture()
-        for p in self.router_params.values():
+        for p in (*self.router_params.values(), *self.dense_params.values()):
             p.grad = None
         if not self.expert_parallel:
             return store.select(self.frac)
@@ -258,10 +290,20 @@ class SparseTrainer:
             for pg in self.router_opt.param_groups:
                 pg["lr"] = lr
             self.router_opt.zero_grad()
+        if self.dense_opt is not None:
+            self.dense_opt.lr = lr
+            self.dense_opt.zero_grad()
         self.store.zero_()
         loss_sum = torch.zeros((), dtype=torch.float32, device=next(iter(self.masters.values())).device)
-        for mb in micro_batches:
-            loss_sum += self._backward(loss_fn, mb)
+        tables = qwen3moe.embeddings(self.model) if self.dense_opt is not None else []
+        for e in tables:            # micro-batches behind the first add to the gradient's own rows
+            e._usaf_into_grad = True
+        try:
+            for mb in micro_batches:
+                loss_sum += self._backward(loss_fn, mb)
+        finally:
+            for e in tables:
+                e._usaf_into_grad = False
         scale = self.scaler.scale
         # train.py:661-662 divides the summed gradients by loss_scale * ACCUM.  Under
         # expert parallelism every shard's gradient (and the all-reduced router
@@ -269,19 +311,23 @@ class SparseTrainer:
         # own tokens: one step is one process accumulating accum * W micro-batches
         denom = scale * self.accum * (dist.get_world_size(self.ep_group) if self.expert_parallel else 1)
         # train.py:662-663: the step runs only if every expert gradient is finite
-        flags = torch.stack([torch.isfinite(g).all() for g in self.store.compact.values()])
+        flags = torch.stack([torch.isfinite(g).all() for g in self.store.compact.values()]
+                            + [torch.isfinite(p.grad).all() for p in self.dense_params.values()
+                               if p.grad is not None])
         blocks = qwen3moe.workspaces(self.model)
+        words = [b.err for b in blocks] + qwen3moe.error_words(self.model)
         nf = flags.numel()
-        dev_vals = torch.cat([flags.float(), loss_sum.reshape(1)] + [b.err.float() for b in blocks])
+        dev_vals = torch.cat([flags.float(), loss_sum.reshape(1)] + [w.float() for w in words])
         if self.expert_parallel:
             dev_vals = ranks_agree(dev_vals, nf, self.ep_group)
         host = dev_vals.cpu()
         if bool(host[nf + 1:].any()):
-            for b in blocks:
-                b.err.zero_()
+            for w in words:
+                w.zero_()
             self.step_num -= 1
             raise UsafError("a block workspace reported a device error in this step (routed "
-                            "pairs beyond its buffer, or a timed-out wait); no update applied")
+                            "pairs beyond its buffer, or a timed-out wait), or a token lay outside "
+                            "the embedding; no update applied")
         finite = bool(host[:nf].all())
         if finite:
             self.opt.step(compact_grads=self.store.compact, grad_div=denom)
@@ -291,8 +337,12 @@ class SparseTrainer:
                         p.grad.data.div_(denom)
                 self.router_opt.step()
                 self.router_opt.zero_grad()
+            if self.dense_opt is not None:
+                self.dense_opt.step(grad_div=denom)
         elif self.router_opt is not None:
             self.router_opt.zero_grad()
+        if self.dense_opt is not None:
+            self.dense_opt.zero_grad()
         self.scaler.update(finite)
         loss = float(host[nf]) / self.accum
         self.losses.append(loss)
@@ -307,12 +357,24 @@ class SparseTrainer:
                                for n in self.experts if ".layers." in n})
         config = {"lr_peak": self.lr_peak, "wd": self.weight_decay, "frac": self.frac,
                   "accum": self.accum, "steps": self.steps, **self.scaler.state_dict()}
+        opt_state = self.opt.state_dict()
+        if self.dense_opt is not None:      # beside SparseAdam's entries, which the reference reads by name
+            opt_state["dense"] = {"params": {n: p.detach() for n, p in self.dense_params.items()},
+                                  "adamw": self.dense_opt.state_dict()}
         return ckpt.save_sparse_checkpoint(path, {n: m.data for n, m in self.masters.items()},
-                                           self.active, self.opt.state_dict(), config,
+                                           self.active, opt_state, config,
                                            self.step_num, self.losses, train_layers, metric)
 
     def load_checkpoint(self, path: str) -> None:
         st = ckpt.load_sparse_checkpoint(path)
+        dense = st["optimizer"].get("dense")
+        held = dense["params"] if dense else {}
+        if {n: tuple(t.shape) for n, t in held.items()} != {n: tuple(p.shape) for n, p in self.dense_params.items()}:
+            raise ValueError(f"{path}: dense tensors {sorted(held)}, this trainer has {sorted(self.dense_params)}")
+        if dense:
+            self.dense_opt.load_state_dict(dense["adamw"])
+            for n, p in self.dense_params.items():
+                p.data.copy_(held[n])
         self.step_num = int(st["step"])
         self.losses = list(st.get("losses", []))
         cfg = st.get("config") or {}
