@@ -311,6 +311,10 @@ def test_refusals(dev):
         step([p], [g], m, v, step=0, lr=1e-3)
     with pytest.raises(ValueError, match="grad_div"):
         step([p], [g], m, v, grad_div=0.0, **kw)
+    with pytest.raises(ValueError, match="betas"):
+        step([p], [g], m, v, betas=(0.9, 1.0), **kw)
+    with pytest.raises(ValueError, match="16-byte"):
+        step([p[:256]], [g[:256]], torch.zeros(257, device=dev)[1:], v[:256], **kw)
     with pytest.raises(TypeError, match="both"):
         step([p], [g], m, q, **kw)
     with pytest.raises(TypeError, match="gradients"):

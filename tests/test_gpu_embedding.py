@@ -159,6 +159,10 @@ def test_empty(dev):
     assert embedding.embedding(ids, table).shape == (2, 0, 8)
     g = embedding.embedding_backward(torch.zeros(2, 0, 8, device=dev), ids, 5)
     assert g.shape == (5, 8) and not bool(g.any())
+    # the zeros come after what ran before, a short sum just launched among it
+    a = embedding.embedding_backward(torch.ones(1, 8, device=dev), ids.new_zeros(1), 5)
+    b = embedding.embedding_backward(torch.zeros(2, 0, 8, device=dev), ids, 5)
+    assert float(a.sum()) == 8.0 and not bool(b.any())
     start = torch.ones(5, 8, device=dev)
     assert torch.equal(embedding.embedding_backward(torch.zeros(2, 0, 8, device=dev), ids, 5, grad=start),
                        torch.ones(5, 8, device=dev))

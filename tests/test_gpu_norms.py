@@ -78,7 +78,7 @@ def check(total, w, y, rstd, eps, dy=None, dsum=None, dx=None, dw=None):
 
 TYPES = [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32),
          (torch.float16, torch.float16), (torch.float16, torch.float32)]
-SIZES = [(1, 1), (1, 2048), (3, 7), (5, 128), (1000, 128), (17, 771), (33, 1000), (300, 2048), (700, 520),
+SIZES = [(1, 1), (1, 2048), (3, 7), (700, 4), (513, 8), (300, 16), (77, 24), (9, 72), (5, 128), (1000, 128), (17, 771), (33, 1000), (300, 2048), (700, 520),
          (9, 6144), (65, 8192), (4, 9000), (3, 16384), (2, 32768), (2, 32767)]
 
 
@@ -208,11 +208,19 @@ def test_autograd_and_differences(dev):
     y2, t2 = norms.rms_norm(x2, w2, 1e-5, residual=res.detach())
     ((y2 * dy).sum() + (t2 * dsum).sum()).backward()
     assert torch.equal(x2.grad, x.grad) and w2.grad is None
-    # only the sum is used
+    # only the norm is used, or only the sum
+    x4 = x.detach().clone().requires_grad_(True)
+    w4 = w.detach().clone().requires_grad_(True)
+    y4, t4 = norms.rms_norm(x4, w4, 1e-5, residual=res.detach())
+    (y4 * dy).sum().backward()
+    check(t4.detach(), w4.detach(), y4.detach(), None, 1e-5, dy, None, x4.grad, w4.grad)
     x3 = x.detach().clone().requires_grad_(True)
     _, t3 = norms.rms_norm(x3, w2, 1e-5, residual=res.detach())
     (t3 * dsum).sum().backward()
     assert torch.equal(x3.grad, dsum)
+    with pytest.raises(RuntimeError):       # no second derivatives: refused, not wrong
+        g, = torch.autograd.grad((norms.rms_norm(x4, w4) * dy).sum(), x4, create_graph=True)
+        g.sum().backward()
 
 
 def test_other_stream_and_graph(dev):

@@ -541,14 +541,18 @@ template <typename T, typename G> static int embed_bwd(const EmbedBwd &a, cudaSt
         (void)cudaGetLastError();
         return USAF_ECUDA;
     }
-    if (a.tokens) {
-        embed_sort_kernel<<<kSortCtas, kSortThreads, smem, st>>>(s);
-        USAF_CHECK_LAUNCH();
-    }
     const int64_t zero = a.add ? 0 : a.V * (int64_t)a.H * (int64_t)sizeof(G);
+    if (a.tokens == 0) {             // nothing sorted: nothing that the zeros may start beside
+        if (zero && cudaMemsetAsync(a.grad, 0, (size_t)zero, st) != cudaSuccess) {
+            (void)cudaGetLastError();
+            return USAF_ECUDA;
+        }
+        return USAF_OK;
+    }
+    embed_sort_kernel<<<kSortCtas, kSortThreads, smem, st>>>(s);
+    USAF_CHECK_LAUNCH();
     if (zero && !launch_early(embed_zero_kernel, dim3(cdiv(zero + 1, kZeroTile)), kZeroThreads, 0, st, (char *)a.grad, zero))
         return USAF_ECUDA;
-    if (a.tokens == 0) return USAF_OK;
     const uint2 *sorted = s.pairs[(s.passes - 1) & 1];
     const int64_t chunks = (a.tokens + kChunk - 1) / kChunk;
     const bool vec = ((uintptr_t)a.dy | (uintptr_t)a.grad | (uintptr_t)a.ws) % 16 == 0 && (int64_t)a.H * sizeof(T) % 16 == 0;

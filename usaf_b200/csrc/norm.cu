@@ -325,7 +325,10 @@ __global__ void __launch_bounds__(kNormMaxBlock) norm_bwd_rows(const NormBwd a, 
         for (int i = 0; i < NV; ++i)
             if (ring.has >> i & 1)
 #pragma unroll
-                for (int k = 0; k < N2; ++k) reinterpret_cast<float2 *>(to + i * tpr * 2 * N2)[k] = halves(acc[i][k]);
+                for (int k = 0; k < N2; k += 2) {
+                    const float2 x = halves(acc[i][k]), y = halves(acc[i][k + 1]);
+                    reinterpret_cast<float4 *>(to + i * tpr * 2 * N2)[k / 2] = make_float4(x.x, x.y, y.x, y.y);
+                }
         if (groups > 1) {
             __syncthreads();
             for (int c = threadIdx.x; c < a.H; c += blockDim.x) {

@@ -15,6 +15,7 @@ rounded by itself in fp32, in a fixed order.
 from __future__ import annotations
 
 from array import array
+from itertools import accumulate
 from typing import Dict, Iterable, List, Optional, Sequence, Tuple, Union
 
 import torch
@@ -30,11 +31,8 @@ Packed = Tuple[torch.Tensor, torch.Tensor]
 def state_layout(numels: Iterable[int]) -> Tuple[List[int], int]:
     """Where the states of tensors of these sizes start, and the size of the
     flat buffers that hold them."""
-    starts, at = [], 0
-    for n in numels:
-        starts.append(at)
-        at += -(-int(n) // BLOCK) * BLOCK
-    return starts, at
+    places = list(accumulate([(int(n) + BLOCK - 1) // BLOCK * BLOCK for n in numels], initial=0))
+    return places[:-1], places[-1]
 
 
 def _check_flat(name: str, t: torch.Tensor, n: int, dtype: torch.dtype, device: torch.device) -> None:
@@ -67,6 +65,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m:
         raise ValueError(f"step: expected >= 1, got {step}")
     if grad_div == 0:
         raise ValueError("grad_div must not be 0")
+    if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1 and eps >= 0):
+        raise ValueError(f"betas {betas} outside [0, 1), or eps {eps} below 0")
     eight = not isinstance(m, torch.Tensor)
     if eight == isinstance(v, torch.Tensor):
         raise TypeError("m and v: both flat tensors, or both (values, scales) pairs")
@@ -77,16 +77,19 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m:
         raise TypeError(f"gradients: expected {dtype} or torch.float32, got {g_dtype}")
     ptr(params[0])      # on a CUDA device, and so are the others
     index = dev.index
-    for i, p in enumerate(params):
-        g = grads[i]
+    numels, at, grads_at = [], [], []
+    for p, g in zip(params, grads):
         if p.dtype is not dtype or g.dtype is not g_dtype:
-            raise TypeError(f"tensor {i}: {p.dtype} with a gradient of {g.dtype}, the first has {dtype} and {g_dtype}")
+            raise TypeError(f"tensor {len(at)}: {p.dtype} with a gradient of {g.dtype}, the first has {dtype} and "
+                            f"{g_dtype}")
         if p.get_device() != index or g.get_device() != index:
-            raise ValueError(f"tensor {i}: expected on {dev}")
-        if not (p.is_same_size(g) and p.is_contiguous() and g.is_contiguous()):
-            raise ValueError(f"tensor {i}: the parameter and a gradient of its shape must be contiguous")
-    numels = [p.numel() for p in params]
-    at = [p.data_ptr() for p in params]
+            raise ValueError(f"tensor {len(at)}: expected on {dev}")
+        k = p.numel()
+        if g.numel() != k or not p.is_contiguous() or not g.is_contiguous():
+            raise ValueError(f"tensor {len(at)}: the parameter and a gradient of its size must be contiguous")
+        numels.append(k)
+        at.append(p.data_ptr())
+        grads_at.append(g.data_ptr())
     size = params[0].element_size()
     end = 0
     for a, k in sorted(zip(at, numels)):
@@ -111,7 +114,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m:
     if len(decays) != n:
         raise ValueError(f"{len(decays)} weight decays for {n} parameters")
     # one host array of each, read before the call returns
-    tab = (array("Q", at), array("Q", [g.data_ptr() for g in grads]), array("q", numels), array("q", places),
+    tab = (array("Q", at), array("Q", grads_at), array("q", numels), array("q", places),
            array("d", decays))
     ms = vs = None
     if eight:

@@ -17,6 +17,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import call_on, ptr
@@ -104,6 +105,7 @@ class _EmbeddingFn(torch.autograd.Function):
         return embedding_forward(ids, table, scale, err)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         (ids,) = ctx.saved_tensors
         held = ctx.into.grad if ctx.into is not None else None

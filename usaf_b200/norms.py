@@ -17,6 +17,7 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import call_on, ptr
@@ -123,12 +124,18 @@ class _RmsNormFn(torch.autograd.Function):
         y, rstd, total = rms_norm_forward(x, weight, eps, residual)
         ctx.save_for_backward(total, weight, rstd)
         ctx.has_residual = residual is not None
+        ctx.set_materialize_grads(False)      # an unused output has no gradient to read
         return (y, total) if ctx.has_residual else y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy, dsum=None):
         total, weight, rstd = ctx.saved_tensors
-        dx, dw = rms_norm_backward(dy, total, weight, rstd, dsum, want_dw=ctx.needs_input_grad[1])
+        want_dw = ctx.needs_input_grad[1]
+        if dy is None:
+            dx, dw = dsum, (torch.zeros_like(weight) if want_dw else None)
+        else:
+            dx, dw = rms_norm_backward(dy, total, weight, rstd, dsum, want_dw=want_dw)
         return dx, dw, None, dx if ctx.has_residual else None
 
 

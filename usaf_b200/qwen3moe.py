@@ -342,7 +342,7 @@ def b200_decoder_layer_forward(self, hidden_states: torch.Tensor, **kwargs) -> t
 def b200_embedding_forward(self, input: torch.Tensor) -> torch.Tensor:
     """The token embedding; tokens outside the table set the module's error
     word (:func:`error_words`) and read as zeros."""
-    if self._usaf_err is None or self._usaf_err.device != self.weight.device:
+    if self._usaf_err.device != self.weight.device:
         self._usaf_err = torch.zeros(1, dtype=torch.int32, device=self.weight.device)
     return _embedding.embedding(input, self.weight, padding_idx=self.padding_idx, err=self._usaf_err,
                                 into_grad=self._usaf_into_grad)
@@ -367,7 +367,8 @@ def use_dense_kernels(model: torch.nn.Module) -> torch.nn.Module:
             e = m.embed_tokens
             if e.max_norm is not None or e.scale_grad_by_freq or e.sparse:
                 raise ValueError("the token embedding's max_norm, scale_grad_by_freq and sparse are not handled")
-            e._usaf_err, e._usaf_into_grad = None, False
+            e._usaf_err = torch.zeros(1, dtype=torch.int32, device=e.weight.device)
+            e._usaf_into_grad = False
             e.forward = types.MethodType(b200_embedding_forward, e)
     return model
 
@@ -380,7 +381,7 @@ def embeddings(model: torch.nn.Module) -> List[torch.nn.Module]:
 def error_words(model: torch.nn.Module) -> List[torch.Tensor]:
     """The embeddings' device error words: nonzero after a token outside the
     table (reading one waits for the device)."""
-    return [m._usaf_err for m in embeddings(model) if m._usaf_err is not None]
+    return [m._usaf_err for m in embeddings(model)]
 
 
 @contextlib.contextmanager
