@@ -170,6 +170,7 @@ __global__ void __launch_bounds__(kNormMaxBlock) norm_fwd_rows(const NormFwd a, 
     const int group = threadIdx.x / tpr, t = threadIdx.x - group * tpr, groups = blockDim.x / tpr;
     for (int i = threadIdx.x; i < 256; i += blockDim.x) (&red[0][0][0])[i] = 0.0f;
     __syncthreads();
+    wait_for_previous();
     const int64_t step = (int64_t)gridDim.x * groups;
     int64_t row = (int64_t)blockIdx.x * groups + group;
     RowRing<T, NV, RES ? 2 : 1, kFwdSlots> ring;
@@ -245,6 +246,7 @@ __global__ void __launch_bounds__(kNormMaxBlock) norm_bwd_rows(const NormBwd a, 
     const int group = threadIdx.x / tpr, t = threadIdx.x - group * tpr, groups = blockDim.x / tpr;
     for (int i = threadIdx.x; i < 256; i += blockDim.x) (&red[0][0][0])[i] = 0.0f;
     __syncthreads();
+    wait_for_previous();
     if constexpr (DW) let_next_start();
     const int64_t step = (int64_t)gridDim.x * groups;
     int64_t row = (int64_t)blockIdx.x * groups + group;
@@ -458,9 +460,7 @@ static int fwd_launch(const NormFwd &a, const RowPlan &p, cudaStream_t st) {
     const int smem = ring_slots(NV, RES ? 2 : 1, kFwdSlots) * 16 * p.block;
     if (!allow_smem(norm_fwd_rows<T, W, NV, RES>, smem)) return USAF_ECUDA;
     const int grid = row_grid(p, smem, NV == 4 ? 128 : 64, a.rows, 1 << 30);
-    norm_fwd_rows<T, W, NV, RES><<<grid, p.block, smem, st>>>(a, p.tpr);
-    USAF_CHECK_LAUNCH();
-    return USAF_OK;
+    return launch_early(norm_fwd_rows<T, W, NV, RES>, dim3(grid), p.block, smem, st, a, p.tpr) ? USAF_OK : USAF_ECUDA;
 }
 
 template <typename T, typename W, int NV> static int fwd_launch(const NormFwd &a, const RowPlan &p, cudaStream_t st) {
@@ -490,8 +490,7 @@ static int bwd_launch(const NormBwd &a, const RowPlan &p, int *P, cudaStream_t s
     const int smem = std::max(ring_slots(NV, DSUM ? 3 : 2, kBwdSlots) * 16 * p.block, fold);
     if (!allow_smem(norm_bwd_rows<T, W, NV, DSUM, DW>, smem)) return USAF_ECUDA;
     const int grid = row_grid(p, smem, NV == 4 ? 128 : 80, a.rows, DW ? kNormMaxPartials : 1 << 30);
-    norm_bwd_rows<T, W, NV, DSUM, DW><<<grid, p.block, smem, st>>>(a, p.tpr);
-    USAF_CHECK_LAUNCH();
+    if (!launch_early(norm_bwd_rows<T, W, NV, DSUM, DW>, dim3(grid), p.block, smem, st, a, p.tpr)) return USAF_ECUDA;
     *P = grid;
     return USAF_OK;
 }
