@@ -262,6 +262,7 @@ template <int N, typename P, typename G, bool EIGHT, bool MASTER>
 __global__ void __launch_bounds__(256, 3)
 adamw_kernel(const __grid_constant__ AdamwTable<N> tab, const AdamwState s, const AdamwConsts c, const int run) {
     extern __shared__ uint4 dyn[];
+    wait_for_previous();
     const int u = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (u >= tab.first[tab.n]) return;
     int lo = 0, hi = tab.n;          // the last tensor that starts at or before this run
@@ -371,9 +372,7 @@ static int adamw_start(const AdamwTable<N> &tab, const AdamwState &s, const Adam
         (void)cudaGetLastError();
         return USAF_ECUDA;
     }
-    kernel<<<cdiv(tab.first[tab.n], 8), 256, smem, st>>>(tab, s, c, run);
-    USAF_CHECK_LAUNCH();
-    return USAF_OK;
+    return launch_early(kernel, dim3(cdiv(tab.first[tab.n], 8)), 256, smem, st, tab, s, c, run) ? USAF_OK : USAF_ECUDA;
 }
 
 template <int N, typename P, typename G, bool EIGHT>

@@ -84,7 +84,7 @@ __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontr
 
 template <typename... Args, typename... Given>
 static inline bool launch_early(void (*kernel)(Args...), dim3 grid, int block, int smem, cudaStream_t st,
-                                Given... given) {
+                                const Given &...given) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(block);

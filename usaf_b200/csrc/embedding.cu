@@ -41,6 +41,7 @@ __global__ void __launch_bounds__(256)
 embed_fwd_kernel(const void *__restrict__ ids, int ids64, int64_t tokens, const T *__restrict__ table, int64_t V,
                  int H, float scale, T *__restrict__ out, int32_t *__restrict__ err) {
     constexpr int N = kLaneN<T>, S = kFwdSlabs;
+    wait_for_previous();
     const int groups = (H + 32 * N * S - 1) / (32 * N * S);
     const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5;
     const int lane = threadIdx.x & 31;
@@ -145,6 +146,7 @@ __device__ __forceinline__ uint32_t same_digit(uint32_t d, int bits) {
 __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads)
 embed_sort_kernel(const SortArgs a) {
     extern __shared__ uint32_t hist[];                 // [32 warps][bins]; total, base [bins]; sums [4][bins]
+    wait_for_previous();             // before the zeros may start: all that was enqueued before has ended
     let_next_start();
     cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -549,8 +551,7 @@ template <typename T, typename G> static int embed_bwd(const EmbedBwd &a, cudaSt
         }
         return USAF_OK;
     }
-    embed_sort_kernel<<<kSortCtas, kSortThreads, smem, st>>>(s);
-    USAF_CHECK_LAUNCH();
+    if (!launch_early(embed_sort_kernel, dim3(kSortCtas), kSortThreads, smem, st, s)) return USAF_ECUDA;
     if (zero && !launch_early(embed_zero_kernel, dim3(cdiv(zero + 1, kZeroTile)), kZeroThreads, 0, st, (char *)a.grad, zero))
         return USAF_ECUDA;
     const uint2 *sorted = s.pairs[(s.passes - 1) & 1];
@@ -575,15 +576,15 @@ template <typename T, typename G> static int embed_bwd(const EmbedBwd &a, cudaSt
 }
 
 template <typename T>
-static void embed_fwd(const void *ids, int ids64, int64_t tokens, const void *table, int64_t V, int H, float scale,
+static int embed_fwd(const void *ids, int ids64, int64_t tokens, const void *table, int64_t V, int H, float scale,
                       void *out, int32_t *err, cudaStream_t st) {
     const int group = 32 * kLaneN<T> * kFwdSlabs;
     const unsigned grid = cdiv(tokens * ((H + group - 1) / group), 8);
     const bool vec = ((uintptr_t)table | (uintptr_t)out) % 16 == 0 && (int64_t)H * sizeof(T) % 16 == 0;
-    if (vec)
-        embed_fwd_kernel<T, true><<<grid, 256, 0, st>>>(ids, ids64, tokens, (const T *)table, V, H, scale, (T *)out, err);
-    else
-        embed_fwd_kernel<T, false><<<grid, 256, 0, st>>>(ids, ids64, tokens, (const T *)table, V, H, scale, (T *)out, err);
+    return launch_early(vec ? embed_fwd_kernel<T, true> : embed_fwd_kernel<T, false>, dim3(grid), 256, 0, st, ids, ids64,
+                        tokens, (const T *)table, V, H, scale, (T *)out, err)
+               ? USAF_OK
+               : USAF_ECUDA;
 }
 
 }  // namespace usaf
@@ -602,13 +603,11 @@ extern "C" int usaf_embedding_fwd(const void *ids, int32_t ids_bits, int64_t tok
     cudaStream_t st = as_stream(stream);
     const int wide = ids_bits == 64;
     switch (dtype) {
-        case USAF_F32: embed_fwd<float>(ids, wide, tokens, table, V, H, (float)scale, out, err, st); break;
-        case USAF_BF16: embed_fwd<__nv_bfloat16>(ids, wide, tokens, table, V, H, (float)scale, out, err, st); break;
-        case USAF_F16: embed_fwd<__half>(ids, wide, tokens, table, V, H, (float)scale, out, err, st); break;
+        case USAF_F32: return embed_fwd<float>(ids, wide, tokens, table, V, H, (float)scale, out, err, st);
+        case USAF_BF16: return embed_fwd<__nv_bfloat16>(ids, wide, tokens, table, V, H, (float)scale, out, err, st);
+        case USAF_F16: return embed_fwd<__half>(ids, wide, tokens, table, V, H, (float)scale, out, err, st);
         default: return USAF_EINVAL;
     }
-    USAF_CHECK_LAUNCH();
-    return USAF_OK;
 }
 
 extern "C" int64_t usaf_embedding_workspace_bytes(int64_t tokens, int64_t V, int32_t H) {
