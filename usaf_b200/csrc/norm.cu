@@ -420,14 +420,22 @@ __global__ void __launch_bounds__(1024) norm_dw_kernel(const float *__restrict__
 }
 
 // How rows of n 16-byte vectors are cut: vectors a thread, threads a row, threads
-// a CTA.  Two vectors a thread let the work of a turn (addresses, the sum over
-// the threads) serve 32 bytes; four only where two would take more than a CTA.
+// a CTA.  More vectors a thread let the work of a turn (addresses, the sum over
+// the threads) serve more bytes and leave fewer warps to wait for one another;
+// the backward pass's dw sums cost 8 registers each.  Measured (us, forward /
+// backward with dw, bf16): n = 256 (8192 rows, residual) two vectors 24.1 / 26.3,
+// three 23.5 / 33.9; n = 512 (4000 rows) two 15.1 / 24.3, four 13.5 / 23.1; n = 640
+// (5000 rows) three 20.9 / 33.0, four 19.0 / 29.9; n = 768 (4096 rows) two 20.5 / 34.4,
+// three 18.8 / 31.1, four 20.3 / 31.9; n = 1024 (3000 rows) two 20.2 / 35.8, four
+// 17.9 / 29.7.  So two up to 256, then three or four, whichever leaves fewer idle
+// lanes, four above 768.
 struct RowPlan {
     int nv, tpr, block;
 };
 
 static RowPlan plan_rows(int n) {
-    RowPlan p{n <= 4 ? 1 : n <= 2 * kNormMaxBlock ? 2 : 4, 1, 0};
+    const auto idle = [n](int nv) { return (n + 32 * nv - 1) / (32 * nv) * 32 * nv - n; };
+    RowPlan p{n <= 4 ? 1 : n <= 256 ? 2 : n <= 768 && idle(3) <= idle(4) ? 3 : 4, 1, 0};
     const int t = (n + p.nv - 1) / p.nv;
     if (t > 32) p.tpr = (t + 31) / 32 * 32;
     else
@@ -459,7 +467,7 @@ template <typename T, typename W, int NV, bool RES>
 static int fwd_launch(const NormFwd &a, const RowPlan &p, cudaStream_t st) {
     const int smem = ring_slots(NV, RES ? 2 : 1, kFwdSlots) * 16 * p.block;
     if (!allow_smem(norm_fwd_rows<T, W, NV, RES>, smem)) return USAF_ECUDA;
-    const int grid = row_grid(p, smem, NV == 4 ? 128 : 64, a.rows, 1 << 30);
+    const int grid = row_grid(p, smem, NV == 4 ? 128 : NV == 3 ? 80 : 64, a.rows, 1 << 30);
     return launch_early(norm_fwd_rows<T, W, NV, RES>, dim3(grid), p.block, smem, st, a, p.tpr) ? USAF_OK : USAF_ECUDA;
 }
 
@@ -474,6 +482,7 @@ template <typename T, typename W> static int norm_fwd(const NormFwd &a, cudaStre
         const RowPlan p = plan_rows((int)(bytes / 16));
         if (p.nv == 1) return fwd_launch<T, W, 1>(a, p, st);
         if (p.nv == 2) return fwd_launch<T, W, 2>(a, p, st);
+        if (p.nv == 3) return fwd_launch<T, W, 3>(a, p, st);
         if (p.nv == 4) return fwd_launch<T, W, 4>(a, p, st);
     }
     const unsigned grid = (unsigned)std::min<int64_t>(a.rows, 148 * 8);
@@ -489,7 +498,7 @@ static int bwd_launch(const NormBwd &a, const RowPlan &p, int *P, cudaStream_t s
     const int groups = p.block / p.tpr, fold = DW && groups > 1 ? groups * a.H * 4 : 0;
     const int smem = std::max(ring_slots(NV, DSUM ? 3 : 2, kBwdSlots) * 16 * p.block, fold);
     if (!allow_smem(norm_bwd_rows<T, W, NV, DSUM, DW>, smem)) return USAF_ECUDA;
-    const int grid = row_grid(p, smem, NV == 4 ? 128 : 80, a.rows, DW ? kNormMaxPartials : 1 << 30);
+    const int grid = row_grid(p, smem, NV == 4 ? 128 : NV == 3 ? 104 : 80, a.rows, DW ? kNormMaxPartials : 1 << 30);
     if (!launch_early(norm_bwd_rows<T, W, NV, DSUM, DW>, dim3(grid), p.block, smem, st, a, p.tpr)) return USAF_ECUDA;
     *P = grid;
     return USAF_OK;
@@ -508,6 +517,7 @@ template <typename T, typename W> static int bwd_rows(const NormBwd &a, int *P, 
         const RowPlan p = plan_rows((int)(bytes / 16));
         if (p.nv == 1) return bwd_launch<T, W, 1>(a, p, P, st);
         if (p.nv == 2) return bwd_launch<T, W, 2>(a, p, P, st);
+        if (p.nv == 3) return bwd_launch<T, W, 3>(a, p, P, st);
         if (p.nv == 4) return bwd_launch<T, W, 4>(a, p, P, st);
     }
     const int smem = a.dw ? a.H * 4 : 0;
