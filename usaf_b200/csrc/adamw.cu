@@ -10,6 +10,11 @@
 // as e4m3 values times one fp32 scale per 256 values (largest magnitude / 448):
 // sqrt(v) keeps the moment's range within e4m3's, and one above zero is never
 // stored as zero, so that the next step does not divide by eps alone.
+//
+// With 32-bit states HBM bounds the step: 312 M bf16 weights with masters take
+// 1.31 ms, 103 % of the measured copy rate.  With 8-bit states (10 bytes a value
+// instead of 28) it is the instructions, 41 a value at 70 % of the issue slots:
+// 0.58 ms, 84 % of that rate.
 #include <cuda_fp8.h>
 
 #include "common.cuh"

