@@ -78,7 +78,7 @@ def check(total, w, y, rstd, eps, dy=None, dsum=None, dx=None, dw=None):
 
 TYPES = [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32),
          (torch.float16, torch.float16), (torch.float16, torch.float32)]
-SIZES = [(1, 1), (1, 2048), (3, 7), (700, 4), (513, 8), (300, 16), (77, 24), (9, 72), (5, 128), (1000, 128), (17, 771), (33, 1000), (300, 2048), (700, 520),
+SIZES = [(1, 1), (1, 2048), (3, 7), (700, 4), (513, 8), (300, 16), (77, 24), (9, 72), (5, 128), (4099, 35), (777, 61), (515, 131), (130, 2050), (1, 35), (8, 771), (9, 771), (1000, 128), (17, 771), (33, 1000), (300, 2048), (700, 520),
          (9, 6144), (65, 8192), (4, 9000), (3, 16384), (2, 32768), (2, 32767)]
 
 
@@ -102,7 +102,7 @@ def test_against_64_bits(dev, rows, H, dt, wdt):
     assert none is None and torch.equal(dx2, dx)
 
 
-@pytest.mark.parametrize("rows,H", [(70000, 128), (20011, 96), (5000, 2048), (3001, 771), (1500, 6144)])
+@pytest.mark.parametrize("rows,H", [(70000, 128), (20011, 96), (5000, 2048), (3001, 771), (1500, 6144), (50001, 35), (9001, 131)])
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
 def test_many_rows_repeat_bit_for_bit(dev, rows, H, dt):
     from usaf_b200 import norms
