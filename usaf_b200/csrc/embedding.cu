@@ -263,6 +263,30 @@ embed_sort_kernel(const SortArgs a) {
     }
 }
 
+// Up to 512 pairs: one CTA counts for every pair those that come before it (a
+// smaller key, or the same one earlier), 4 keys a load: 2 to 3 us, where the
+// cluster's passes and barriers take 12 whatever they sort.
+constexpr int kFewTokens = 512;
+
+__global__ void __launch_bounds__(kFewTokens) embed_sort_few_kernel(const SortArgs a, uint2 *__restrict__ sorted) {
+    __shared__ alignas(16) uint32_t key[kFewTokens];
+    wait_for_previous();
+    let_next_start();
+    const uint32_t j = threadIdx.x, mine = j < a.tokens ? sort_key(a, j) : 0xffffffffu;
+    key[j] = mine;
+    __syncthreads();
+    if (j >= a.tokens) return;
+    uint32_t to = 0;
+    const uint32_t last = (a.tokens + 3) / 4;           // the keys behind the tokens are larger than any
+#pragma unroll 4
+    for (uint32_t i = 0; i < last; ++i) {
+        const uint4 k = reinterpret_cast<const uint4 *>(key)[i];
+        to += (k.x < mine || (k.x == mine && 4 * i < j)) + (k.y < mine || (k.y == mine && 4 * i + 1 < j)) +
+              (k.z < mine || (k.z == mine && 4 * i + 2 < j)) + (k.w < mine || (k.w == mine && 4 * i + 3 < j));
+    }
+    sorted[to] = make_uint2(mine, j);
+}
+
 // ---- backward: sums -----------------------------------------------------------
 // A slab is 32 lanes times NV vectors of 16 bytes of T; a lane's values are those
 // of vectors lane, 32 + lane, ... (VEC), else every 32nd column.  From a slot of the
@@ -554,10 +578,13 @@ template <typename T, typename G> static int embed_bwd(const EmbedBwd &a, cudaSt
         }
         return USAF_OK;
     }
-    if (!launch_early(embed_sort_kernel, dim3(kSortCtas), kSortThreads, smem, st, s)) return USAF_ECUDA;
+    const bool few = a.tokens <= kFewTokens;
+    if (!(few ? launch_early(embed_sort_few_kernel, dim3(1), kFewTokens, 0, st, s, s.pairs[0])
+              : launch_early(embed_sort_kernel, dim3(kSortCtas), kSortThreads, smem, st, s)))
+        return USAF_ECUDA;
     if (zero && !launch_early(embed_zero_kernel, dim3(cdiv(zero + 1, kZeroTile)), kZeroThreads, 0, st, (char *)a.grad, zero))
         return USAF_ECUDA;
-    const uint2 *sorted = s.pairs[(s.passes - 1) & 1];
+    const uint2 *sorted = s.pairs[few ? 0 : (s.passes - 1) & 1];
     const int64_t chunks = (a.tokens + kChunk - 1) / kChunk;
     const bool vec = ((uintptr_t)a.dy | (uintptr_t)a.grad | (uintptr_t)a.ws) % 16 == 0 && (int64_t)a.H * sizeof(T) % 16 == 0;
     // Two vectors a lane halve what a row costs beside its bytes (16384 rows of 1001

@@ -167,6 +167,12 @@ struct NormBwd {
     void *dx, *dw; float *part;
 };
 
+// a CTA's sum of column c: a partial one, or where it is the only CTA, dw itself
+template <typename W> __device__ __forceinline__ void put_dw(const NormBwd &a, int c, float v) {
+    if (gridDim.x == 1) static_cast<W *>(a.dw)[c] = from_f<W>(v);
+    else a.part[(int64_t)blockIdx.x * a.H + c] = v;
+}
+
 template <typename T, typename W, int NV, bool RES>
 __global__ void __launch_bounds__(kNormMaxBlock) norm_fwd_rows(const NormFwd a, int tpr) {
     __shared__ alignas(16) float red[2][8][16];
@@ -325,7 +331,8 @@ __global__ void __launch_bounds__(kNormMaxBlock) norm_bwd_rows(const NormBwd a, 
     }
     if constexpr (DW) {
         float *part = a.part + (int64_t)blockIdx.x * a.H, *fold = reinterpret_cast<float *>(dyn);
-        float *to = (groups > 1 ? fold + group * a.H : part) + t * 2 * N2;
+        const bool folds = groups > 1 || gridDim.x == 1;
+        float *to = (folds ? fold + group * a.H : part) + t * 2 * N2;
         asm volatile("cp.async.wait_all;" ::: "memory");
         __syncthreads();                     // the ring is read; its space takes the sums
 #pragma unroll
@@ -336,12 +343,12 @@ __global__ void __launch_bounds__(kNormMaxBlock) norm_bwd_rows(const NormBwd a, 
                     const float2 x = halves(acc[i][k]), y = halves(acc[i][k + 1]);
                     reinterpret_cast<float4 *>(to + i * tpr * 2 * N2)[k / 2] = make_float4(x.x, x.y, y.x, y.y);
                 }
-        if (groups > 1) {
+        if (folds) {
             __syncthreads();
             for (int c = threadIdx.x; c < a.H; c += blockDim.x) {
                 float v = 0.0f;
                 for (int g = 0; g < groups; ++g) v += fold[g * a.H + c];
-                part[c] = v;
+                put_dw<W>(a, c, v);
             }
         }
     }
@@ -485,7 +492,7 @@ __global__ void __launch_bounds__(256) norm_bwd_tile(const NormBwd a, int R, int
         for (int c = threadIdx.x; c < a.H; c += 256) {
             float v = 0.0f;
             for (int k = 0; k < parts; ++k) v += acc[k * a.H + c];
-            a.part[(int64_t)blockIdx.x * a.H + c] = v;
+            put_dw<W>(a, c, v);
         }
 }
 
@@ -522,7 +529,7 @@ template <typename T, typename W>
 __global__ void __launch_bounds__(256)
 norm_bwd_any(const T *__restrict__ dy, int64_t lddy, const T *__restrict__ x, int64_t ldx,
              const W *__restrict__ w, const float *__restrict__ rstd, const T *__restrict__ dsum,
-             int64_t ldds, int64_t rows, int H, T *__restrict__ dx, float *__restrict__ part) {
+             int64_t ldds, int64_t rows, int H, T *__restrict__ dx, float *__restrict__ part, W *__restrict__ dw) {
     extern __shared__ float acc[];      // [H] dw sums, a thread's own columns only
     __shared__ float red[8];
     if (part)
@@ -544,7 +551,10 @@ norm_bwd_any(const T *__restrict__ dy, int64_t lddy, const T *__restrict__ x, in
         }
     }
     if (part)
-        for (int c = threadIdx.x; c < H; c += 256) part[(int64_t)blockIdx.x * H + c] = acc[c];
+        for (int c = threadIdx.x; c < H; c += 256) {
+            if (gridDim.x == 1) dw[c] = from_f<W>(acc[c]);
+            else part[(int64_t)blockIdx.x * H + c] = acc[c];
+        }
 }
 
 // dw[c] = sum over the P partial rows: 32 columns a CTA, 32 warps over the rows
@@ -677,10 +687,13 @@ template <typename T, typename W> static int norm_fwd(const NormFwd &a, cudaStre
 // the launches write P partial rows of dw
 template <typename T, typename W, int NV, bool DSUM, bool DW>
 static int bwd_launch(const NormBwd &a, const RowPlan &p, int *P, cudaStream_t st) {
-    const int groups = p.block / p.tpr, fold = DW && groups > 1 ? groups * a.H * 4 : 0;
+    const int groups = p.block / p.tpr, fold = DW ? groups * a.H * 4 : 0;
     const int smem = std::max(ring_slots(NV, DSUM ? 3 : 2, kBwdSlots) * 16 * p.block, fold);
     if (!allow_smem(norm_bwd_rows<T, W, NV, DSUM, DW>, smem)) return USAF_ECUDA;
-    const int grid = row_grid(p, smem, NV == 4 ? 128 : NV == 3 ? 104 : 80, a.rows, DW ? kNormMaxPartials : 1 << 30);
+    // up to four turns in one CTA, which then needs no reduction of partial sums
+    const int grid = DW && a.rows <= 4 * groups
+                         ? 1
+                         : row_grid(p, smem, NV == 4 ? 128 : NV == 3 ? 104 : 80, a.rows, DW ? kNormMaxPartials : 1 << 30);
     if (!launch_early(norm_bwd_rows<T, W, NV, DSUM, DW>, dim3(grid), p.block, smem, st, a, p.tpr)) return USAF_ECUDA;
     *P = grid;
     return USAF_OK;
@@ -716,7 +729,8 @@ template <typename T, typename W> static int bwd_rows(const NormBwd &a, int *P, 
     if (!allow_smem(norm_bwd_any<T, W>, smem)) return USAF_ECUDA;
     *P = (int)std::min<int64_t>(a.rows, kNormMaxPartials);
     norm_bwd_any<T, W><<<*P, 256, smem, st>>>((const T *)a.dy, a.lddy, (const T *)a.x, a.ldx, (const W *)a.w, a.rstd,
-                                              (const T *)a.dsum, a.ldds, a.rows, a.H, (T *)a.dx, a.dw ? a.part : nullptr);
+                                              (const T *)a.dsum, a.ldds, a.rows, a.H, (T *)a.dx, a.dw ? a.part : nullptr,
+                                              (W *)a.dw);
     USAF_CHECK_LAUNCH();
     return USAF_OK;
 }
@@ -727,7 +741,7 @@ template <typename T, typename W> static int norm_bwd(const NormBwd &a, cudaStre
         const int rc = bwd_rows<T, W>(a, &P, st);
         if (rc) return rc;
     }
-    if (a.dw) {
+    if (a.dw && P != 1) {                    // one CTA has written dw itself
         if (!launch_early(norm_dw_kernel<W>, dim3(cdiv(a.H, 32)), 1024, 0, st, (const float *)a.part, P, a.H,
                           (W *)a.dw))
             return USAF_ECUDA;
