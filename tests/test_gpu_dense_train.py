@@ -217,3 +217,49 @@ def test_tokens_outside_the_table_and_refusals(dev):
     with pytest.raises(ValueError, match="leaf"):
         from usaf_b200 import embedding
         embedding.embedding(batch(1), m.model.embed_tokens.weight * 1.0, into_grad=True)
+
+
+@pytest.mark.parametrize("into", [False, True])
+def test_captured_forward_and_backward(dev, into):
+    """Lookup, norm with residual and their backward pass through autograd as one
+    graph (warmed up on a side stream, as torch asks): a replay with other
+    tokens gives what the eager pass gives."""
+    from usaf_b200 import embedding, norms
+    V, W = 300, 256
+    g = torch.Generator(device=dev).manual_seed(4)
+    table = torch.randn(V, W, device=dev, generator=g).requires_grad_(True)
+    weight = torch.rand(W, device=dev, generator=g).requires_grad_(True)
+    ids = torch.randint(0, V, (3, 50), device=dev, generator=g)
+    other = torch.randint(0, V, (3, 50), device=dev, generator=g)
+
+    def run():
+        x = embedding.embedding(ids, table, 2.0, padding_idx=1, into_grad=into)
+        y, total = norms.rms_norm(x, weight, 1e-6, residual=x.detach())
+        (y.square().sum() + total.sum()).backward()
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            table.grad = weight.grad = None
+            run()
+    torch.cuda.current_stream().wait_stream(side)
+    if into:
+        table.grad.zero_()
+        weight.grad.zero_()
+    else:
+        table.grad = weight.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    ids.copy_(other)
+    if into:
+        table.grad.zero_()
+        weight.grad.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    got = table.grad.clone(), weight.grad.clone()
+    table.grad = weight.grad = None
+    run()
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], table.grad) and torch.equal(got[1], weight.grad)

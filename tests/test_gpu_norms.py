@@ -175,6 +175,24 @@ def test_rows_of_zeros_and_of_bad_values(dev):
         assert bool(torch.isnan(y[9]).all())
 
 
+@pytest.mark.parametrize("H", [128, 771, 2048, 40000 // 8])
+def test_rows_near_the_ends_of_the_range(dev, H):
+    """Rows of 1e-20 with their rstd of 1e20, and of 1e15: no intermediate value
+    leaves the range that the result has."""
+    from usaf_b200 import norms
+    w, dy = 1 + 0.3 * rand(dev, 1, H), rand(dev, 2, 6, H)
+    x = rand(dev, 3, 6, H) * torch.tensor([1e-20, 1e-17, 1e-10, 1.0, 1e10, 1e15], device=dev).view(6, 1)
+    rstd = (1 / x.double().square().mean(1).sqrt()).float()
+    dx, dw = norms.rms_norm_backward(dy, x, w, rstd)
+    r = rstd.double().view(6, 1)
+    g, hat = dy.double() * w.double(), x.double() * r
+    c = (g * hat).mean(1, keepdim=True)
+    tol = (H / 32 + 60) * E * r * (g.abs() + hat.abs() * (g * hat).abs().mean(1, keepdim=True))
+    assert bool(((dx.double() - r * (g - hat * c)).abs() <= tol).all())
+    t = dy.double() * hat
+    assert bool(((dw.double() - t.sum(0)).abs() <= (66 + H / 32) * E * t.abs().sum(0)).all())
+
+
 def test_autograd_and_differences(dev):
     """The gradients of the differentiable form against the formulas' and
     against central differences of the 64-bit function."""

@@ -303,8 +303,7 @@ __global__ void __launch_bounds__(kNormMaxBlock) norm_bwd_rows(const NormBwd a, 
             }
         }
         const float2 h = halves(dot);
-        // hat c = s r mean(g s r): s times this
-        const float along = row_sum(h.x + h.y, tpr, group, red[flip]) * inv_h * r * r * r;
+        const float along = row_sum(h.x + h.y, tpr, group, red[flip]) * inv_h * r;     // mean(g s r)
         flip ^= 1;
         if (in) {
             const uint64_t back = pair(-along, -along);
@@ -315,7 +314,8 @@ __global__ void __launch_bounds__(kNormMaxBlock) norm_bwd_rows(const NormBwd a, 
                     unpack<T>(ring.get(0, i), x);
                     unpack<T>(ring.get(1, i), d);
 #pragma unroll
-                    for (int k = 0; k < N2; ++k) x[k] = fma2(mul2(d[k], w[i][k]), r2, mul2(x[k], back));
+                    for (int k = 0; k < N2; ++k)
+                        x[k] = mul2(fma2(mul2(x[k], r2), back, mul2(d[k], w[i][k])), r2);
                     if constexpr (DSUM) {
                         unpack<T>(ring.get(DSUM ? 2 : 0, i), d);
 #pragma unroll
@@ -394,7 +394,7 @@ __device__ __forceinline__ float lane_sum(float v, int per) {
 constexpr int kTileRows = 256;
 
 template <typename T, typename W, bool RES>
-__global__ void __launch_bounds__(256) norm_fwd_tile(const NormFwd a, int R, int per) {
+__global__ void __launch_bounds__(256, 5) norm_fwd_tile(const NormFwd a, int R, int per) {
     extern __shared__ uint4 dyn[];
     T *t0 = reinterpret_cast<T *>(dyn), *t1 = t0 + R * a.H;
     float *w = reinterpret_cast<float *>(RES ? t1 + R * a.H : t1);
@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(256) norm_fwd_tile(const NormFwd a, int R, int
 }
 
 template <typename T, typename W, bool DSUM, bool DW>
-__global__ void __launch_bounds__(256) norm_bwd_tile(const NormBwd a, int R, int per) {
+__global__ void __launch_bounds__(256, 5) norm_bwd_tile(const NormBwd a, int R, int per) {
     extern __shared__ uint4 dyn[];
     __shared__ float rstd[kTileRows];
     T *tx = reinterpret_cast<T *>(dyn), *td = tx + R * a.H, *ts = td + R * a.H;
@@ -476,10 +476,10 @@ __global__ void __launch_bounds__(256) norm_bwd_tile(const NormBwd a, int R, int
                 rs = rstd[r];
                 for (int c = l; c < a.H; c += per) dot = fmaf(to_f(d[c]) * w[c], to_f(x[c]), dot);
             }
-            const float along = lane_sum(dot, per) / (float)a.H * rs * rs * rs;
+            const float along = lane_sum(dot, per) / (float)a.H * rs;                  // mean(g s r)
             if (r < nr)
                 for (int c = l; c < a.H; c += per) {
-                    float v = fmaf(to_f(d[c]) * w[c], rs, -along * to_f(x[c]));
+                    float v = rs * fmaf(to_f(x[c]) * rs, -along, to_f(d[c]) * w[c]);
                     if (DSUM) v += to_f(s[c]);
                     d[c] = from_f<T>(v);
                 }
