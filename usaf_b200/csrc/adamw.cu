@@ -15,6 +15,8 @@
 // 1.31 ms, 103 % of the measured copy rate.  With 8-bit states (10 bytes a value
 // instead of 28) it is the instructions, 41 a value at 70 % of the issue slots:
 // 0.58 ms, 84 % of that rate.
+#include <cstring>
+
 #include <cuda_fp8.h>
 
 #include "common.cuh"
@@ -24,9 +26,15 @@ namespace usaf {
 
 constexpr int kAdamBlock = 256;      // values per scale, and the unit of the tensors' places
 
+// each constant twice, as the operand of an f32x2 instruction
 struct AdamwConsts {
-    float b1, omb1, b2, omb2, inv_root2, eps, step_size, gmul, one;
+    uint64_t b1, omb1, b2, omb2, inv_root2, eps, neg_step, gmul, one, half, neg_one, huge;
 };
+static uint64_t twice(float v) {
+    uint32_t u;
+    std::memcpy(&u, &v, 4);
+    return (uint64_t)u << 32 | u;
+}
 
 // the tensors of one launch, passed by value: nothing on the device to keep or to update
 template <int N> struct AdamwTable {
@@ -97,7 +105,7 @@ template <typename T> __device__ __forceinline__ void store8(T *p, bool whole, i
 // a + b by a multiply-add with a 1 that comes with the launch: f32x2 additions of
 // f32x2 products, and multiply-adds with a known 1, were fused with the products
 // (observed: the weights came out as a fused multiply-add's)
-__device__ __forceinline__ uint64_t sum2(uint64_t a, uint64_t b, float one) { return fma2(a, pair(one, one), b); }
+__device__ __forceinline__ uint64_t sum2(uint64_t a, uint64_t b, uint64_t one) { return fma2(a, one, b); }
 
 // Root and quotient by an approximation and one corrected step (Markstein's
 // method: the residual of the first result by a fused multiply-add, times the
@@ -105,7 +113,6 @@ __device__ __forceinline__ uint64_t sum2(uint64_t a, uint64_t b, float one) { re
 // for every significand (2^24 of each of eleven exponents compared) down to a
 // radicand of 2^-125, below which the residual is too small for a number; with a
 // third of the instructions, which bound the step with 8-bit states.
-__device__ __forceinline__ uint64_t neg2(uint64_t a) { return mul2(a, pair(-1.0f, -1.0f)); }
 __device__ __forceinline__ float rsqrt_approx(float v) {
     float r;
     asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
@@ -116,17 +123,17 @@ __device__ __forceinline__ float rcp_approx(float v) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
-__device__ __forceinline__ uint64_t root2(uint64_t v) {
+__device__ __forceinline__ uint64_t root2(const AdamwConsts &c, uint64_t v) {
     const float2 w = halves(v);
     const uint64_t y = pair(rsqrt_approx(w.x), rsqrt_approx(w.y));
     const uint64_t s = mul2(v, y);
-    return fma2(fma2(neg2(s), s, v), mul2(y, pair(0.5f, 0.5f)), s);
+    return fma2(fma2(mul2(s, c.neg_one), s, v), mul2(y, c.half), s);
 }
-__device__ __forceinline__ uint64_t quot2(uint64_t a, uint64_t b) {
+__device__ __forceinline__ uint64_t quot2(const AdamwConsts &c, uint64_t a, uint64_t b) {
     const float2 w = halves(b);
     const uint64_t y = pair(rcp_approx(w.x), rcp_approx(w.y));
     const uint64_t q = mul2(a, y);
-    return fma2(fma2(neg2(q), b, a), y, q);
+    return fma2(fma2(mul2(q, c.neg_one), b, a), y, q);
 }
 __device__ __forceinline__ float warp_top(float v) {     // largest magnitude of the warp
     float r;
@@ -140,20 +147,20 @@ __device__ __forceinline__ void step8(const AdamwConsts &c, float keep, uint64_t
                                       uint64_t *v, uint64_t *root) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        const uint64_t gk = mul2(g[k], pair(c.gmul, c.gmul));
-        m[k] = sum2(mul2(m[k], pair(c.b1, c.b1)), mul2(gk, pair(c.omb1, c.omb1)), c.one);
-        v[k] = sum2(mul2(v[k], pair(c.b2, c.b2)), mul2(mul2(gk, pair(c.omb2, c.omb2)), gk), c.one);
+        const uint64_t gk = mul2(g[k], c.gmul);
+        m[k] = sum2(mul2(m[k], c.b1), mul2(gk, c.omb1), c.one);
+        v[k] = sum2(mul2(v[k], c.b2), mul2(mul2(gk, c.omb2), gk), c.one);
         uint64_t up;
         if (EIGHT) {
-            root[k] = root2(v[k]);
-            up = quot2(m[k], sum2(mul2(root[k], pair(c.inv_root2, c.inv_root2)), pair(c.eps, c.eps), c.one));
+            root[k] = root2(c, v[k]);
+            up = quot2(c, m[k], sum2(mul2(root[k], c.inv_root2), c.eps, c.one));
         } else {
             const float2 w = halves(v[k]), h = halves(m[k]);
             root[k] = pair(__fsqrt_rn(w.x), __fsqrt_rn(w.y));
-            const float2 den = halves(sum2(mul2(root[k], pair(c.inv_root2, c.inv_root2)), pair(c.eps, c.eps), c.one));
+            const float2 den = halves(sum2(mul2(root[k], c.inv_root2), c.eps, c.one));
             up = pair(__fdiv_rn(h.x, den.x), __fdiv_rn(h.y, den.y));
         }
-        p[k] = sum2(mul2(p[k], pair(keep, keep)), mul2(up, pair(-c.step_size, -c.step_size)), c.one);
+        p[k] = sum2(mul2(p[k], pair(keep, keep)), mul2(up, c.neg_step), c.one);
     }
 }
 
@@ -175,7 +182,7 @@ __device__ __forceinline__ void decode(const Codes &q, uint64_t *m, uint64_t *v)
         v[k] = mul2(v[k], v[k]);
     }
 }
-__device__ __forceinline__ Codes encode(const uint64_t *m, const uint64_t *root) {
+__device__ __forceinline__ Codes encode(const AdamwConsts &c, const uint64_t *m, const uint64_t *root) {
     float am = 0.0f, av = 0.0f;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -194,7 +201,7 @@ __device__ __forceinline__ Codes encode(const uint64_t *m, const uint64_t *root)
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         a[k] = mul2(m[k], pair(mm, mm));
-        const float2 q = halves(mul2(root[k], pair(mv, mv))), any = halves(mul2(root[k], pair(1e30f, 1e30f)));
+        const float2 q = halves(mul2(root[k], pair(mv, mv))), any = halves(mul2(root[k], c.huge));
         b[k] = pair(fmaxf(q.x, fminf(any.x, least)), fmaxf(q.y, fminf(any.y, least)));
     }
     Codes q;
@@ -315,7 +322,7 @@ adamw_kernel(const __grid_constant__ AdamwTable<N> tab, const AdamwState s, cons
             step8<true>(c, keep, g, p, m, v, root);
             store8<P>(pp, true, 8, p);
             if (MASTER) store8<float>(s.master + f, true, 8, p);
-            store_codes(s, encode(m, root), f, blk, lane);
+            store_codes(s, encode(c, m, root), f, blk, lane);
             stage = stage == Ring::D - 1 ? 0 : stage + 1;
             pp += kAdamBlock;
             f += kAdamBlock;
@@ -355,7 +362,7 @@ adamw_kernel(const __grid_constant__ AdamwTable<N> tab, const AdamwState s, cons
         // the values behind a tensor's end stay as they are
         if (MASTER) store8<float>(s.master + f, n == 8, n, p);
         if (EIGHT) {
-            store_codes(s, encode(m, root), f, blk, lane);
+            store_codes(s, encode(c, m, root), f, blk, lane);
         } else {
             store8<float>(m32, n == 8, n, m);
             store8<float>(v32, n == 8, n, v);
@@ -443,15 +450,18 @@ extern "C" int usaf_adamw(int32_t n_tensors, void *const *p, const void *const *
         USAF_REQUIRE(numel[i] >= 0 && (numel[i] == 0 || (p[i] && g[i])) && start[i] >= 0 && start[i] % kAdamBlock == 0);
     const AdamwList tensors{p, g, numel, start, weight_decay};
     AdamwConsts c;
-    c.b1 = (float)beta1;
-    c.omb1 = (float)(1.0 - beta1);
-    c.b2 = (float)beta2;
-    c.omb2 = (float)(1.0 - beta2);
-    c.inv_root2 = (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step)));
-    c.eps = (float)eps;
-    c.step_size = (float)(lr / (1.0 - std::pow(beta1, (double)step)));
-    c.gmul = (float)(1.0 / grad_div);
-    c.one = 1.0f;
+    c.b1 = twice((float)beta1);
+    c.omb1 = twice((float)(1.0 - beta1));
+    c.b2 = twice((float)beta2);
+    c.omb2 = twice((float)(1.0 - beta2));
+    c.inv_root2 = twice((float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step))));
+    c.eps = twice((float)eps);
+    c.neg_step = twice(-(float)(lr / (1.0 - std::pow(beta1, (double)step))));
+    c.gmul = twice((float)(1.0 / grad_div));
+    c.one = twice(1.0f);
+    c.half = twice(0.5f);
+    c.neg_one = twice(-1.0f);
+    c.huge = twice(1e30f);
     const AdamwState s{master, m, v, m_scale, v_scale};
     const bool eight = bits == 8;
     cudaStream_t st = as_stream(stream);
