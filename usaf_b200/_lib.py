@@ -115,16 +115,17 @@ def call(name: str, *args):
         raise UsafError(f"{name} failed: {_STATUS.get(rc, rc)} (status {rc})")
 
 
-def call_on(device: torch.device, name: str, *args):
-    """:func:`call` on the current stream of ``device`` (appended as the last
-    argument), whichever device is current.  The raw stream handle is taken
-    directly: building the Stream object costs as much as a launch."""
-    st = torch._C._cuda_getCurrentRawStream(device.index)
-    if device.index == torch.cuda.current_device():
-        call(name, *args, st)
+def call_on(index: int, name: str, *args):
+    """:func:`call` on the current stream of CUDA device ``index`` (appended as
+    the last argument), whichever device is current.  The raw stream handle is
+    taken directly: building the Stream object costs as much as a launch."""
+    if index == torch._C._cuda_getDevice():
+        rc = getattr(LIB, name)(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(device):
-            call(name, *args, st)
+        with torch.cuda.device(index):
+            rc = getattr(LIB, name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != 0:
+        raise UsafError(f"{name} failed: {_STATUS.get(rc, rc)} (status {rc})")
 
 
 _DTYPES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}

@@ -23,17 +23,20 @@ from . import _lib
 from ._lib import call_on, ptr
 
 
-def _check_ids(ids: torch.Tensor, device: torch.device) -> torch.Tensor:
-    if ids.dtype not in (torch.int32, torch.int64):
+def _check_ids(ids: torch.Tensor, of: torch.Tensor) -> torch.Tensor:
+    if ids.dtype is not torch.int64 and ids.dtype is not torch.int32:
         raise TypeError(f"ids: expected int32 or int64, got {ids.dtype}")
-    if ids.device != device:
-        raise ValueError(f"ids: expected on {device}, got {ids.device}")
+    if ids.get_device() != of.get_device():
+        raise ValueError(f"ids: expected on {of.device}, got {ids.device}")
     return ids.contiguous()
 
 
-def _check_err(err: Optional[torch.Tensor], device: torch.device) -> None:
-    if err is not None and (err.dtype != torch.int32 or err.numel() < 1 or err.device != device):
-        raise ValueError(f"err: expected an int32 word on {device}")
+def _err_at(err: Optional[torch.Tensor], of: torch.Tensor) -> Optional[int]:
+    if err is None:
+        return None
+    if err.dtype is not torch.int32 or err.numel() < 1 or err.get_device() != of.get_device():
+        raise ValueError(f"err: expected an int32 word on {of.device}")
+    return err.data_ptr()
 
 
 def _padding(padding_idx: Optional[int], V: int) -> int:
@@ -51,12 +54,14 @@ def embedding_forward(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0
         raise ValueError(f"table: expected [rows, width], got {tuple(table.shape)}")
     if not table.is_contiguous():
         raise ValueError("table: must be contiguous")
-    ids = _check_ids(ids, table.device)
-    _check_err(err, table.device)
+    ids = _check_ids(ids, table)
+    err_at = _err_at(err, table)
+    code = _lib.dtype_code(table.dtype)
+    at = ptr(table)               # on a CUDA device, and so are the others
     V, H = table.shape
-    out = torch.empty(*ids.shape, H, dtype=table.dtype, device=table.device)
-    call_on(table.device, "usaf_embedding_fwd", ptr(ids), 8 * ids.element_size(), ids.numel(), ptr(table),
-            _lib.dtype_code(table.dtype), V, H, float(scale), ptr(out), ptr(err))
+    out = table.new_empty((*ids.shape, H))
+    call_on(table.get_device(), "usaf_embedding_fwd", ids.data_ptr(), 8 * ids.element_size(), ids.numel(), at, code, V, H,
+            float(scale), out.data_ptr(), err_at)
     return out
 
 
@@ -70,29 +75,31 @@ def embedding_backward(dout: torch.Tensor, ids: torch.Tensor, num_embeddings: in
     V = int(num_embeddings)
     if V < 0:
         raise ValueError(f"num_embeddings: expected >= 0, got {V}")
-    if dout.dim() < 1 or dout.shape[:-1] != ids.shape or dout.shape[-1] < 1:
-        raise ValueError(f"dout: expected shape {tuple(ids.shape)} + (width,), got {tuple(dout.shape)}")
-    H = dout.shape[-1]
-    ids = _check_ids(ids, dout.device)
-    _check_err(err, dout.device)
+    shape = dout.shape
+    if not shape or shape[:-1] != ids.shape or shape[-1] < 1:
+        raise ValueError(f"dout: expected shape {tuple(ids.shape)} + (width,), got {tuple(shape)}")
+    H = shape[-1]
+    ids = _check_ids(ids, dout)
+    err_at = _err_at(err, dout)
     pad = _padding(padding_idx, V)
     dout = dout.contiguous()
+    code = g_code = _lib.dtype_code(dout.dtype)
+    at = ptr(dout)                # on a CUDA device, and so are the others
     adds = grad is not None
     if adds:
         if tuple(grad.shape) != (V, H):
             raise ValueError(f"grad: expected shape {(V, H)}, got {tuple(grad.shape)}")
-        if grad.dtype not in (dout.dtype, torch.float32):
+        if grad.dtype is not dout.dtype and grad.dtype is not torch.float32:
             raise TypeError(f"grad: expected {dout.dtype} or torch.float32, got {grad.dtype}")
-        if grad.device != dout.device or not grad.is_contiguous():
+        if grad.get_device() != dout.get_device() or not grad.is_contiguous():
             raise ValueError(f"grad: must be contiguous, on {dout.device}")
+        g_code = _lib.dtype_code(grad.dtype)
     else:
-        grad = torch.empty(V, H, dtype=dout.dtype, device=dout.device)
+        grad = dout.new_empty((V, H))
     n = ids.numel()
-    ws = torch.empty(max(int(_lib.LIB.usaf_embedding_workspace_bytes(n, V, H)), 16), dtype=torch.uint8,
-                     device=dout.device)
-    call_on(dout.device, "usaf_embedding_bwd", ptr(dout), ptr(ids), 8 * ids.element_size(), n,
-            _lib.dtype_code(dout.dtype), V, H, float(scale), pad, int(adds), ptr(grad),
-            _lib.dtype_code(grad.dtype), ptr(ws), ptr(err))
+    ws = dout.new_empty(_lib.LIB.usaf_embedding_workspace_bytes(n, V, H), dtype=torch.uint8)
+    call_on(dout.get_device(), "usaf_embedding_bwd", at, ids.data_ptr(), 8 * ids.element_size(), n, code, V, H,
+            float(scale), pad, int(adds), grad.data_ptr(), g_code, ws.data_ptr(), err_at)
     return grad
 
 

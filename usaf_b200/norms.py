@@ -25,9 +25,8 @@ from ._lib import call_on, ptr
 MAX_WIDTH = 32768
 
 
-def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
+def _rows(t: torch.Tensor, H: int) -> Tuple[torch.Tensor, int]:
     """``t`` (or a copy) as rows of its last dimension, and their stride."""
-    H = t.shape[-1]
     if t.is_contiguous():
         return t, H
     if t.stride(-1) == 1:
@@ -39,28 +38,31 @@ def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
     return t.contiguous(), H
 
 
-def _check(x: torch.Tensor, weight: torch.Tensor) -> int:
-    """The width of the rows."""
-    if x.dim() < 1 or weight.dim() != 1 or weight.shape[0] != x.shape[-1] or x.shape[-1] < 1:
-        raise ValueError(f"weight: expected shape ({x.shape[-1] if x.dim() else '?'},), got {tuple(weight.shape)}")
-    H = x.shape[-1]
+def _check(x: torch.Tensor, weight: torch.Tensor) -> Tuple[int, int, int, int]:
+    """Width of the rows, their device and the types' codes."""
+    shape = x.shape
+    H = shape[-1] if shape else 0
+    if H < 1 or weight.dim() != 1 or weight.numel() != H:
+        raise ValueError(f"weight: expected shape ({H or '?'},), got {tuple(weight.shape)}")
     if H > MAX_WIDTH:
         raise ValueError(f"rows of {H} values; at most {MAX_WIDTH} are handled")
-    if weight.dtype is not x.dtype and weight.dtype is not torch.float32:
-        raise TypeError(f"weight: expected {x.dtype} or torch.float32, got {weight.dtype}")
-    if weight.device != x.device:
+    dt, wdt, dev = x.dtype, weight.dtype, x.get_device()
+    if wdt is not dt and wdt is not torch.float32:
+        raise TypeError(f"weight: expected {dt} or torch.float32, got {wdt}")
+    if weight.get_device() != dev:
         raise ValueError("weight: expected on the device of the rows")
     if not weight.is_contiguous():
         raise ValueError("weight: must be contiguous")
-    return H
+    code = _lib.dtype_code(dt)
+    return H, dev, code, code if wdt is dt else _lib.F32
 
 
 def _check_like(name: str, t: torch.Tensor, x: torch.Tensor) -> None:
-    if t.shape != x.shape:
+    if not t.is_same_size(x):
         raise ValueError(f"{name}: expected shape {tuple(x.shape)}, got {tuple(t.shape)}")
     if t.dtype is not x.dtype:
         raise TypeError(f"{name}: expected dtype {x.dtype}, got {t.dtype}")
-    if t.device != x.device:
+    if t.get_device() != x.get_device():
         raise ValueError(f"{name}: expected on {x.device}, got {t.device}")
 
 
@@ -74,20 +76,22 @@ def rms_norm_forward(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     type (``x`` itself without a residual), ``y`` its norm, ``rstd`` the fp32
     1/sqrt(mean + eps) of every row for :func:`rms_norm_backward` (None unless
     wanted)."""
-    H = _check(x, weight)
+    H, dev, code, wcode = _check(x, weight)
     if not eps >= 0:
         raise ValueError(f"eps: expected >= 0, got {eps}")
     n = x.numel() // H
-    xr, ldx = _rows(x)
+    xr, ldx = _rows(x, H)
+    at = ptr(xr)                  # on a CUDA device, and so are the others
     y = _dense_like(x)
     rstd = x.new_empty(n, dtype=torch.float32) if want_rstd else None
-    total, rr, ldr = x, None, 0
+    total, res_at, ldr, total_at = x, None, 0, None
     if residual is not None:
         _check_like("residual", residual, x)
-        rr, ldr = _rows(residual)
+        residual, ldr = _rows(residual, H)
         total = _dense_like(x)
-    call_on(x.device, "usaf_rms_norm_fwd", ptr(xr), ldx, ptr(rr), ldr, ptr(weight), _lib.dtype_code(x.dtype),
-            _lib.dtype_code(weight.dtype), n, H, float(eps), None if rr is None else ptr(total), ptr(y), ptr(rstd))
+        res_at, total_at = residual.data_ptr(), total.data_ptr()
+    call_on(dev, "usaf_rms_norm_fwd", at, ldx, res_at, ldr, weight.data_ptr(), code, wcode, n, H, float(eps), total_at,
+            y.data_ptr(), rstd.data_ptr() if want_rstd else None)
     return y, rstd, total
 
 
@@ -97,24 +101,27 @@ def rms_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, r
     :func:`rms_norm_forward`.  ``dsum``, the gradient of ``total`` where it is
     used further, is added to ``dx``, which is then the gradient of ``x`` and of
     ``residual`` alike.  ``dw`` has the weight's type (None unless wanted)."""
-    H = _check(x, weight)
+    H, dev, code, wcode = _check(x, weight)
     n = x.numel() // H
     _check_like("dy", dy, x)
-    if rstd.numel() != n or rstd.dtype != torch.float32 or rstd.device != x.device or not rstd.is_contiguous():
+    if rstd.numel() != n or rstd.dtype is not torch.float32 or rstd.get_device() != dev or not rstd.is_contiguous():
         raise ValueError(f"rstd: expected {n} contiguous fp32 values on {x.device}")
-    xr, ldx = _rows(x)
-    dyr, lddy = _rows(dy)
-    dsr, ldds = None, 0
+    xr, ldx = _rows(x, H)
+    at = ptr(xr)                  # on a CUDA device, and so are the others
+    dyr, lddy = _rows(dy, H)
+    ds_at, ldds = None, 0
     if dsum is not None:
         _check_like("dsum", dsum, x)
-        dsr, ldds = _rows(dsum)
+        dsum, ldds = _rows(dsum, H)
+        ds_at = dsum.data_ptr()
     dx = _dense_like(x)
-    dw = ws = None
+    dw = dw_at = ws_at = None
     if want_dw:
         dw = torch.empty_like(weight)
         ws = x.new_empty(_lib.LIB.usaf_rms_norm_workspace_bytes(n, H), dtype=torch.uint8)
-    call_on(x.device, "usaf_rms_norm_bwd", ptr(dyr), lddy, ptr(xr), ldx, ptr(weight), ptr(rstd), ptr(dsr), ldds,
-            _lib.dtype_code(x.dtype), _lib.dtype_code(weight.dtype), n, H, ptr(dx), ptr(dw), ptr(ws))
+        dw_at, ws_at = dw.data_ptr(), ws.data_ptr()
+    call_on(dev, "usaf_rms_norm_bwd", dyr.data_ptr(), lddy, at, ldx, weight.data_ptr(), rstd.data_ptr(), ds_at, ldds,
+            code, wcode, n, H, dx.data_ptr(), dw_at, ws_at)
     return dx, dw
 
 
