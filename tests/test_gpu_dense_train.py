@@ -105,7 +105,7 @@ def test_gradients_against_the_modules(dev, tie, recompute):
         finally:
             if dense:
                 norms.call_on = embedding.call_on = kept
-        losses.append(float(loss))
+        losses.append(float(loss.detach()))
         grads.append({n: p.grad.double() for n, p in m.named_parameters() if p.grad is not None})
     twice = 2 if recompute else 1
     assert calls["usaf_rms_norm_fwd"] == 1 + 4 * LAYERS * twice and calls["usaf_rms_norm_bwd"] == 1 + 4 * LAYERS
@@ -263,3 +263,21 @@ def test_captured_forward_and_backward(dev, into):
     run()
     torch.cuda.synchronize()
     assert torch.equal(got[0], table.grad) and torch.equal(got[1], weight.grad)
+
+
+def test_token_by_token_with_a_cache(dev):
+    """Single tokens through the patched layers and the model's cache: the
+    logits of the modules, within the rounding of ~25 operations (2e-4)."""
+    ids = batch(7)
+    out = []
+    for dense in (False, True):
+        m = make(dev, torch.float32, dense=dense).eval()
+        with torch.no_grad():
+            first = m(input_ids=ids[:, :40], use_cache=True)
+            logits, past = [first.logits[:, -1]], first.past_key_values
+            for t in range(40, 44):
+                step = m(input_ids=ids[:, t:t + 1], past_key_values=past, use_cache=True)
+                logits.append(step.logits[:, -1])
+                past = step.past_key_values
+        out.append(torch.stack(logits).double())
+    assert float((out[0] - out[1]).norm()) <= 2e-4 * float(out[0].norm())

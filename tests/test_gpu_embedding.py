@@ -63,7 +63,8 @@ def check_grad(got, dy, ids, V, scale, pad=None, start=None):
 
 
 CASES = [(1, 1, 1), (1, 50, 7), (2, 3, 64), (16, 1000, 2048), (33, 40, 129), (300, 77, 1000), (511, 90, 40), (512, 3000, 72), (513, 90, 40), (1025, 5000, 256),
-         (4097, 300, 96), (9000, 70000, 40), (3001, 2, 2048), (20000, 1, 24)]
+         (4097, 300, 96), (9000, 70000, 40), (3001, 2, 2048), (20000, 1, 24),
+         (100, 2 ** 23 + 5, 2), (3000, 2 ** 18 + 1, 4)]
 
 
 @pytest.mark.parametrize("n,V,H", CASES)

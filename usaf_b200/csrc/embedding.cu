@@ -263,28 +263,30 @@ embed_sort_kernel(const SortArgs a) {
     }
 }
 
-// Up to 512 pairs: one CTA counts for every pair those that come before it (a
-// smaller key, or the same one earlier), 4 keys a load: 2 to 3 us, where the
-// cluster's passes and barriers take 12 whatever they sort.
+// Up to 512 pairs of a table of up to 2^23 - 2 rows: key and position fit 32 bits
+// together, and one CTA counts for every pair those that are smaller, 4 a load.
+// The cluster's passes and barriers take 12 us whatever they sort.
 constexpr int kFewTokens = 512;
+constexpr int64_t kFewRows = (1 << 23) - 2;
 
-__global__ void __launch_bounds__(kFewTokens) embed_sort_few_kernel(const SortArgs a, uint2 *__restrict__ sorted) {
-    __shared__ alignas(16) uint32_t key[kFewTokens];
+__global__ void __launch_bounds__(2 * kFewTokens) embed_sort_few_kernel(const SortArgs a, uint2 *__restrict__ sorted) {
+    __shared__ alignas(16) uint32_t keys[kFewTokens];
     wait_for_previous();
     let_next_start();
-    const uint32_t j = threadIdx.x, mine = j < a.tokens ? sort_key(a, j) : 0xffffffffu;
-    key[j] = mine;
+    // two threads a pair, each over every other four keys
+    const uint32_t j = threadIdx.x >> 1, half = threadIdx.x & 1;
+    const uint32_t key = j < a.tokens ? sort_key(a, j) : 0, mine = j < a.tokens ? key << 9 | j : 0xffffffffu;
+    if (half == 0) keys[j] = mine;
     __syncthreads();
-    if (j >= a.tokens) return;
     uint32_t to = 0;
-    const uint32_t last = (a.tokens + 3) / 4;           // the keys behind the tokens are larger than any
+    const uint32_t n = (a.tokens + 3) / 4;              // what lies behind the tokens is larger than any
 #pragma unroll 4
-    for (uint32_t i = 0; i < last; ++i) {
-        const uint4 k = reinterpret_cast<const uint4 *>(key)[i];
-        to += (k.x < mine || (k.x == mine && 4 * i < j)) + (k.y < mine || (k.y == mine && 4 * i + 1 < j)) +
-              (k.z < mine || (k.z == mine && 4 * i + 2 < j)) + (k.w < mine || (k.w == mine && 4 * i + 3 < j));
+    for (uint32_t i = half; i < n; i += 2) {
+        const uint4 k = reinterpret_cast<const uint4 *>(keys)[i];
+        to += (k.x < mine) + (k.y < mine) + (k.z < mine) + (k.w < mine);
     }
-    sorted[to] = make_uint2(mine, j);
+    to += __shfl_xor_sync(0xffffffffu, to, 1);
+    if (half == 0 && j < a.tokens) sorted[to] = make_uint2(key, j);
 }
 
 // ---- backward: sums -----------------------------------------------------------
@@ -578,8 +580,8 @@ template <typename T, typename G> static int embed_bwd(const EmbedBwd &a, cudaSt
         }
         return USAF_OK;
     }
-    const bool few = a.tokens <= kFewTokens;
-    if (!(few ? launch_early(embed_sort_few_kernel, dim3(1), kFewTokens, 0, st, s, s.pairs[0])
+    const bool few = a.tokens <= kFewTokens && a.V <= kFewRows;
+    if (!(few ? launch_early(embed_sort_few_kernel, dim3(1), 2 * kFewTokens, 0, st, s, s.pairs[0])
               : launch_early(embed_sort_kernel, dim3(kSortCtas), kSortThreads, smem, st, s)))
         return USAF_ECUDA;
     if (zero && !launch_early(embed_zero_kernel, dim3(cdiv(zero + 1, kZeroTile)), kZeroThreads, 0, st, (char *)a.grad, zero))
