@@ -360,9 +360,9 @@ __global__ void __launch_bounds__(kNormMaxBlock) norm_bwd_rows(const NormBwd a, 
 // comes into shared memory in 16-byte copies, `per` threads take a row there value
 // by value, and the results leave from where the inputs lay, in 16-byte stores.
 // dw is summed by columns, a thread's own ones, over each tile's rows.  Forward /
-// backward with dw, against a CTA a row: 20000 x 771 bf16 22 / 46 us (48 / 80),
-// 260000 x 35 21 / 39 (279 / 422); bound by the shared-memory accesses of single
-// values (about five a value forward).
+// backward with dw, against a CTA a row: 20000 x 771 bf16 21 / 47 us (48 / 80),
+// 260000 x 35 15 / 35 (279 / 422); bound by instructions, single values' accesses
+// to shared memory among them (78 % of the issue slots forward).
 template <typename T> __device__ __forceinline__ void tile_in(T *to, const T *from, int n) {
     const int nv = n * (int)sizeof(T) / 16;
     const uint32_t at = (uint32_t)__cvta_generic_to_shared(to);
@@ -401,6 +401,7 @@ __global__ void __launch_bounds__(256, 5) norm_fwd_tile(const NormFwd a, int R, 
     wait_for_previous();
     for (int c = threadIdx.x; c < a.H; c += 256) w[c] = to_f(static_cast<const W *>(a.w)[c]);
     const int l = threadIdx.x & (per - 1), g = threadIdx.x / per, groups = 256 / per;
+    const float inv_h = 1.0f / (float)a.H;
     for (int64_t row0 = (int64_t)blockIdx.x * R; row0 < a.rows; row0 += (int64_t)gridDim.x * R) {
         const int nr = (int)min((int64_t)R, a.rows - row0), n = nr * a.H;
         const int64_t at = row0 * a.H;
@@ -420,7 +421,7 @@ __global__ void __launch_bounds__(256, 5) norm_fwd_tile(const NormFwd a, int R, 
                     }
                     ss = fmaf(v, v, ss);
                 }
-            const float rs = __frcp_rn(__fsqrt_rn(lane_sum(ss, per) / (float)a.H + a.eps));
+            const float rs = __frcp_rn(__fsqrt_rn(lane_sum(ss, per) * inv_h + a.eps));
             if (r < nr) {
                 if (a.rstd && l == 0) a.rstd[row0 + r] = rs;
                 for (int c = l; c < a.H; c += per) y[c] = from_f<T>(to_f(x[c]) * rs * w[c]);
@@ -448,6 +449,7 @@ __global__ void __launch_bounds__(256, 5) norm_bwd_tile(const NormBwd a, int R, 
     if (DW)
         for (int c = threadIdx.x; c < parts * a.H; c += 256) acc[c] = 0.0f;
     const int l = threadIdx.x & (per - 1), g = threadIdx.x / per, groups = 256 / per;
+    const float inv_h = 1.0f / (float)a.H;
     for (int64_t row0 = (int64_t)blockIdx.x * R; row0 < a.rows; row0 += (int64_t)gridDim.x * R) {
         const int nr = (int)min((int64_t)R, a.rows - row0), n = nr * a.H;
         const int64_t at = row0 * a.H;
@@ -476,7 +478,7 @@ __global__ void __launch_bounds__(256, 5) norm_bwd_tile(const NormBwd a, int R, 
                 rs = rstd[r];
                 for (int c = l; c < a.H; c += per) dot = fmaf(to_f(d[c]) * w[c], to_f(x[c]), dot);
             }
-            const float along = lane_sum(dot, per) / (float)a.H * rs;                  // mean(g s r)
+            const float along = lane_sum(dot, per) * inv_h * rs;                       // mean(g s r)
             if (r < nr)
                 for (int c = l; c < a.H; c += per) {
                     float v = rs * fmaf(to_f(x[c]) * rs, -along, to_f(d[c]) * w[c]);
@@ -612,7 +614,9 @@ static int row_grid(const RowPlan &p, int smem, int regs, int64_t rows, int most
     return (int)std::min<int64_t>((rows + groups - 1) / groups, std::min(148 * per_sm, most));
 }
 
-// Tiles of dense rows: R rows (0: too wide), threads a row, bytes of shared memory.
+// Tiles of dense rows: R rows (0: too wide), threads a row (each of 16 values or
+// more: what a row costs beside them, a sum, a root and addresses, was 150 of 229
+// instructions with 32 threads to 131 values), bytes of shared memory.
 // About 8 KB a tensor, so that several CTAs an SM load, compute and store at
 // different times; at most 64 KB in all (8000 x 2050 bf16 with a residual, in 73 KB
 // forward: 39.5 us, a CTA a row 33.7).
@@ -624,8 +628,7 @@ static TilePlan plan_tile(int H, int size, int tensors, bool backward) {
     TilePlan t{16 / size, 32, 0};            // rows until the bytes are a multiple of 16
     while (t.R > 1 && (int64_t)H * size * (t.R / 2) % 16 == 0) t.R /= 2;
     t.R *= std::max(1, std::min(kTileRows, 8192 / (H * size)) / t.R);
-    if (H < 256)
-        while (t.per > 1 && t.per * 4 >= H) t.per /= 2;
+    while (t.per > 1 && t.per * 16 >= H && t.per * t.R >= 512) t.per /= 2;      // and the tile's rows for 256 threads
     // whether dw is wanted does not choose the kernel: dx has the same bits either way
     const int64_t smem = (int64_t)tensors * t.R * H * size + H * 4 + (backward ? std::max(256, H) * 4 : 0);
     if (smem > 64 * 1024) t.R = 0;
