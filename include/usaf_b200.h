@@ -396,7 +396,8 @@ int usaf_rms_norm_bwd(const void *dy, int64_t lddy, const void *x, int64_t ldx, 
  * rows without tokens become 0, or with accumulate keep their values and the
  * sum is added to the others'.  Tokens equal to padding_idx (< 0: none) are
  * left out, tokens outside [0, V) too (USAF_ERR_BAD_INDEX).  ws:
- * usaf_embedding_workspace_bytes(tokens, V, H) bytes. */
+ * usaf_embedding_workspace_bytes(tokens, V, H) bytes.
+ * H <= 2^22, tokens <= 2^30 and, backward, V <= 2^30 (USAF_EUNSUPPORTED above). */
 int usaf_embedding_fwd(const void *ids, int32_t ids_bits, int64_t tokens, const void *table,
                        int32_t dtype, int64_t V, int32_t H, double scale, void *out, int32_t *err,
                        void *stream);

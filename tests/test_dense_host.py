@@ -47,6 +47,19 @@ def test_argument_checks_come_before_the_device():
         dense_optim.adamw_step([x], [x], torch.zeros(256), torch.zeros(256), step=0, lr=1e-3)
 
 
+def test_sizes_beyond_the_call_are_refused():
+    """Widths and step numbers that the C interface's 32 bits would cut off."""
+    from usaf_b200 import dense_optim, embedding
+    wide, ids = torch.empty(1, embedding.MAX_WIDTH + 1), torch.zeros(1, dtype=torch.long)
+    with pytest.raises(ValueError, match="at most"):
+        embedding.embedding(ids, wide)
+    with pytest.raises(ValueError, match="at most"):
+        embedding.embedding_backward(wide, ids, 4)
+    x = torch.ones(2, 8)
+    with pytest.raises(ValueError, match="step"):
+        dense_optim.adamw_step([x], [x], torch.zeros(256), torch.zeros(256), step=1 << 32 | 1, lr=1e-3)
+
+
 def test_model_glue(monkeypatch):
     """use_dense_kernels on a model without MoE blocks, the kernels replaced by
     their formulas: same logits and gradients as the modules, to the rounding of

@@ -331,6 +331,12 @@ def test_refusals(dev):
         step([p], [g], q, (q[0], q[1][:1]), **kw)
     with pytest.raises(ValueError, match="masters"):
         step([p], [g], m, v, masters=p, **kw)
+    with pytest.raises(ValueError, match="must not share"):
+        step([p], [g], m, m, **kw)
+    with pytest.raises(ValueError, match="must not share"):
+        step([p], [g], m, v, masters=v, **kw)
+    with pytest.raises(ValueError, match="must not share"):
+        step([p], [g], q, (q[0].clone(), q[1]), **kw)
     with pytest.raises(ValueError, match="twice"):
         step([p, p], [g, g], torch.zeros(1024, device=dev), torch.zeros(1024, device=dev), **kw)
     with pytest.raises(ValueError, match="share memory"):

@@ -625,13 +625,14 @@ using namespace usaf;
 
 // positions and rows are 32-bit in the sort; a launch has at most 2^31 - 1 CTAs
 constexpr int64_t kMostTokens = (int64_t)1 << 30, kMostRows = (int64_t)1 << 30;
+constexpr int32_t kMostWidth = 1 << 22;
 
 extern "C" int usaf_embedding_fwd(const void *ids, int32_t ids_bits, int64_t tokens, const void *table, int32_t dtype,
                                   int64_t V, int32_t H, double scale, void *out, int32_t *err, void *stream) {
     USAF_REQUIRE(tokens >= 0 && V >= 0 && H >= 1 && (ids_bits == 32 || ids_bits == 64));
     if (tokens == 0) return USAF_OK;
     USAF_REQUIRE(ids && (table || V == 0) && out);
-    if (tokens > kMostTokens || tokens * ((H + 511) / 512) > ((int64_t)1 << 33)) return USAF_EUNSUPPORTED;
+    if (H > kMostWidth || tokens > kMostTokens || tokens * ((H + 511) / 512) > ((int64_t)1 << 33)) return USAF_EUNSUPPORTED;
     cudaStream_t st = as_stream(stream);
     const int wide = ids_bits == 64;
     switch (dtype) {
@@ -652,7 +653,7 @@ extern "C" int usaf_embedding_bwd(const void *dy, const void *ids, int32_t ids_b
                                   void *grad, int32_t grad_dtype, void *ws, int32_t *err, void *stream) {
     USAF_REQUIRE(tokens >= 0 && V >= 0 && H >= 1 && (ids_bits == 32 || ids_bits == 64));
     USAF_REQUIRE((grad || V == 0) && (tokens == 0 || (dy && ids && ws)));
-    if (tokens > kMostTokens || V > kMostRows || H > (1 << 22) ||
+    if (tokens > kMostTokens || V > kMostRows || H > kMostWidth ||
         (tokens / kChunk + 1) * ((H + 127) / 128) > ((int64_t)1 << 33))
         return USAF_EUNSUPPORTED;
     cudaStream_t st = as_stream(stream);

@@ -61,8 +61,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m:
     n = len(params)
     if len(grads) != n:
         raise ValueError(f"{len(grads)} gradients for {n} parameters")
-    if step < 1:
-        raise ValueError(f"step: expected >= 1, got {step}")
+    if not 1 <= step < 1 << 31:
+        raise ValueError(f"step: expected 1 to 2^31 - 1, got {step}")
     if grad_div == 0:
         raise ValueError("grad_div must not be 0")
     if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1 and eps >= 0):
@@ -127,6 +127,9 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m:
         _check_flat("v", v, total, torch.float32, dev)
     if masters is not None:
         _check_flat("masters", masters, total, torch.float32, dev)
+    flat = [t.data_ptr() for t in (m, v, ms, vs, masters) if t is not None]
+    if total and len(set(flat)) < len(flat):
+        raise ValueError("m, v, their scales and the masters must not share memory")
     call_on(index, "usaf_adamw", n, *[a.buffer_info()[0] for a in tab], _lib.dtype_code(dtype),
             _lib.dtype_code(g_dtype), ptr(masters), 8 if eight else 32, ptr(m), ptr(v), ptr(ms), ptr(vs),
             float(grad_div), int(step), float(lr), float(betas[0]), float(betas[1]), float(eps))

@@ -22,6 +22,8 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 from ._lib import call_on, ptr
 
+MAX_WIDTH = 1 << 22
+
 
 def _check_ids(ids: torch.Tensor, of: torch.Tensor) -> torch.Tensor:
     if ids.dtype is not torch.int64 and ids.dtype is not torch.int32:
@@ -52,6 +54,8 @@ def embedding_forward(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0
     """``scale * table[ids]``, rounded once to the table's type."""
     if table.dim() != 2 or table.shape[1] < 1:
         raise ValueError(f"table: expected [rows, width], got {tuple(table.shape)}")
+    if table.shape[1] > MAX_WIDTH:
+        raise ValueError(f"rows of {table.shape[1]} values; at most {MAX_WIDTH} are handled")
     if not table.is_contiguous():
         raise ValueError("table: must be contiguous")
     ids = _check_ids(ids, table)
@@ -79,6 +83,8 @@ def embedding_backward(dout: torch.Tensor, ids: torch.Tensor, num_embeddings: in
     if not shape or shape[:-1] != ids.shape or shape[-1] < 1:
         raise ValueError(f"dout: expected shape {tuple(ids.shape)} + (width,), got {tuple(shape)}")
     H = shape[-1]
+    if H > MAX_WIDTH:
+        raise ValueError(f"rows of {H} values; at most {MAX_WIDTH} are handled")
     ids = _check_ids(ids, dout)
     err_at = _err_at(err, dout)
     pad = _padding(padding_idx, V)
