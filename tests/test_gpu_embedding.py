@@ -217,6 +217,29 @@ def test_autograd_streams_and_graph(dev):
     assert torch.equal(held, embedding.embedding_backward(dy, ids, V))
 
 
+@pytest.mark.parametrize("kept", [False, True])
+def test_into_grad_of_a_lookup_on_another_stream(dev, kept):
+    """The gradient is whole on the stream that backward() was called on, also
+    where a graph made there earlier keeps the leaf's accumulator."""
+    from usaf_b200.embedding import embedding
+    table = torch.randn(1000, 256, device=dev, generator=gen(dev, 1), requires_grad=True)
+    ids = tokens(dev, 500, 1000, "uniform", 2)
+    table.grad = torch.ones_like(table)
+    earlier = (table * 2).sum() if kept else None
+    here, side = torch.cuda.current_stream(dev), torch.cuda.Stream(dev)
+    side.wait_stream(here)
+    with torch.cuda.stream(side):
+        y = embedding(ids, table, into_grad=True)
+        y.register_hook(lambda g: torch.cuda._sleep(100_000_000))      # 50 ms, in front of the node
+    here.wait_stream(side)
+    y.sum().backward()
+    got = table.grad.clone()
+    torch.cuda.synchronize()
+    want = 1.0 + torch.bincount(ids, minlength=1000).float()[:, None].expand(-1, 256)    # whole numbers: exact
+    assert torch.equal(got, want)
+    del earlier
+
+
 def test_refusals(dev):
     from usaf_b200 import embedding
     table = torch.ones(5, 8, device=dev)

@@ -109,6 +109,21 @@ def embedding_backward(dout: torch.Tensor, ids: torch.Tensor, num_embeddings: in
     return grad
 
 
+def _wait_at_the_end(grad: torch.Tensor) -> None:
+    """The stream that backward() was called on waits for this node's (the
+    lookup's): autograd does that by itself only for gradients it is given."""
+    dev = grad.get_device()
+    stream = torch.cuda.current_stream(dev)
+    grad.record_stream(stream)
+
+    def wait() -> None:
+        caller = torch.cuda.current_stream(dev)
+        if caller != stream:
+            caller.wait_stream(stream)
+
+    torch.autograd.Variable._execution_engine.queue_callback(wait)
+
+
 class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, table, scale, padding_idx, err, into_grad):
@@ -124,6 +139,7 @@ class _EmbeddingFn(torch.autograd.Function):
         held = ctx.into.grad if ctx.into is not None else None
         if held is not None and held.is_contiguous() and held.dtype in (dout.dtype, torch.float32):
             embedding_backward(dout, ids, *ctx.args, grad=held)
+            _wait_at_the_end(held)
             return None, None, None, None, None, None
         return None, embedding_backward(dout, ids, *ctx.args), None, None, None, None
 
