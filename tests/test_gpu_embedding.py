@@ -218,24 +218,30 @@ def test_autograd_streams_and_graph(dev):
 
 
 @pytest.mark.parametrize("kept", [False, True])
-def test_into_grad_of_a_lookup_on_another_stream(dev, kept):
-    """The gradient is whole on the stream that backward() was called on, also
-    where a graph made there earlier keeps the leaf's accumulator."""
+def test_into_grad_of_lookups_on_other_streams(dev, kept):
+    """The gradient is whole on the stream that backward() was called on, of two
+    lookups on streams of their own and of the table's use beside them, also where
+    an earlier graph keeps the leaf's accumulator on that stream."""
     from usaf_b200.embedding import embedding
-    table = torch.randn(1000, 256, device=dev, generator=gen(dev, 1), requires_grad=True)
-    ids = tokens(dev, 500, 1000, "uniform", 2)
+    V, H = 1000, 256
+    table = torch.randn(V, H, device=dev, generator=gen(dev, 1), requires_grad=True)
     table.grad = torch.ones_like(table)
     earlier = (table * 2).sum() if kept else None
-    here, side = torch.cuda.current_stream(dev), torch.cuda.Stream(dev)
-    side.wait_stream(here)
-    with torch.cuda.stream(side):
-        y = embedding(ids, table, into_grad=True)
-        y.register_hook(lambda g: torch.cuda._sleep(100_000_000))      # 50 ms, in front of the node
-    here.wait_stream(side)
-    y.sum().backward()
+    here = torch.cuda.current_stream(dev)
+    loss, want = (table * 3).sum(), torch.full((V, H), 4.0, device=dev)
+    for k in range(2):
+        side = torch.cuda.Stream(dev)
+        side.wait_stream(here)
+        ids = tokens(dev, 500, V, "uniform", 2 + k)
+        with torch.cuda.stream(side):
+            y = embedding(ids, table, into_grad=True)
+            y.register_hook(lambda g: torch.cuda._sleep(100_000_000))      # 50 ms, in front of the node
+        here.wait_stream(side)
+        loss = loss + y.sum()
+        want += torch.bincount(ids, minlength=V).float()[:, None]         # whole numbers: exact
+    loss.backward()
     got = table.grad.clone()
     torch.cuda.synchronize()
-    want = 1.0 + torch.bincount(ids, minlength=1000).float()[:, None].expand(-1, 256)    # whole numbers: exact
     assert torch.equal(got, want)
     del earlier
 

@@ -109,19 +109,31 @@ def embedding_backward(dout: torch.Tensor, ids: torch.Tensor, num_embeddings: in
     return grad
 
 
-def _wait_at_the_end(grad: torch.Tensor) -> None:
-    """The stream that backward() was called on waits for this node's (the
-    lookup's): autograd does that by itself only for gradients it is given."""
-    dev = grad.get_device()
+def _add_at_the_end(table: torch.Tensor, dout: torch.Tensor, ids: torch.Tensor, *args) -> None:
+    """Adds to ``table.grad`` when the backward pass is through, on the stream
+    that backward() was called on: autograd has made it wait for the leaves'
+    gradients there, and neither another lookup of the table on a stream of its
+    own nor the table's use elsewhere in the model adds at the same time."""
+    dev = dout.get_device()
     stream = torch.cuda.current_stream(dev)
-    grad.record_stream(stream)
 
-    def wait() -> None:
+    def add() -> None:
         caller = torch.cuda.current_stream(dev)
         if caller != stream:
             caller.wait_stream(stream)
+            dout.record_stream(caller)
+            ids.record_stream(caller)
+        if _can_add(table.grad, dout):
+            embedding_backward(dout, ids, *args, grad=table.grad)
+        else:
+            new = embedding_backward(dout, ids, *args)
+            table.grad = new if table.grad is None else table.grad + new
 
-    torch.autograd.Variable._execution_engine.queue_callback(wait)
+    torch.autograd.Variable._execution_engine.queue_callback(add)
+
+
+def _can_add(held: Optional[torch.Tensor], dout: torch.Tensor) -> bool:
+    return held is not None and held.is_contiguous() and held.dtype in (dout.dtype, torch.float32)
 
 
 class _EmbeddingFn(torch.autograd.Function):
@@ -136,10 +148,8 @@ class _EmbeddingFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout):
         (ids,) = ctx.saved_tensors
-        held = ctx.into.grad if ctx.into is not None else None
-        if held is not None and held.is_contiguous() and held.dtype in (dout.dtype, torch.float32):
-            embedding_backward(dout, ids, *ctx.args, grad=held)
-            _wait_at_the_end(held)
+        if ctx.into is not None and _can_add(ctx.into.grad, dout):
+            _add_at_the_end(ctx.into, dout, ids, *ctx.args)
             return None, None, None, None, None, None
         return None, embedding_backward(dout, ids, *ctx.args), None, None, None, None
 
@@ -149,9 +159,10 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, paddin
     """``scale * table[ids]`` (any shape of ``ids``), differentiable in the
     table; ``padding_idx``'s row gets no gradient.
 
-    ``into_grad``: the backward pass adds to ``table.grad``, where the table
-    (a leaf) has one, and gives autograd nothing: for loops that accumulate
-    micro-batches with ``backward()``.  Not for ``torch.autograd.grad``, which
+    ``into_grad``: the gradient is added to ``table.grad``, where the table
+    (a leaf) has one, when the backward pass is through (on the stream that
+    ``backward()`` was called on), and autograd is given nothing: for loops that
+    accumulate micro-batches with ``backward()``.  Not for ``torch.autograd.grad``, which
     would find no gradient."""
     _padding(padding_idx, table.shape[0])
     if torch.is_grad_enabled() and table.requires_grad:
