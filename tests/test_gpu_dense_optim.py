@@ -298,6 +298,17 @@ def test_captured_step(dev):
             opt.step({"w": gs[0]})
 
 
+def test_a_graph_that_saved_the_weights_notices_the_step(dev):
+    from usaf_b200 import dense_optim
+    w = torch.nn.Parameter(torch.ones(64, device=dev))
+    x = torch.ones(64, device=dev, requires_grad=True)
+    loss = (x * w).sum()
+    loss.backward(retain_graph=True)
+    dense_optim.AdamW({"w": w}).step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
 def test_refusals(dev):
     from usaf_b200 import dense_optim
     p, g = torch.ones(300, device=dev), torch.ones(300, device=dev)

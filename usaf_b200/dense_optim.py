@@ -133,6 +133,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m:
     call_on(index, "usaf_adamw", n, *[a.buffer_info()[0] for a in tab], _lib.dtype_code(dtype),
             _lib.dtype_code(g_dtype), ptr(masters), 8 if eight else 32, ptr(m), ptr(v), ptr(ms), ptr(vs),
             float(grad_div), int(step), float(lr), float(betas[0]), float(betas[1]), float(eps))
+    torch.autograd.graph.increment_version(params)      # a graph that saved them finds them changed
 
 
 class _Group:
