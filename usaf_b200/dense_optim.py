@@ -231,7 +231,7 @@ class AdamW:
                 d = p.grad if grads is None else grads.get(name)
                 if d is not None:
                     by_type.setdefault(d.dtype, []).append(
-                        (p.detach(), d.detach().contiguous(), start,
+                        (p, d if d.is_contiguous() else d.detach().contiguous(), start,
                          0.0 if name in self.no_decay else self.weight_decay))
             work += [(g, *map(list, zip(*rows))) for rows in by_type.values()]
         for g, params, ds, starts, decays in work:
