@@ -78,7 +78,9 @@ __device__ __forceinline__ float warp_max(float v) {
 // A kernel launched with launch_early may be set up while the one before it in
 // the stream still runs (once every CTA of that one has called let_next_start
 // or ended); wait_for_previous returns when the one before has ended and its
-// writes are visible, and comes before the first access to them.
+// writes are visible, and comes before the first access to them.  Such a kernel
+// takes no const __restrict__ pointers and no __ldg: both promise that the memory
+// keeps its values for the kernel's whole life, which begins before the writer's ends.
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

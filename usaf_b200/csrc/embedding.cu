@@ -41,8 +41,8 @@ constexpr int kFwdSlabs = 8;
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
-embed_fwd_kernel(const void *__restrict__ ids, int ids64, int64_t tokens, const T *__restrict__ table, int64_t V,
-                 int H, float scale, T *__restrict__ out, int32_t *__restrict__ err) {
+embed_fwd_kernel(const void *ids, int ids64, int64_t tokens, const T *table, int64_t V, int H, float scale, T *out,
+                 int32_t *err) {
     constexpr int N = kLaneN<T>, S = kFwdSlabs;
     wait_for_previous();
     const int groups = (H + 32 * N * S - 1) / (32 * N * S);
@@ -269,7 +269,7 @@ embed_sort_kernel(const SortArgs a) {
 constexpr int kFewTokens = 512;
 constexpr int64_t kFewRows = (1 << 23) - 2;
 
-__global__ void __launch_bounds__(2 * kFewTokens) embed_sort_few_kernel(const SortArgs a, uint2 *__restrict__ sorted) {
+__global__ void __launch_bounds__(2 * kFewTokens) embed_sort_few_kernel(const SortArgs a, uint2 *sorted) {
     __shared__ alignas(16) uint32_t keys[kFewTokens];
     wait_for_previous();
     let_next_start();
@@ -315,7 +315,7 @@ __device__ __forceinline__ void read_slot(const char *slot, int shift, int c0, i
 
 // the lane's sums into its columns of a row
 template <typename T, typename X, int NV, bool VEC>
-__device__ __forceinline__ void put_row(X *__restrict__ row, int c0, int lane, int H, const uint64_t *v) {
+__device__ __forceinline__ void put_row(X *row, int c0, int lane, int H, const uint64_t *v) {
     constexpr int N2 = kPairs<T>;
     if constexpr (VEC) {
 #pragma unroll
@@ -350,8 +350,8 @@ constexpr int kSlot = 512 * NV * (int)(sizeof(G) / sizeof(T)) + (VEC ? 0 : 16);
 
 template <typename T, typename G, int NV, bool VEC>
 __global__ void __launch_bounds__(256)
-embed_sum_kernel(const T *__restrict__ dy, const uint2 *__restrict__ sorted, uint32_t tokens, uint32_t V, int H,
-                 float scale, int add, G *__restrict__ grad, float *__restrict__ part) {
+embed_sum_kernel(const T *dy, const uint2 *sorted, uint32_t tokens, uint32_t V, int H, float scale, int add, G *grad,
+                 float *part) {
     constexpr int N = kLaneN<T> * NV, N2 = N / 2, D = kAhead<NV>, S = kSlot<T, G, NV, VEC>;
     extern __shared__ uint4 dyn[];   // [8 warps][D][S bytes]
     wait_for_previous();
@@ -452,8 +452,8 @@ embed_sum_kernel(const T *__restrict__ dy, const uint2 *__restrict__ sorted, uin
 // sums) by all 8 warps, each a contiguous part, which are then added in order.
 template <typename G>
 __global__ void __launch_bounds__(256)
-embed_join_kernel(const uint2 *__restrict__ sorted, uint32_t tokens, uint32_t V, int H, float scale, int add,
-                  G *__restrict__ grad, const float *__restrict__ part, int64_t chunks) {
+embed_join_kernel(const uint2 *sorted, uint32_t tokens, uint32_t V, int H, float scale, int add, G *grad,
+                  const float *part, int64_t chunks) {
     __shared__ float s[8][128];
     __shared__ int follow[8];
     __shared__ uint32_t token[8];

@@ -48,7 +48,7 @@ template <typename T, typename W> __device__ __forceinline__ void load_weight(co
     constexpr int N = 2 * kPairs<T>;
     uint4 u[N * sizeof(W) / 16];
 #pragma unroll
-    for (int i = 0; i < (int)(N * sizeof(W) / 16); ++i) u[i] = __ldg(reinterpret_cast<const uint4 *>(w) + i);
+    for (int i = 0; i < (int)(N * sizeof(W) / 16); ++i) u[i] = reinterpret_cast<const uint4 *>(w)[i];
 #pragma unroll
     for (int i = 0; i < (int)(N * sizeof(W) / 16); ++i) unpack<W>(u[i], p + i * kPairs<W>);
 }
@@ -562,8 +562,7 @@ norm_bwd_any(const T *__restrict__ dy, int64_t lddy, const T *__restrict__ x, in
 // dw[c] = sum over the P partial rows: 32 columns a CTA, 32 warps over the rows
 // (a few loads each, all in flight), their sums added in warp order
 template <typename W>
-__global__ void __launch_bounds__(1024) norm_dw_kernel(const float *__restrict__ part, int P, int H,
-                                                       W *__restrict__ dw) {
+__global__ void __launch_bounds__(1024) norm_dw_kernel(const float *part, int P, int H, W *dw) {
     __shared__ float s[32][33];
     const int lane = threadIdx.x & 31, k = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     float v = 0.0f;
