@@ -10,6 +10,7 @@ import ctypes as C
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libusaf_b200.so")
 
@@ -145,6 +146,19 @@ def ptr(t):
     if not t.is_cuda:
         raise TypeError("usaf_b200 ops take CUDA tensors (no CPU fallback)")
     return t.data_ptr()
+
+
+def differentiated(*tensors) -> bool:
+    """Whether a call on these tensors (or None) goes through autograd: one of
+    them requires a gradient, or forward mode is on, which autograd refuses for
+    operators without a forward derivative where an input has a tangent."""
+    if forward_ad._current_level >= 0:
+        return True
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def stream():

@@ -20,7 +20,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import call_on, ptr
+from ._lib import call_on, differentiated, ptr
 
 MAX_WIDTH = 1 << 22
 
@@ -157,7 +157,8 @@ class _EmbeddingFn(torch.autograd.Function):
 def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, padding_idx: Optional[int] = None,
               err: Optional[torch.Tensor] = None, into_grad: bool = False) -> torch.Tensor:
     """``scale * table[ids]`` (any shape of ``ids``), differentiable in the
-    table; ``padding_idx``'s row gets no gradient.
+    table, once and backward (forward mode is refused); ``padding_idx``'s row
+    gets no gradient.
 
     ``into_grad``: the gradient is added to ``table.grad``, where the table
     (a leaf) has one, when the backward pass is through (on the stream that
@@ -165,8 +166,8 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, paddin
     accumulate micro-batches with ``backward()``.  Not for ``torch.autograd.grad``, which
     would find no gradient."""
     _padding(padding_idx, table.shape[0])
-    if torch.is_grad_enabled() and table.requires_grad:
-        if into_grad and not table.is_leaf:
+    if differentiated(table):
+        if into_grad and table.requires_grad and not table.is_leaf:
             raise ValueError("into_grad: the table must be a leaf")
         return _EmbeddingFn.apply(ids, table, scale, padding_idx, err, into_grad)
     return embedding_forward(ids, table, scale, err)

@@ -20,7 +20,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import call_on, ptr
+from ._lib import call_on, differentiated, ptr
 
 MAX_WIDTH = 32768
 
@@ -149,9 +149,9 @@ class _RmsNormFn(torch.autograd.Function):
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: Optional[torch.Tensor] = None):
     """``y``, the RMS norm of ``x`` over its last dimension; with ``residual``
     the pair ``(y, total)`` of the norm of ``x + residual`` and that sum.
-    Differentiable in ``x``, ``weight`` and ``residual``."""
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
-                                    or (residual is not None and residual.requires_grad)):
+    Differentiable in ``x``, ``weight`` and ``residual``, once and backward;
+    forward mode is refused."""
+    if differentiated(x, weight, residual):
         return _RmsNormFn.apply(x, weight, eps, residual)
     y, _, total = rms_norm_forward(x, weight, eps, residual, want_rstd=False)
     return y if residual is None else (y, total)
