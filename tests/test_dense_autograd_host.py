@@ -49,3 +49,45 @@ def test_forward_mode_is_refused(formulas, grads, leaf):
         y, total = norms.rms_norm(x, w, residual=res)
         assert torch.equal(total, x + res) and not y.requires_grad
     assert torch.equal(embedding.embedding(ids, table), table[ids])
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """CPU tensors pass for the device's; the entry points only record their names."""
+    from usaf_b200 import dense_optim, embedding
+    names = []
+    for mod in (embedding, dense_optim):
+        monkeypatch.setattr(mod, "ptr", lambda t: None if t is None else t.data_ptr())
+        monkeypatch.setattr(mod, "call_on", lambda index, name, *a: names.append(name))
+    return names
+
+
+def saved_by_a_graph(t):
+    """A loss whose backward pass reads ``t`` as it is now."""
+    x = torch.ones_like(t, requires_grad=True)
+    return (x * t).sum()
+
+
+def test_a_gradient_added_to_in_place_counts_as_changed(launches):
+    from usaf_b200 import embedding
+    grad, ids, dout = torch.zeros(5, 8), torch.tensor([1, 4]), torch.ones(2, 8)
+    loss = saved_by_a_graph(grad)
+    embedding.embedding_backward(dout, ids, 5, grad=grad)
+    assert launches == ["usaf_embedding_bwd"] and grad._version == 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    # a new gradient is nobody's yet
+    assert embedding.embedding_backward(dout, ids, 5)._version == 0
+
+
+def test_the_tables_gradient_counts_as_changed(formulas, launches):
+    """The same where the lookup adds to ``table.grad`` itself."""
+    from usaf_b200 import embedding
+    table = torch.zeros(5, 8, requires_grad=True)
+    table.grad = torch.zeros(5, 8)
+    held = table.grad
+    loss = saved_by_a_graph(held)
+    embedding.embedding_backward(torch.ones(2, 8), torch.tensor([1, 4]), 5, grad=table.grad)
+    assert table.grad is held and held._version == 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()

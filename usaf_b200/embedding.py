@@ -104,6 +104,8 @@ def embedding_backward(dout: torch.Tensor, ids: torch.Tensor, num_embeddings: in
         grad = dout.new_empty((V, H))
     n = ids.numel()
     ws = dout.new_empty(_lib.LIB.usaf_embedding_workspace_bytes(n, V, H), dtype=torch.uint8)
+    if adds:
+        torch.autograd.graph.increment_version(grad)      # a graph that saved it finds it changed
     call_on(dout.get_device(), "usaf_embedding_bwd", at, ids.data_ptr(), 8 * ids.element_size(), n, code, V, H,
             float(scale), pad, int(adds), grad.data_ptr(), g_code, ws.data_ptr(), err_at)
     return grad
