@@ -91,3 +91,19 @@ def test_the_tables_gradient_counts_as_changed(formulas, launches):
     assert table.grad is held and held._version == 1
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_states_and_masters_count_as_changed(launches, bits):
+    """The step writes them in place as it does the parameters."""
+    from usaf_b200 import dense_optim
+    p, g, master = torch.ones(300), torch.ones(300), torch.zeros(512)
+    m, v = torch.zeros(512), torch.zeros(512)
+    if bits == 8:
+        m, v = ((torch.zeros(512, dtype=torch.float8_e4m3fn), torch.zeros(2)) for _ in range(2))
+    held = [p, master, *(m if bits == 8 else (m,)), *(v if bits == 8 else (v,))]
+    loss = saved_by_a_graph(master)
+    dense_optim.adamw_step([p], [g], m, v, step=1, lr=1e-3, masters=master)
+    assert launches == ["usaf_adamw"] and [t._version for t in held] == [1] * len(held) and g._version == 0
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()

@@ -76,7 +76,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m:
     if g_dtype is not dtype and g_dtype is not torch.float32:
         raise TypeError(f"gradients: expected {dtype} or torch.float32, got {g_dtype}")
     ptr(params[0])      # on a CUDA device, and so are the others
-    index = dev.index
+    index = params[0].get_device()
     numels, at, grads_at = [], [], []
     for p, g in zip(params, grads):
         if p.dtype is not dtype or g.dtype is not g_dtype:
@@ -127,13 +127,13 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m:
         _check_flat("v", v, total, torch.float32, dev)
     if masters is not None:
         _check_flat("masters", masters, total, torch.float32, dev)
-    flat = [t.data_ptr() for t in (m, v, ms, vs, masters) if t is not None]
-    if total and len(set(flat)) < len(flat):
+    flat = [t for t in (m, v, ms, vs, masters) if t is not None]
+    if total and len({t.data_ptr() for t in flat}) < len(flat):
         raise ValueError("m, v, their scales and the masters must not share memory")
     call_on(index, "usaf_adamw", n, *[a.buffer_info()[0] for a in tab], _lib.dtype_code(dtype),
             _lib.dtype_code(g_dtype), ptr(masters), 8 if eight else 32, ptr(m), ptr(v), ptr(ms), ptr(vs),
             float(grad_div), int(step), float(lr), float(betas[0]), float(betas[1]), float(eps))
-    torch.autograd.graph.increment_version(params)      # a graph that saved them finds them changed
+    torch.autograd.graph.increment_version([*params, *flat])      # a graph that saved them finds them changed
 
 
 class _Group:
