@@ -58,6 +58,20 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m:
     rounded from.  ``weight_decay``: one value, or one for each tensor.
     ``grad_div`` divides the gradients first.  ``starts`` gives the tensors'
     places when they are not all that the buffers hold."""
+    _launch(_checked(params, grads, m, v, step, lr, betas, eps, weight_decay, masters, grad_div, starts))
+
+
+def _launch(call: Optional[tuple]) -> None:
+    if call is not None:
+        index, args, _, written = call
+        call_on(index, "usaf_adamw", *args)
+        torch.autograd.graph.increment_version(written)      # a graph that saved them finds them changed
+
+
+def _checked(params, grads, m, v, step, lr, betas, eps, weight_decay, masters, grad_div, starts) -> Optional[tuple]:
+    """The arguments of :func:`adamw_step`, refused or made ready: the device, the
+    entry point's arguments, the host arrays that they point into and the tensors
+    that the step writes (None: nothing to do)."""
     n = len(params)
     if len(grads) != n:
         raise ValueError(f"{len(grads)} gradients for {n} parameters")
@@ -71,7 +85,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m:
     if eight == isinstance(v, torch.Tensor):
         raise TypeError("m and v: both flat tensors, or both (values, scales) pairs")
     if n == 0:
-        return
+        return None
     dev, dtype, g_dtype = params[0].device, params[0].dtype, grads[0].dtype
     if g_dtype is not dtype and g_dtype is not torch.float32:
         raise TypeError(f"gradients: expected {dtype} or torch.float32, got {g_dtype}")
@@ -130,10 +144,10 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m:
     flat = [t for t in (m, v, ms, vs, masters) if t is not None]
     if total and len({t.data_ptr() for t in flat}) < len(flat):
         raise ValueError("m, v, their scales and the masters must not share memory")
-    call_on(index, "usaf_adamw", n, *[a.buffer_info()[0] for a in tab], _lib.dtype_code(dtype),
-            _lib.dtype_code(g_dtype), ptr(masters), 8 if eight else 32, ptr(m), ptr(v), ptr(ms), ptr(vs),
-            float(grad_div), int(step), float(lr), float(betas[0]), float(betas[1]), float(eps))
-    torch.autograd.graph.increment_version([*params, *flat])      # a graph that saved them finds them changed
+    return index, (n, *[a.buffer_info()[0] for a in tab], _lib.dtype_code(dtype), _lib.dtype_code(g_dtype), ptr(masters),
+                   8 if eight else 32, ptr(m), ptr(v), ptr(ms), ptr(vs), float(grad_div), int(step), float(lr),
+                   float(betas[0]), float(betas[1]), float(eps)), tab, [*params, *flat]
+
 
 
 class _Group:
@@ -220,7 +234,8 @@ class AdamW:
     def step(self, grads: Optional[Dict[str, torch.Tensor]] = None, grad_div: float = 1.0):
         """One step with ``grads`` by name (default: the parameters' ``.grad``);
         a parameter without a gradient stays as it is.  ``grad_div`` divides
-        the gradients first, as in :meth:`SparseAdam.step`."""
+        the gradients first, as in :meth:`SparseAdam.step`.  A call that is
+        refused changes nothing."""
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW.step counts its steps on the host; a captured one would repeat the same step")
         work = []
@@ -234,9 +249,11 @@ class AdamW:
                         (p, d if d.is_contiguous() else d.detach().contiguous(), start,
                          0.0 if name in self.no_decay else self.weight_decay))
             work += [(g, *map(list, zip(*rows))) for rows in by_type.values()]
-        for g, params, ds, starts, decays in work:
-            adamw_step(params, ds, g.m, g.v, step=self._step + 1, lr=self.lr, betas=self.betas, eps=self.eps,
-                       weight_decay=decays, masters=g.masters, grad_div=grad_div, starts=starts)
+        # all of them are checked before the first one moves
+        calls = [_checked(params, ds, g.m, g.v, self._step + 1, self.lr, self.betas, self.eps, decays, g.masters, grad_div,
+                          starts) for g, params, ds, starts, decays in work]
+        for call in calls:
+            _launch(call)
         self._step += 1
 
     def state(self, name: str) -> Dict[str, torch.Tensor]:
