@@ -40,3 +40,65 @@ def test_a_refused_step_changes_nothing(dev):
     fresh.step(good)
     opt.step(good)
     assert all(torch.equal(named[n], p) for n, p in want.items())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_steps_are_counted_per_parameter(dev, bits):
+    """A parameter whose gradients come late, or not always, takes the steps that
+    it would take alone: bias corrections follow its own count."""
+    from usaf_b200 import dense_optim
+    shapes = {"always": (300,), "late": (70, 8), "gaps": (513,)}
+    due = {"always": range(1, 8), "late": (5, 6, 7), "gaps": (1, 2, 5, 7)}
+    gen = torch.Generator(device=dev).manual_seed(1)
+    start = {n: torch.randn(s, device=dev, generator=gen) for n, s in shapes.items()}
+    named = {n: parameter(t.clone()) for n, t in start.items()}
+    alone = {n: parameter(t.clone()) for n, t in start.items()}
+    opt = dense_optim.AdamW(named, lr=1e-2, state_bits=bits)
+    opts = {n: dense_optim.AdamW({n: p}, lr=1e-2, state_bits=bits) for n, p in alone.items()}
+    for t in range(1, 8):
+        grads = {n: torch.randn(s, device=dev, generator=gen) for n, s in shapes.items() if t in due[n]}
+        opt.step(grads)
+        for n, g in grads.items():
+            opts[n].step({n: g})
+        assert all(torch.equal(named[n], alone[n]) for n in shapes), t
+        if t == 5:      # the first step of a parameter: lr times the gradient's sign, and the decay
+            move = (named["late"] - start["late"] * (1 - 1e-2 * 0.01)).abs()
+            assert bool((move <= 1e-2 * (1 + 2.0 ** -18)).all()) and float(move.median()) > 0.99e-2
+        if t == 6:      # counts travel with the state
+            sd = opt.state_dict()
+            assert sd["step"] == 6 and sd["steps"] == {"always": 6, "late": 2, "gaps": 3}
+            opt = dense_optim.AdamW(named, lr=1e-2, state_bits=bits)
+            opt.load_state_dict(sd)
+    # a state without counts is one whose parameters took every step
+    sd = opts["always"].state_dict()
+    del sd["steps"]
+    opts["always"].load_state_dict(sd)
+    assert opts["always"].state_dict()["steps"] == {"always": 7}
+
+
+def test_late_parameters_follow_torch(dev):
+    """Against torch.optim.AdamW in 64 bits, gradients missing now and then: the update
+    is a chain of ~24 fp32 operations on lr-sized values (24 E lr a step), the
+    weight's own roundings 3 E |p| a step."""
+    from usaf_b200 import dense_optim
+    gen = torch.Generator(device=dev).manual_seed(2)
+    start = [torch.randn(400, device=dev, generator=gen) for _ in range(3)]
+    named = {str(i): parameter(t.clone()) for i, t in enumerate(start)}
+    ref = [torch.nn.Parameter(t.double().clone()) for t in start]
+    opt = dense_optim.AdamW(named, lr=1e-2, weight_decay=0.1)
+    want = torch.optim.AdamW(ref, lr=1e-2, weight_decay=0.1)
+    steps = 30
+    for t in range(steps):
+        grads = {}
+        for i, p in enumerate(ref):
+            p.grad = None
+            if (t + 1) % (i + 1) == 0 and t >= 4 * i:
+                g = torch.randn(400, device=dev, generator=gen) * torch.exp(torch.randn(400, device=dev, generator=gen))
+                grads[str(i)], p.grad = g, g.double()
+        opt.step(grads)
+        want.step()
+    for i, p in enumerate(ref):
+        size = 1.0 + p.detach().abs() + steps * 1e-2
+        # |update| <= 10 lr (Cauchy-Schwarz: m / (1 - b1^t) over the root of v is at most that)
+        tol = steps * (24 * E * 10 * 1e-2 + 3 * E * size)
+        assert bool(((named[str(i)].double() - p.detach()).abs() <= tol).all()), i

@@ -3,8 +3,9 @@
 Beside :class:`usaf_b200.sparse_optim.SparseAdam`, which steps the selected
 coordinates of the experts: :class:`AdamW` steps whole tensors (norms,
 embedding, routers) with decoupled weight decay, all of them in one launch per
-parameter type.  :func:`adamw_step` is the step itself over tensors and state
-buffers that the caller keeps.
+parameter type (and count of steps, where some had no gradient at times).
+:func:`adamw_step` is the step itself over tensors and state buffers that the
+caller keeps.
 
 States lie in flat buffers shared by the tensors, each tensor from a multiple
 of 256 values on (:func:`state_layout`).  With 8-bit states the first moment m
@@ -201,7 +202,8 @@ class AdamW:
         unknown = self.no_decay - self._named.keys()
         if unknown:
             raise ValueError(f"no_decay: no parameter named {sorted(unknown)}")
-        self._step = 0
+        self._step = 0                              # calls of step()
+        self._steps = dict.fromkeys(self._named, 0)     # of them, those with a gradient of the parameter
         by_type: Dict[tuple, List[str]] = {}
         for name, p in self._named.items():
             if not p.is_cuda:
@@ -233,27 +235,30 @@ class AdamW:
 
     def step(self, grads: Optional[Dict[str, torch.Tensor]] = None, grad_div: float = 1.0):
         """One step with ``grads`` by name (default: the parameters' ``.grad``);
-        a parameter without a gradient stays as it is.  ``grad_div`` divides
+        a parameter without a gradient stays as it is and does not count the
+        step: bias corrections follow the steps that it took.  ``grad_div`` divides
         the gradients first, as in :meth:`SparseAdam.step`.  A call that is
         refused changes nothing."""
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW.step counts its steps on the host; a captured one would repeat the same step")
         work = []
         for g in self._groups:
-            by_type: Dict[torch.dtype, list] = {}
+            alike: Dict[tuple, list] = {}       # one launch for each type of gradient and count of steps
             for name, start in zip(g.names, g.starts):
                 p = self._named[name]
                 d = p.grad if grads is None else grads.get(name)
                 if d is not None:
-                    by_type.setdefault(d.dtype, []).append(
+                    alike.setdefault((d.dtype, self._steps[name]), []).append(
                         (p, d if d.is_contiguous() else d.detach().contiguous(), start,
-                         0.0 if name in self.no_decay else self.weight_decay))
-            work += [(g, *map(list, zip(*rows))) for rows in by_type.values()]
+                         0.0 if name in self.no_decay else self.weight_decay, name))
+            work += [(g, taken + 1, *map(list, zip(*rows))) for (_, taken), rows in alike.items()]
         # all of them are checked before the first one moves
-        calls = [_checked(params, ds, g.m, g.v, self._step + 1, self.lr, self.betas, self.eps, decays, g.masters, grad_div,
-                          starts) for g, params, ds, starts, decays in work]
+        calls = [_checked(params, ds, g.m, g.v, step, self.lr, self.betas, self.eps, decays, g.masters, grad_div,
+                          starts) for g, step, params, ds, starts, decays, _ in work]
         for call in calls:
             _launch(call)
+        for _, step, *_, names in work:
+            self._steps.update(dict.fromkeys(names, step))
         self._step += 1
 
     def state(self, name: str) -> Dict[str, torch.Tensor]:
@@ -274,7 +279,7 @@ class AdamW:
 
     def state_dict(self) -> dict:
         """CPU tensors by name; 8-bit states as their bytes and scales."""
-        out: dict = {"step": self._step, "state_bits": self.state_bits}
+        out: dict = {"step": self._step, "steps": dict(self._steps), "state_bits": self.state_bits}
         for name, p in self._named.items():
             for k, t in self._group_of[name].parts(name, p.numel()).items():
                 t = t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t
@@ -283,7 +288,7 @@ class AdamW:
 
     def load_state_dict(self, sd: dict) -> None:
         """Refuses states of another width or size (``ValueError``) before any
-        of them is taken over."""
+        of them is taken over.  Without ``steps``, every parameter took ``step``."""
         if int(sd["state_bits"]) != self.state_bits:
             raise ValueError(f"states of {sd['state_bits']} bits for an AdamW of {self.state_bits}")
         todo = []
@@ -294,9 +299,12 @@ class AdamW:
                 if new is None or new.numel() != t.numel() or new.dtype != held.dtype:
                     raise ValueError(f"{name}: no {k} of {t.numel()} {held.dtype} values in the state")
                 todo.append((held, new))
+        steps = sd.get("steps", dict.fromkeys(self._named, sd["step"]))
+        if not self._named.keys() <= steps.keys():
+            raise ValueError(f"no count of steps of {sorted(self._named.keys() - steps.keys())} in the state")
         for held, new in todo:
             held.copy_(new.reshape(-1))
-        self._step = int(sd["step"])
+        self._step, self._steps = int(sd["step"]), {n: int(steps[n]) for n in self._named}
 
     @property
     def optimizer_memory_mb(self) -> float:
