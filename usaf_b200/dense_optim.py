@@ -16,6 +16,7 @@ rounded by itself in fp32, in a fixed order.
 from __future__ import annotations
 
 from array import array
+from bisect import bisect_left
 from itertools import accumulate
 from typing import Dict, Iterable, List, Optional, Sequence, Tuple, Union
 
@@ -58,7 +59,10 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m:
     ``masters``: flat fp32 weights that the step updates and ``params`` are
     rounded from.  ``weight_decay``: one value, or one for each tensor.
     ``grad_div`` divides the gradients first.  ``starts`` gives the tensors'
-    places when they are not all that the buffers hold."""
+    places when they are not all that the buffers hold.
+
+    Parameters, states and masters that share memory are refused; gradients
+    must not lie in any of them either."""
     _launch(_checked(params, grads, m, v, step, lr, betas, eps, weight_decay, masters, grad_div, starts))
 
 
@@ -106,12 +110,12 @@ def _checked(params, grads, m, v, step, lr, betas, eps, weight_decay, masters, g
         at.append(p.data_ptr())
         grads_at.append(g.data_ptr())
     size = params[0].element_size()
+    order = sorted((a, a + k * size) for a, k in zip(at, numels) if k)
     end = 0
-    for a, k in sorted(zip(at, numels)):
-        if k:
-            if a < end:
-                raise ValueError("a parameter is listed twice, or two share memory")
-            end = a + k * size
+    for a, b in order:
+        if a < end:
+            raise ValueError("a parameter is listed twice, or two share memory")
+        end = b
     if starts is None:
         places, total = state_layout(numels)
     else:
@@ -143,8 +147,13 @@ def _checked(params, grads, m, v, step, lr, betas, eps, weight_decay, masters, g
     if masters is not None:
         _check_flat("masters", masters, total, torch.float32, dev)
     flat = [t for t in (m, v, ms, vs, masters) if t is not None]
-    if total and len({t.data_ptr() for t in flat}) < len(flat):
-        raise ValueError("m, v, their scales and the masters must not share memory")
+    if total:
+        end = 0
+        for a, b in sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in flat):
+            i = bisect_left(order, (b,))        # the parameters before it begin below the buffer's end
+            if a < end or (i and order[i - 1][1] > a):
+                raise ValueError("m, v, their scales and the masters must not share memory, nor with a parameter")
+            end = b
     return index, (n, *[a.buffer_info()[0] for a in tab], _lib.dtype_code(dtype), _lib.dtype_code(g_dtype), ptr(masters),
                    8 if eight else 32, ptr(m), ptr(v), ptr(ms), ptr(vs), float(grad_div), int(step), float(lr),
                    float(betas[0]), float(betas[1]), float(eps)), tab, [*params, *flat]
