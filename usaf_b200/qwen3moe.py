@@ -330,12 +330,25 @@ def b200_rms_norm_forward(self, hidden_states: torch.Tensor) -> torch.Tensor:
     return norms.rms_norm(hidden_states, self.weight, self.variance_epsilon)
 
 
+def _only_norms(m: torch.nn.Module) -> bool:
+    """Whether calling ``m`` does no more than :func:`b200_rms_norm_forward`: no hooks
+    (its own or all modules'), no other module in its place."""
+    return (getattr(m.forward, "__func__", None) is b200_rms_norm_forward
+            and not (m._forward_pre_hooks or m._forward_hooks or m._backward_pre_hooks or m._backward_hooks
+                     or torch.nn.modules.module._has_any_global_hook()))
+
+
 def b200_decoder_layer_forward(self, hidden_states: torch.Tensor, **kwargs) -> torch.Tensor:
     """A pre-norm decoder layer; the residual addition behind the attention is
-    part of the norm in front of the MoE block."""
+    part of the norm in front of the MoE block, unless that module has hooks or
+    is another one: it is then called with the sum (the same values)."""
     attn = self.self_attn(hidden_states=self.input_layernorm(hidden_states), **kwargs)[0]
     post = self.post_attention_layernorm
-    normed, total = norms.rms_norm(attn, post.weight, post.variance_epsilon, residual=hidden_states)
+    if _only_norms(post):
+        normed, total = norms.rms_norm(attn, post.weight, post.variance_epsilon, residual=hidden_states)
+    else:
+        total = hidden_states + attn
+        normed = post(total)
     return total + self.mlp(normed)
 
 
