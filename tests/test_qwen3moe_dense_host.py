@@ -88,3 +88,16 @@ def test_the_fused_addition_is_what_runs_otherwise(model, monkeypatch):
                         (fused.append(residual is not None), kept(x, w, eps, residual))[1])
     copy.deepcopy(model)(input_ids=IDS)
     assert fused.count(True) == 2
+
+
+def test_mixed_types_under_autocast(model):
+    """fp32 weights with 16-bit products: the attention's rows are 16-bit, the
+    residual's are not; torch's addition takes them, so the layer does."""
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        got = model(input_ids=IDS).logits
+    want = model(input_ids=IDS).logits
+    # ~20 bf16 operations in a row, 2^-8 of their sizes each
+    assert got.dtype == torch.bfloat16
+    assert float((got.float() - want).norm()) <= 20 * 2.0 ** -8 * float(want.norm())
+    got.float().square().mean().backward()
+    assert model.model.layers[0].post_attention_layernorm.weight.grad.dtype == torch.float32

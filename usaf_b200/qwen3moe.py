@@ -341,10 +341,11 @@ def _only_norms(m: torch.nn.Module) -> bool:
 def b200_decoder_layer_forward(self, hidden_states: torch.Tensor, **kwargs) -> torch.Tensor:
     """A pre-norm decoder layer; the residual addition behind the attention is
     part of the norm in front of the MoE block, unless that module has hooks or
-    is another one: it is then called with the sum (the same values)."""
+    is another one, or the two rows are of unlike types (as under autocast): it is
+    then called with the sum (the same values)."""
     attn = self.self_attn(hidden_states=self.input_layernorm(hidden_states), **kwargs)[0]
     post = self.post_attention_layernorm
-    if _only_norms(post):
+    if attn.dtype is hidden_states.dtype and _only_norms(post):
         normed, total = norms.rms_norm(attn, post.weight, post.variance_epsilon, residual=hidden_states)
     else:
         total = hidden_states + attn
