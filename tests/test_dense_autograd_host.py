@@ -107,3 +107,43 @@ def test_states_and_masters_count_as_changed(launches, bits):
     assert launches == ["usaf_adamw"] and [t._version for t in held] == [1] * len(held) and g._version == 0
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+def test_into_grad_leaves_autograd_grad_its_gradient(formulas, monkeypatch):
+    """A backward pass that does not add to the leaves' gradients gets the table's
+    as any other, and ``.grad`` stays; ``backward()`` adds."""
+    from usaf_b200 import embedding
+    added = []
+
+    def backward(dout, ids, V, scale=1.0, padding_idx=None, grad=None, err=None):
+        g = torch.zeros(V, dout.shape[-1]) if grad is None else grad
+        return g.index_add_(0, ids, dout * scale)
+
+    def add(table, dout, ids, *args):
+        added.append(1)
+        backward(dout, ids, *args, grad=table.grad)
+
+    monkeypatch.setattr(embedding, "embedding_backward", backward)
+    monkeypatch.setattr(embedding, "_add_at_the_end", add)
+    table, other = torch.randn(5, 8, requires_grad=True), torch.ones(2, 8, requires_grad=True)
+    table.grad = torch.ones(5, 8)
+    ids = torch.tensor([1, 4])
+    err = torch.zeros(1, dtype=torch.int32)
+    want = torch.zeros(5, 8).index_fill_(0, ids, 2.0)
+
+    def loss():
+        return (embedding.embedding(ids, table, 2.0, err=err, into_grad=True) * other).sum()
+
+    for inputs in (table, [other, table]):
+        got = torch.autograd.grad(loss(), inputs)
+        assert torch.equal(got[-1], want) and not added and torch.equal(table.grad, torch.ones(5, 8))
+    loss().backward(inputs=[other])
+    assert not added and torch.equal(table.grad, torch.ones(5, 8))
+    loss().backward()
+    assert added == [1] and torch.equal(table.grad, 1 + want)
+    loss().backward(inputs=[table])
+    assert added == [1, 1] and torch.equal(table.grad, 1 + 2 * want)
+    # a second derivative's pass inside another
+    g, = torch.autograd.grad(loss(), table)
+    (loss() + g.detach().sum()).backward()
+    assert torch.equal(table.grad, 1 + 3 * want)

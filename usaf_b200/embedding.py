@@ -138,6 +138,16 @@ def _can_add(held: Optional[torch.Tensor], dout: torch.Tensor) -> bool:
     return held is not None and held.is_contiguous() and held.dtype in (dout.dtype, torch.float32)
 
 
+def _adds_to(leaf_node) -> bool:
+    """Whether the backward pass that runs now adds to this leaf's ``.grad``;
+    ``torch.autograd.grad`` hands the gradient out instead (the engine then
+    refuses the question for a leaf)."""
+    try:
+        return torch._C._will_engine_execute_node(leaf_node)
+    except RuntimeError:
+        return False
+
+
 class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, table, scale, padding_idx, err, into_grad):
@@ -150,7 +160,8 @@ class _EmbeddingFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout):
         (ids,) = ctx.saved_tensors
-        if ctx.into is not None and _can_add(ctx.into.grad, dout):
+        # next_functions: of the tensors among the inputs, ids and the table first
+        if ctx.into is not None and _can_add(ctx.into.grad, dout) and _adds_to(ctx.next_functions[1][0]):
             _add_at_the_end(ctx.into, dout, ids, *ctx.args)
             return None, None, None, None, None, None
         return None, embedding_backward(dout, ids, *ctx.args), None, None, None, None
@@ -162,11 +173,11 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, paddin
     table, once and backward (forward mode is refused); ``padding_idx``'s row
     gets no gradient.
 
-    ``into_grad``: the gradient is added to ``table.grad``, where the table
-    (a leaf) has one, when the backward pass is through (on the stream that
-    ``backward()`` was called on), and autograd is given nothing: for loops that
-    accumulate micro-batches with ``backward()``.  Not for ``torch.autograd.grad``, which
-    would find no gradient."""
+    ``into_grad``: ``backward()`` adds the gradient to ``table.grad`` itself, where
+    the table (a leaf) has one, when the pass is through (on the stream that it
+    was called on), and autograd is given nothing, so the table's hooks do not see
+    it: for loops that accumulate micro-batches.  ``torch.autograd.grad`` gets its
+    gradient as ever."""
     _padding(padding_idx, table.shape[0])
     if differentiated(table):
         if into_grad and table.requires_grad and not table.is_leaf:
