@@ -32,3 +32,27 @@ def test_a_loss_that_asks_for_the_embeddings_gradient(dev):  # noqa: F811
     assert len(asked) == 2 and all(bool(g.any()) for g in asked)
     want = (asked[0] + asked[1]) * (held["div"] / 2)
     assert float((held["grad"] - want).norm()) <= 1e-5 * float(want.norm())
+
+
+@pytest.mark.parametrize("name", ["model.norm.weight", "model.embed_tokens.weight"])
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+def test_a_dense_gradient_that_is_not_finite_skips_the_step(dev, name, value):  # noqa: F811
+    """One value of one dense gradient, all expert gradients finite: nothing moves."""
+    m = make(dev, torch.float32)
+    tr = trainer(m)
+    p = tr.dense_params[name]
+    experts = {n: t.data.clone() for n, t in tr.masters.items()}
+    dense = {n: t.detach().clone() for n, t in tr.dense_params.items()}
+
+    def loss(mdl, ids):
+        if p.grad is not None:      # in front of the last micro-batch's backward pass
+            p.grad.view(-1)[-1] = value
+        return lm_loss(mdl, ids)
+
+    out = tr.train_step([batch(1), batch(2)], loss)
+    assert not out["finite"] and tr.dense_opt.state_dict()["step"] == 0
+    assert all(bool(torch.isfinite(g).all()) for g in tr.store.compact.values())
+    assert all(torch.equal(experts[n], t.data) for n, t in tr.masters.items())
+    assert all(torch.equal(dense[n], t) for n, t in tr.dense_params.items())
+    assert tr.train_step([batch(1), batch(2)], lm_loss)["finite"]
+    assert not any(torch.equal(dense[n], t) for n, t in tr.dense_params.items())
