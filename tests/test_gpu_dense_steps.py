@@ -102,3 +102,73 @@ def test_late_parameters_follow_torch(dev):
         # |update| <= 10 lr (Cauchy-Schwarz: m / (1 - b1^t) over the root of v is at most that)
         tol = steps * (24 * E * 10 * 1e-2 + 3 * E * size)
         assert bool(((named[str(i)].double() - p.detach()).abs() <= tol).all()), i
+
+
+def same(a, b):
+    """Equal values, NaN where the other has one."""
+    return torch.equal(torch.isnan(a), torch.isnan(b)) and torch.equal(a.nan_to_num(0.0, 1e38, -1e38), b.nan_to_num(0.0, 1e38, -1e38))
+
+
+@pytest.mark.parametrize("master", [False, True])
+@pytest.mark.parametrize("eps", [1e-8, 1e-20, 0.0])
+@pytest.mark.parametrize("size", [1e-35, 1e-26, 1e-22, 1e-18, 1e-14, 1e-10, 1e8, 1e15, 1e17])
+def test_8_bit_states_at_the_ends_of_the_range(dev, size, eps, master):
+    """Second moments down to the smallest numbers (gradients of 1e-35 have none) and
+    up to the largest, eps that does not hide the root: states as by the single
+    operations, bit for bit, and the weights too where eps is small.  Else the step's
+    quotient is within 2^-22 of itself (its reciprocal within 2^-23, a product and a
+    sum, where the residual is too small to correct them), so a step moves the weight by
+    2^-22 of its size u more or less, and two roundings of both weights are 2^-22 |p|.
+    Weights start at zero, so that small steps show."""
+    from test_gpu_dense_optim import Plain
+    from usaf_b200 import dense_optim
+    gen = torch.Generator(device=dev).manual_seed(5)
+    n, dt = 3000, torch.bfloat16 if master else torch.float32
+    p = torch.zeros(n, device=dev, dtype=dt)
+    plain = Plain(p, 8, master)
+    opt = dense_optim.AdamW({"w": parameter(p)}, lr=1e-2, eps=eps, state_bits=8, master_weights=master)
+    tol, last = torch.full((n,), 2.0 ** -148, dtype=torch.float64), torch.zeros(n, dtype=torch.float64)
+    for t in (1, 2, 3):
+        # values of one block 10 powers of e apart, some zeros; a block of zeros; the tail within a block
+        g = size * torch.randn(n, device=dev, generator=gen) * torch.exp(3 * torch.randn(n, device=dev, generator=gen))
+        g[torch.rand(n, device=dev, generator=gen) < 0.1] = 0
+        g[512:768] = 0
+        g.clamp_(-1e18, 1e18)          # v stays finite
+        opt.step({"w": g})
+        plain.step(g, t, 1e-2, 0.9, 0.999, eps, 0.01, 1.0)
+        sd = opt.state_dict()
+        got, want = (sd["master"]["w"], plain.master) if master else (p.cpu(), plain.p)
+        if eps < 1e-8:
+            assert same(got, want), t
+        else:
+            u = (want.double() - last * (1 - 1e-4)).abs()
+            tol += 2.0 ** -22 * (u + want.double().abs())
+            assert bool(((got.double() - want.double()).abs() <= tol).all()), t
+        last = want.double()
+        assert same(p.cpu(), got.to(dt))
+        for k, (q, s) in (("m", plain.m), ("v", plain.v)):
+            assert torch.equal(sd[k]["w"], q.view(torch.uint8)[:n]) and torch.equal(sd[k + "_scale"]["w"], s), (t, k)
+
+
+def test_a_second_moment_beyond_the_range(dev):
+    """A finite gradient whose square is not: that value takes no step (its root is
+    infinite), stays finite, and its moment is kept as the largest there is."""
+    from usaf_b200 import dense_optim
+    for bits in (8, 32):
+        p, g = torch.ones(2000, device=dev), torch.full((2000,), 1e-3, device=dev)
+        q = p.clone()
+        bad = g.clone()
+        bad[600] = 1e22
+        for w, first in ((p, g), (q, bad)):
+            opt = dense_optim.AdamW({"w": parameter(w)}, state_bits=bits, weight_decay=0.0, lr=1e-2)
+            opt.step({"w": first})
+            if first is bad:
+                assert float(w[600]) == 1.0
+                if bits == 8:
+                    assert 3e38 < float(opt.state("w")["v"][600]) < float("inf")
+            opt.step({"w": g})
+        assert bool(torch.isfinite(q).all())
+        keep = torch.ones(2000, dtype=torch.bool, device=dev)
+        keep[512:768] = bits == 32        # in 8 bits the block's other values have its scale
+        keep[600] = False
+        assert torch.equal(p[keep], q[keep])

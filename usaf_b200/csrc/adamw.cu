@@ -4,7 +4,8 @@
 //   p = p (1 - lr wd) - lr / (1-b1^t) * m / (sqrt(v) / sqrt(1-b2^t) + eps)
 //
 // Every product and sum is one rounded fp32 operation in this order (no fused
-// multiply-add), so a step can be reproduced bit for bit operation by operation.
+// multiply-add), so a step can be reproduced bit for bit operation by operation
+// (with 8-bit states but for the last bit of a quotient now and then, see quot2).
 // The states m, v and the masters of all tensors lie in flat buffers, each
 // tensor from a multiple of 256 values on.  States in 8 bits are m and sqrt(v)
 // as e4m3 values times one fp32 scale per 256 values (largest magnitude / 448):
@@ -29,6 +30,7 @@ constexpr int kAdamBlock = 256;      // values per scale, and the unit of the te
 // each constant twice, as the operand of an f32x2 instruction
 struct AdamwConsts {
     uint64_t b1, omb1, b2, omb2, inv_root2, eps, neg_step, gmul, one, half, neg_one, huge;
+    bool usual;                      // eps: update_block
 };
 static uint64_t twice(float v) {
     uint32_t u;
@@ -109,10 +111,17 @@ __device__ __forceinline__ uint64_t sum2(uint64_t a, uint64_t b, uint64_t one) {
 
 // Root and quotient by an approximation and one corrected step (Markstein's
 // method: the residual of the first result by a fused multiply-add, times the
-// approximate reciprocal), two at a time.  Equal to the correctly rounded ones
-// for every significand (2^24 of each of eleven exponents compared) down to a
-// radicand of 2^-125, below which the residual is too small for a number; with a
-// third of the instructions, which bound the step with 8-bit states.
+// approximate reciprocal), two at a time, with a third of the instructions of the
+// correctly rounded ones, which bound the step with 8-bit states.
+//
+// The root is the nearest value for radicands from 2^-125 on (compared for all 2^23
+// significands at an even and an odd exponent, at thirteen places of the range; below,
+// the residual is too small for a number), and of zero.  The quotient is within 1/2 + 2^-20 units in the
+// last place: the reciprocal is off by 2^-23 at most and the first quotient by
+// 1.5 * 2^-23, so what the correction leaves is their product, 2.3 * 2^-46, and only
+// quotients that lie so close to the middle of two values may become the farther
+// one (for numerators below 2^-101, whose residuals have fewer bits, within 2^-22 of the
+// quotient).  update_fast says where these are used.
 __device__ __forceinline__ float rsqrt_approx(float v) {
     float r;
     asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
@@ -141,31 +150,75 @@ __device__ __forceinline__ float warp_top(float v) {     // largest magnitude of
     return r;
 }
 
-// the step of 8 values: p, m and v are replaced, root is the new sqrt(v)
-template <bool EIGHT>
-__device__ __forceinline__ void step8(const AdamwConsts &c, float keep, uint64_t *g, uint64_t *p, uint64_t *m,
-                                      uint64_t *v, uint64_t *root) {
+// the moments of 8 values with a new gradient
+__device__ __forceinline__ void moments(const AdamwConsts &c, const uint64_t *g, uint64_t *m, uint64_t *v) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         const uint64_t gk = mul2(g[k], c.gmul);
         m[k] = sum2(mul2(m[k], c.b1), mul2(gk, c.omb1), c.one);
         v[k] = sum2(mul2(v[k], c.b2), mul2(mul2(gk, c.omb2), gk), c.one);
-        uint64_t up;
-        if (EIGHT) {
-            root[k] = root2(c, v[k]);
-            up = quot2(c, m[k], sum2(mul2(root[k], c.inv_root2), c.eps, c.one));
-        } else {
-            const float2 w = halves(v[k]), h = halves(m[k]);
-            root[k] = pair(__fsqrt_rn(w.x), __fsqrt_rn(w.y));
-            const float2 den = halves(sum2(mul2(root[k], c.inv_root2), c.eps, c.one));
-            up = pair(__fdiv_rn(h.x, den.x), __fdiv_rn(h.y, den.y));
-        }
-        p[k] = sum2(mul2(p[k], pair(keep, keep)), mul2(up, c.neg_step), c.one);
     }
 }
 
+// p with the roots of v: the step's second half
+__device__ __forceinline__ uint64_t stepped(const AdamwConsts &c, float keep, uint64_t p, uint64_t up) {
+    return sum2(mul2(p, pair(keep, keep)), mul2(up, c.neg_step), c.one);
+}
+
+// the step of 8 values with correctly rounded operations; root, where it is kept, is
+// the largest number where v is infinite (such a value takes a step of zero)
+template <bool KEPT>
+__device__ __forceinline__ void update(const AdamwConsts &c, float keep, uint64_t *p, const uint64_t *m, const uint64_t *v,
+                                       uint64_t *root) {
+    constexpr float kMost = 0x1.fffffep63f;          // sqrt of the largest fp32 value
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float2 w = halves(v[k]), h = halves(m[k]);
+        const float rx = __fsqrt_rn(w.x), ry = __fsqrt_rn(w.y);
+        const float2 den = halves(sum2(mul2(pair(rx, ry), c.inv_root2), c.eps, c.one));
+        p[k] = stepped(c, keep, p[k], pair(__fdiv_rn(h.x, den.x), __fdiv_rn(h.y, den.y)));
+        if (KEPT) root[k] = pair(rx > kMost ? kMost : rx, ry > kMost ? kMost : ry);      // NaN stays
+    }
+}
+
+__device__ __forceinline__ float top_nan(float a, float b) {     // the larger one, NaN where one is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// The fast step of a block with 8-bit states: p, the roots and the block's largest
+// root.  False where it may have changed a bit beside the quotient's last, and the
+// block has to be stepped again by update: it holds where the largest root is zero or
+// 2^-44 and above, so that one whose square is below 2^-125 becomes the lowest code
+// either way; eps is larger than 2^25 times what such a root adds to it (c.usual); no
+// v is near the range's upper end (a root of infinity comes out as NaN).
+__device__ __forceinline__ bool update_fast(const AdamwConsts &c, float keep, uint64_t *p, const uint64_t *m,
+                                            const uint64_t *v, uint64_t *root, float &top) {
+    top = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        root[k] = root2(c, v[k]);
+        p[k] = stepped(c, keep, p[k], quot2(c, m[k], sum2(mul2(root[k], c.inv_root2), c.eps, c.one)));
+        const float2 w = halves(root[k]);
+        top = top_nan(top, top_nan(w.x, w.y));
+    }
+    asm("redux.sync.max.abs.NaN.f32 %0, %1, 0xffffffff;" : "=f"(top) : "f"(top));
+    return c.usual && (top == 0.0f || (top >= 0x1p-44f && top < 0x1p63f));
+}
+// the largest number among the block's roots: NaN takes no part in its scale
+__device__ __forceinline__ float top_root(const uint64_t *root) {
+    float top = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float2 w = halves(root[k]);
+        top = fmaxf(top, fmaxf(w.x, w.y));
+    }
+    return warp_top(top);
+}
+
 // m and v of a lane's 8 values from their e4m3 codes and the block's scales, and
-// back: the scales are the warp's largest magnitudes / 448
+// back: the scales are the warp's largest magnitudes (av, of the roots) / 448
 struct Codes {
     uint2 m, v;
     float m_scale, v_scale;
@@ -182,16 +235,14 @@ __device__ __forceinline__ void decode(const Codes &q, uint64_t *m, uint64_t *v)
         v[k] = mul2(v[k], v[k]);
     }
 }
-__device__ __forceinline__ Codes encode(const AdamwConsts &c, const uint64_t *m, const uint64_t *root) {
-    float am = 0.0f, av = 0.0f;
+__device__ __forceinline__ Codes encode(const AdamwConsts &c, const uint64_t *m, const uint64_t *root, float av) {
+    float am = 0.0f;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        const float2 h = halves(m[k]), w = halves(root[k]);
+        const float2 h = halves(m[k]);
         am = fmaxf(am, fmaxf(fabsf(h.x), fabsf(h.y)));
-        av = fmaxf(av, fmaxf(w.x, w.y));
     }
     am = warp_top(am);
-    av = warp_top(av);
     const float mm = am >= 1e-30f ? __fmul_rn(__frcp_rn(am), 448.0f) : 0.0f;
     const float mv = av >= 1e-30f ? __fmul_rn(__frcp_rn(av), 448.0f) : 0.0f;
     // a root above zero (3e-23 at least, of the smallest fp32 value) becomes no
@@ -264,6 +315,46 @@ __device__ __forceinline__ void store_codes(const AdamwState &s, const Codes &q,
     }
 }
 
+// a lane's weights and new moments of a block, from memory; n < 8: the tensor ends
+// within them, and what lies behind its end takes no part and stays as it is
+template <typename P, typename G, bool EIGHT, bool MASTER>
+__device__ __forceinline__ void load_block(const AdamwConsts &c, const AdamwState &s, const P *pp, const G *gg, int64_t f,
+                                           int64_t blk, int n, bool whole, uint64_t *p, uint64_t *m, uint64_t *v) {
+    uint64_t g[4];
+    load8<G>(gg, whole, n, g);
+    if (MASTER) load8<float>(s.master + f, true, 8, p);
+    else load8<P>(pp, whole, n, p);
+    if (EIGHT) {
+        Codes q;
+        q.m = *reinterpret_cast<const uint2 *>(static_cast<uint8_t *>(s.m) + f);
+        q.v = *reinterpret_cast<const uint2 *>(static_cast<uint8_t *>(s.v) + f);
+        q.m_scale = s.m_scale[blk];
+        q.v_scale = s.v_scale[blk];
+        decode(q, m, v);
+    } else {
+        load8<float>(static_cast<float *>(s.m) + f, true, 8, m);
+        load8<float>(static_cast<float *>(s.v) + f, true, 8, v);
+    }
+    if (n < 8) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float2 x = halves(m[k]), y = halves(v[k]);
+            m[k] = pair(2 * k < n ? x.x : 0.0f, 2 * k + 1 < n ? x.y : 0.0f);
+            v[k] = pair(2 * k < n ? y.x : 0.0f, 2 * k + 1 < n ? y.y : 0.0f);
+        }
+    }
+    moments(c, g, m, v);
+}
+template <typename P, bool MASTER>
+__device__ __forceinline__ void store_weights(const AdamwState &s, P *pp, int64_t f, int n, bool whole, const uint64_t *p) {
+    store8<P>(pp, whole, n, p);
+    if (MASTER) store8<float>(s.master + f, n == 8, n, p);
+}
+
+__device__ __forceinline__ int values_left(int64_t numel, int64_t i) {      // of a lane's 8
+    return numel - i >= 8 ? 8 : numel - i > 0 ? (int)(numel - i) : 0;
+}
+
 // A warp steps a run of up to `run` blocks of 256 values one after another, 8
 // values a lane: every load of a warp is of whole sectors and a block's scales are
 // its lanes' maximum.  With 8-bit states a block takes as long to compute as its
@@ -272,7 +363,8 @@ __device__ __forceinline__ void store_codes(const AdamwState &s, const Codes &q,
 // run's 16 blocks at most lie in its lanes.
 template <int N, typename P, typename G, bool EIGHT, bool MASTER>
 __global__ void __launch_bounds__(256, 3)
-adamw_kernel(const __grid_constant__ AdamwTable<N> tab, const AdamwState s, const AdamwConsts c, const int run) {
+adamw_kernel(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ AdamwState s,
+             const __grid_constant__ AdamwConsts c, const int run) {
     extern __shared__ uint4 dyn[];
     wait_for_previous();
     const int u = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -285,31 +377,34 @@ adamw_kernel(const __grid_constant__ AdamwTable<N> tab, const AdamwState s, cons
     }
     using PM = std::conditional_t<MASTER, float, P>;     // where the exact weight is
     const int64_t rel = (int64_t)(u - tab.first[lo]) * run, numel = tab.numel[lo];
-    int64_t i = rel * kAdamBlock + lane * 8;
-    int64_t blk = tab.start[lo] + rel, f = blk * kAdamBlock + lane * 8;
-    P *pp = static_cast<P *>(tab.p[lo]) + i;
-    const G *gg = static_cast<const G *>(tab.g[lo]) + i;
+    const int64_t i = rel * kAdamBlock + lane * 8;
+    const int64_t blk = tab.start[lo] + rel, f = blk * kAdamBlock + lane * 8;
+    P *const p0 = static_cast<P *>(tab.p[lo]) + i;
+    const G *const g0 = static_cast<const G *>(tab.g[lo]) + i;
     const float keep = tab.keep[lo];
-    const bool aligned = (((uintptr_t)pp | (uintptr_t)gg) & 15) == 0;
+    const bool aligned = (((uintptr_t)p0 | (uintptr_t)g0) & 15) == 0;
     const int64_t left = (numel + kAdamBlock - 1) / kAdamBlock - rel;
     const int blocks = (int)(left < run ? left : run);
+    uint32_t again = 0;              // blocks that update_fast does not hold for: bit r, of 16 at most
     if (EIGHT && aligned && numel - rel * kAdamBlock >= (int64_t)blocks * kAdamBlock) {
         using Ring = AdamRing<PM, G>;
         Ring ring;
         ring.base = (uint32_t)__cvta_generic_to_shared(dyn + threadIdx.x);
         const PM *from;
         if constexpr (MASTER) from = s.master + f;
-        else from = pp;
+        else from = p0;
         const uint8_t *m8 = static_cast<const uint8_t *>(s.m) + f, *v8 = static_cast<const uint8_t *>(s.v) + f;
         auto fetch = [&](int stage, int r) {
             const int64_t at = (int64_t)r * kAdamBlock;
-            ring.fetch(stage, r < blocks, from + at, gg + at, m8 + at, v8 + at);
+            ring.fetch(stage, r < blocks, from + at, g0 + at, m8 + at, v8 + at);
         };
 #pragma unroll
         for (int d = 0; d < Ring::D - 1; ++d) fetch(d, d);
         float scale = 0.0f;          // lanes 0-15: of m, 16-31: of v
         if ((lane & 15) < blocks) scale = (lane < 16 ? s.m_scale : s.v_scale)[blk + (lane & 15)];
         int stage = 0;
+        P *pp = p0;
+        int64_t at = f, b = blk;
         for (int r = 0; r < blocks; ++r) {
             fetch(stage == 0 ? Ring::D - 1 : stage - 1, r + Ring::D - 1);
             Ring::wait();
@@ -319,59 +414,54 @@ adamw_kernel(const __grid_constant__ AdamwTable<N> tab, const AdamwState s, cons
             q.m_scale = __shfl_sync(0xffffffffu, scale, r);
             q.v_scale = __shfl_sync(0xffffffffu, scale, 16 + r);
             decode(q, m, v);
-            step8<true>(c, keep, g, p, m, v, root);
-            store8<P>(pp, true, 8, p);
-            if (MASTER) store8<float>(s.master + f, true, 8, p);
-            store_codes(s, encode(c, m, root), f, blk, lane);
+            moments(c, g, m, v);
+            float av;
+            if (update_fast(c, keep, p, m, v, root, av)) {
+                store_weights<P, MASTER>(s, pp, at, 8, true, p);
+                store_codes(s, encode(c, m, root, av), at, b, lane);
+            } else {
+                again |= 1u << r;
+            }
             stage = stage == Ring::D - 1 ? 0 : stage + 1;
             pp += kAdamBlock;
-            f += kAdamBlock;
-            ++blk;
+            at += kAdamBlock;
+            ++b;
         }
-        return;
-    }
-    for (int r = 0; r < blocks; ++r) {
-        const int n = numel - i >= 8 ? 8 : numel - i > 0 ? (int)(numel - i) : 0;
-        const bool whole = aligned && n == 8;
-        float *m32 = static_cast<float *>(s.m) + f, *v32 = static_cast<float *>(s.v) + f;
-        uint64_t p[4], g[4], m[4], v[4], root[4];
-        load8<G>(gg, whole, n, g);
-        if (MASTER) load8<float>(s.master + f, true, 8, p);
-        else load8<P>(pp, whole, n, p);
-        if (EIGHT) {
-            Codes q;
-            q.m = *reinterpret_cast<const uint2 *>(static_cast<uint8_t *>(s.m) + f);
-            q.v = *reinterpret_cast<const uint2 *>(static_cast<uint8_t *>(s.v) + f);
-            q.m_scale = s.m_scale[blk];
-            q.v_scale = s.v_scale[blk];
-            decode(q, m, v);
-        } else {
-            load8<float>(m32, true, 8, m);
-            load8<float>(v32, true, 8, v);
-        }
-        if (n < 8) {                 // what lies behind a tensor's end takes no part
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float2 x = halves(m[k]), y = halves(v[k]);
-                m[k] = pair(2 * k < n ? x.x : 0.0f, 2 * k + 1 < n ? x.y : 0.0f);
-                v[k] = pair(2 * k < n ? y.x : 0.0f, 2 * k + 1 < n ? y.y : 0.0f);
+    } else {
+        for (int r = 0; r < blocks; ++r) {
+            const int64_t at = (int64_t)r * kAdamBlock;
+            const int n = values_left(numel, i + at);
+            const bool whole = aligned && n == 8;
+            uint64_t p[4], m[4], v[4], root[4];
+            float av;
+            load_block<P, G, EIGHT, MASTER>(c, s, p0 + at, g0 + at, f + at, blk + r, n, whole, p, m, v);
+            if constexpr (EIGHT) {
+                if (update_fast(c, keep, p, m, v, root, av)) {
+                    store_weights<P, MASTER>(s, p0 + at, f + at, n, whole, p);
+                    store_codes(s, encode(c, m, root, av), f + at, blk + r, lane);
+                } else {
+                    again |= 1u << r;
+                }
+            } else {
+                update<false>(c, keep, p, m, v, root);
+                store_weights<P, MASTER>(s, p0 + at, f + at, n, whole, p);
+                store8<float>(static_cast<float *>(s.m) + f + at, n == 8, n, m);
+                store8<float>(static_cast<float *>(s.v) + f + at, n == 8, n, v);
             }
         }
-        step8<EIGHT>(c, keep, g, p, m, v, root);
-        store8<P>(pp, whole, n, p);
-        // the values behind a tensor's end stay as they are
-        if (MASTER) store8<float>(s.master + f, n == 8, n, p);
-        if (EIGHT) {
-            store_codes(s, encode(c, m, root), f, blk, lane);
-        } else {
-            store8<float>(m32, n == 8, n, m);
-            store8<float>(v32, n == 8, n, v);
+    }
+    if constexpr (EIGHT) {
+        for (; again; again &= again - 1) {          // rare, from the beginning: nothing of the block is stored yet
+            const int r = __ffs(again) - 1;
+            const int64_t at = (int64_t)r * kAdamBlock;
+            const int n = values_left(numel, i + at);
+            const bool whole = aligned && n == 8;
+            uint64_t p[4], m[4], v[4], root[4];
+            load_block<P, G, true, MASTER>(c, s, p0 + at, g0 + at, f + at, blk + r, n, whole, p, m, v);
+            update<true>(c, keep, p, m, v, root);
+            store_weights<P, MASTER>(s, p0 + at, f + at, n, whole, p);
+            store_codes(s, encode(c, m, root, top_root(root)), f + at, blk + r, lane);
         }
-        pp += kAdamBlock;
-        gg += kAdamBlock;
-        f += kAdamBlock;
-        i += kAdamBlock;
-        ++blk;
     }
 }
 
@@ -454,7 +544,9 @@ extern "C" int usaf_adamw(int32_t n_tensors, void *const *p, const void *const *
     c.omb1 = twice((float)(1.0 - beta1));
     c.b2 = twice((float)beta2);
     c.omb2 = twice((float)(1.0 - beta2));
-    c.inv_root2 = twice((float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step))));
+    const double inv_root2 = 1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step));
+    c.inv_root2 = twice((float)inv_root2);
+    c.usual = eps >= inv_root2 * 0x1p-37 && eps <= 0x1p60;     // a root of 2^-62.5 vanishes beside eps
     c.eps = twice((float)eps);
     c.neg_step = twice(-(float)(lr / (1.0 - std::pow(beta1, (double)step))));
     c.gmul = twice((float)(1.0 / grad_div));

@@ -11,7 +11,8 @@ States lie in flat buffers shared by the tensors, each tensor from a multiple
 of 256 values on (:func:`state_layout`).  With 8-bit states the first moment m
 and the root of the second, sqrt(v), are e4m3 values times one fp32 scale per
 256 values: 2.03 bytes a value instead of 8.  Every operation of the step is
-rounded by itself in fp32, in a fixed order.
+rounded by itself in fp32, in a fixed order; with 8-bit states the update's
+quotient may be off by one in its last place.
 """
 from __future__ import annotations
 
@@ -96,7 +97,8 @@ def _checked(params, grads, m, v, step, lr, betas, eps, weight_decay, masters, g
         raise TypeError(f"gradients: expected {dtype} or torch.float32, got {g_dtype}")
     ptr(params[0])      # on a CUDA device, and so are the others
     index = params[0].get_device()
-    numels, at, grads_at = [], [], []
+    size = params[0].element_size()
+    numels, at, grads_at, spans = [], [], [], []
     for p, g in zip(params, grads):
         if p.dtype is not dtype or g.dtype is not g_dtype:
             raise TypeError(f"tensor {len(at)}: {p.dtype} with a gradient of {g.dtype}, the first has {dtype} and "
@@ -106,13 +108,15 @@ def _checked(params, grads, m, v, step, lr, betas, eps, weight_decay, masters, g
         k = p.numel()
         if g.numel() != k or not p.is_contiguous() or not g.is_contiguous():
             raise ValueError(f"tensor {len(at)}: the parameter and a gradient of its size must be contiguous")
+        a = p.data_ptr()
         numels.append(k)
-        at.append(p.data_ptr())
+        at.append(a)
         grads_at.append(g.data_ptr())
-    size = params[0].element_size()
-    order = sorted((a, a + k * size) for a, k in zip(at, numels) if k)
+        if k:
+            spans.append((a, a + k * size))
+    spans.sort()
     end = 0
-    for a, b in order:
+    for a, b in spans:
         if a < end:
             raise ValueError("a parameter is listed twice, or two share memory")
         end = b
@@ -149,9 +153,9 @@ def _checked(params, grads, m, v, step, lr, betas, eps, weight_decay, masters, g
     flat = [t for t in (m, v, ms, vs, masters) if t is not None]
     if total:
         end = 0
-        for a, b in sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in flat):
-            i = bisect_left(order, (b,))        # the parameters before it begin below the buffer's end
-            if a < end or (i and order[i - 1][1] > a):
+        for a, b in sorted([(t.data_ptr(), t.data_ptr() + t.nbytes) for t in flat]):
+            i = bisect_left(spans, (b,))        # the parameters before it begin below the buffer's end
+            if a < end or (i and spans[i - 1][1] > a):
                 raise ValueError("m, v, their scales and the masters must not share memory, nor with a parameter")
             end = b
     return index, (n, *[a.buffer_info()[0] for a in tab], _lib.dtype_code(dtype), _lib.dtype_code(g_dtype), ptr(masters),
