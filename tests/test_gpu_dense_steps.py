@@ -172,3 +172,143 @@ def test_a_second_moment_beyond_the_range(dev):
         keep[512:768] = bits == 32        # in 8 bits the block's other values have its scale
         keep[600] = False
         assert torch.equal(p[keep], q[keep])
+
+
+# ---- 8-bit states over many steps -----------------------------------------------------
+# A value's code may only stand for a part of a step (beta2 = 0.999 moves the root of v by
+# 0.05 % at most while codes lie 6 to 12 % apart), so from the step on where the new
+# gradient's weight (1 - b) / (1 - b^t) is below 1/8, the scaled value q between two codes
+# becomes the upper one where its fraction and a number of the step and the place, spread
+# evenly over [0, 1), reach 1.
+
+def reversed16(x):
+    for a, b in ((0x5555, 1), (0x3333, 2), (0x0f0f, 4), (0x00ff, 8)):
+        x = (x & a) << b | (x >> b) & a
+    return x
+
+
+def spread_numbers(n, t, lo, hi):
+    """The numbers of a step's values, in 2^-16."""
+    i = torch.arange(n)
+    h = (i // 4) * 0x9E3779B1 & 0xffffffff
+    h = h ^ h >> 15
+    h = h ^ ((t * lo & 0xffff) | (t * hi & 0xffff) << 16)
+    half = torch.where(i % 4 < 2, h & 0xffff, h >> 16)
+    return torch.where(i % 2 == 0, half, reversed16(half))
+
+
+def pack_spread(x, least, numbers):
+    """Codes and scales, as test_gpu_dense_optim.pack but for the rounding."""
+    b = x.view(-1, BLOCK)
+    top = b.abs().amax(1, keepdim=True)
+    live = top >= 1e-30
+    q = (b * torch.where(live, (1 / top) * 448.0, 0.0)).view(-1)
+    if least:
+        q = torch.maximum(q, torch.where((b > 0) & live, 2.0 ** -9, 0.0).view(-1))
+    size = q.abs().double()
+    step = torch.exp2(torch.floor(torch.log2(size.clamp_min(2.0 ** -6))) - 3)
+    low = torch.floor(size / step)
+    code = (low + ((size / step - low) + numbers / 65536.0 >= 1)) * step
+    code = torch.copysign(code.clamp_max(448.0), q.double()).float().to(torch.float8_e4m3fn)
+    return code, torch.where(live, top * torch.tensor(1 / 448.0, dtype=torch.float32), 0.0).view(-1)
+
+
+@pytest.mark.parametrize("dt,master", [(torch.float32, False), (torch.bfloat16, True)])
+@pytest.mark.parametrize("b1", [0.9, 0.98])
+def test_codes_bit_for_bit_over_many_steps(dev, dt, master, b1):
+    """States of 24 steps, nearest codes first, then spread: bit for bit, in whole blocks
+    and in a tensor's tail, wherever the tensor lies in the buffers.  (The weights may
+    differ by the last bit of the step's quotient; the states do not depend on them.)"""
+    import test_gpu_dense_optim as plain_form
+    from usaf_b200 import dense_optim
+    gen = torch.Generator(device=dev).manual_seed(9)
+    sizes, b2 = (1, 255, 256, 5000, 8192), 0.98
+    params = [(torch.randn(n, device=dev, generator=gen)).to(dt) for n in sizes]
+    plain = [plain_form.Plain(p, 8, master) for p in params]
+    opt = dense_optim.AdamW({str(i): parameter(p) for i, p in enumerate(params)}, betas=(b1, b2), state_bits=8,
+                            master_weights=master)
+    spread = 0
+    for t in range(1, 25):
+        grads = [(1e-3 * torch.randn(n, device=dev, generator=gen)
+                  * torch.exp(2 * torch.randn(n, device=dev, generator=gen))).to(dt) for n in sizes]
+        if t == 20:
+            grads = [g * 0 for g in grads]
+        opt.step({str(i): g for i, g in enumerate(grads)})
+        sd = opt.state_dict()
+        kept = plain_form.pack
+        for i, (pl, g) in enumerate(zip(plain, grads)):
+            n = -(-sizes[i] // BLOCK) * BLOCK
+
+            def pack(x, least):
+                b, lo, hi = (b2, 0x9E37, 0xC13F) if least else (b1, 0x91E1, 0x9E37)
+                if (1 - b) / (1 - b ** t) >= 0.125:
+                    return kept(x, least)
+                return pack_spread(x, least, spread_numbers(n, t, lo, hi))
+
+            plain_form.pack = pack
+            try:
+                pl.step(g, t, 1e-4, b1, b2, 1e-8, 0.01, 1.0)
+            finally:
+                plain_form.pack = kept
+            for k, (q, s) in (("m", pl.m), ("v", pl.v)):
+                assert torch.equal(sd[k][str(i)], q.view(torch.uint8)[:sizes[i]]), (t, i, k)
+                assert torch.equal(sd[k + "_scale"][str(i)], s), (t, i, k)
+        spread += (1 - b2) / (1 - b2 ** t) < 0.125
+    assert spread == 16
+
+
+@pytest.mark.parametrize("case", ["stationary", "falls", "stops"])
+def test_the_second_moment_follows_beta2(dev, case):
+    """sqrt(v) in 8 bits beside 32 after thousands of steps with beta2 = 0.999, also where
+    the gradients of every other value of a block fall 30-fold, or stop.
+
+    The mean of the ratios is 1 within 0.15: a rounding is right in the mean, and its variance
+    (p (1 - p) s^2 with p s = x / 2000 a step's move, s <= x / 8) adds at most x s / 2000 a step
+    to the mean of x^2, which decays by x^2 / 1000: 1/16 of x^2 in equilibrium and 1/32 of x,
+    and as much again on the way down; sampling noise of 8192 values at most 60 % wide is
+    0.7 %.  The spread is sqrt(s / 2x) = 0.25 of a value in equilibrium, so 5 % to 95 % lie
+    within 0.4 of the median; on the way down it doubles at most."""
+    from usaf_b200 import dense_optim
+    n = 16384
+    gen = torch.Generator(device=dev).manual_seed(11)
+    size = torch.exp(0.7 * torch.randn(n, device=dev, generator=gen))
+    other = torch.ones(n, device=dev)
+    other[::2] = {"stationary": 1.0, "falls": 1 / 30, "stops": 0.0}[case]
+    opts = [dense_optim.AdamW({"w": parameter(torch.zeros(n, device=dev))}, lr=0.0, weight_decay=0.0, state_bits=bits)
+            for bits in (32, 8)]
+    for t in range(6000):
+        g = size * torch.randn(n, device=dev, generator=gen)
+        if t >= 2000:
+            g *= other
+        for opt in opts:
+            opt.step({"w": g})
+    want, got = (opt.state("w")["v"].sqrt() for opt in opts)
+    ratio = (got / want).double()
+    for part in (ratio[::2], ratio[1::2]):
+        assert abs(float(part.mean()) - 1) <= 0.15, float(part.mean())
+        lo, mid, hi = (float(torch.quantile(part, q)) for q in (0.05, 0.5, 0.95))
+        wide = 0.4 if case == "stationary" else 0.8
+        assert 1 - wide <= lo and hi <= 1 + wide and abs(mid - 1) <= 0.25, (lo, mid, hi)
+
+
+def test_the_first_moment_follows_beta1(dev):
+    """beta1 = 0.99 moves m by 1 % of its way a step: constant gradients are reached, and
+    where they stop (beside others of the block that go on) m goes to zero.  The mean of
+    8192 values, each within 25 % of the mean it has in equilibrium: 1 % and a half for
+    what of the start is left (0.99^800); afterwards 0.99^1500 = 3e-7 of it and
+    roundings of the lowest codes, 2^-9 of 448 of the block's largest (3e-6)."""
+    from usaf_b200 import dense_optim
+    n = 16384
+    g = torch.exp(0.5 * torch.randn(n, device=dev, generator=torch.Generator(device=dev).manual_seed(12)))
+    g[1::4] *= -1
+    opt = dense_optim.AdamW({"w": parameter(torch.zeros(n, device=dev))}, lr=0.0, betas=(0.99, 0.999), state_bits=8)
+    for _ in range(800):
+        opt.step({"w": g})
+    ratio = (opt.state("w")["m"] / g).double()
+    assert abs(float(ratio.mean()) - 1) <= 0.015 and float(ratio.min()) > 0.2, (float(ratio.mean()), float(ratio.min()))
+    half = g.clone()
+    half[::2] = 0
+    for _ in range(1500):
+        opt.step({"w": half})
+    m = opt.state("w")["m"].abs()
+    assert float(m[::2].mean()) <= 1e-5 * float(m.max()), float(m[::2].mean() / m.max())

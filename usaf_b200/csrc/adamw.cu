@@ -30,7 +30,9 @@ constexpr int kAdamBlock = 256;      // values per scale, and the unit of the te
 // each constant twice, as the operand of an f32x2 instruction
 struct AdamwConsts {
     uint64_t b1, omb1, b2, omb2, inv_root2, eps, neg_step, gmul, one, half, neg_one, huge;
-    bool usual;                      // eps: update_block
+    bool usual;                      // eps: update_fast
+    bool spread_m, spread_v;         // rounding of the codes: encode
+    uint32_t seed_m, seed_v;
 };
 static uint64_t twice(float v) {
     uint32_t u;
@@ -76,6 +78,16 @@ __device__ __forceinline__ uint32_t pack_e4m3(const uint64_t *p) {
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(halves(p[0]), __NV_SATFINITE, __NV_E4M3);
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(halves(p[1]), __NV_SATFINITE, __NV_E4M3);
     return lo | hi << 16;
+}
+// a value between two codes becomes the upper one where its fraction and a number in
+// [0, 1) reach 1: 16 bits of r for two values each, the second's in reversed order
+__device__ __forceinline__ uint32_t pack_e4m3_spread(const uint64_t *p, uint32_t r) {
+    const float2 a = halves(p[0]), b = halves(p[1]);
+    uint32_t d;
+    asm("cvt.rs.satfinite.e4m3x4.f32 %0, {%1, %2, %3, %4}, %5;"
+        : "=r"(d)
+        : "f"(b.y), "f"(b.x), "f"(a.y), "f"(a.x), "r"(r));
+    return d;
 }
 
 // 8 values of T from memory as 4 pairs, and back; one by one where the tensor is
@@ -235,7 +247,21 @@ __device__ __forceinline__ void decode(const Codes &q, uint64_t *m, uint64_t *v)
         v[k] = mul2(v[k], v[k]);
     }
 }
-__device__ __forceinline__ Codes encode(const AdamwConsts &c, const uint64_t *m, const uint64_t *root, float av) {
+//
+// Codes lie 1/16 to 1/8 of a value apart.  A step moves m by w = (1 - b) / (1 - b^t) of
+// the way to the gradient (bias-corrected), the root of v by half of that at most, so
+// while w is 1/8 or more the nearest codes follow.  Later most steps move a value by
+// less than half the distance of two codes: rounded to the nearest, a root would never
+// fall (beta2 = 0.999, half of a block's gradients 30 times smaller from some step on:
+// 11 times the 32-bit root 5000 steps later) and m would stop at a part of its way.
+// So a value then becomes the upper code as often as its place between the two asks
+// for: its fraction plus a number of the step and the value's place in the tensor,
+// where the numbers of one place's steps are evenly spread (multiples of a golden
+// ratio's or the like, mod 1, their bits exchanged by a hash of the place; in reversed
+// order the low bits of an odd number's multiples, which are even as well).  Nothing
+// is drawn at random and a step repeats bit for bit.
+__device__ __forceinline__ Codes encode(const AdamwConsts &c, const uint64_t *m, const uint64_t *root, float av,
+                                        uint32_t quad) {
     float am = 0.0f;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -256,8 +282,18 @@ __device__ __forceinline__ Codes encode(const AdamwConsts &c, const uint64_t *m,
         b[k] = pair(fmaxf(q.x, fminf(any.x, least)), fmaxf(q.y, fminf(any.y, least)));
     }
     Codes q;
-    q.m = make_uint2(pack_e4m3(a), pack_e4m3(a + 2));
-    q.v = make_uint2(pack_e4m3(b), pack_e4m3(b + 2));
+    auto place = [quad](int k) {             // quad: the place in the tensor / 4
+        const uint32_t h = (quad + k) * 0x9E3779B1u;
+        return h ^ h >> 15;
+    };
+    if (c.spread_m)
+        q.m = make_uint2(pack_e4m3_spread(a, c.seed_m ^ place(0)), pack_e4m3_spread(a + 2, c.seed_m ^ place(1)));
+    else
+        q.m = make_uint2(pack_e4m3(a), pack_e4m3(a + 2));
+    if (c.spread_v)
+        q.v = make_uint2(pack_e4m3_spread(b, c.seed_v ^ place(0)), pack_e4m3_spread(b + 2, c.seed_v ^ place(1)));
+    else
+        q.v = make_uint2(pack_e4m3(b), pack_e4m3(b + 2));
     q.m_scale = mm > 0.0f ? __fmul_rn(am, (float)(1.0 / 448.0)) : 0.0f;
     q.v_scale = mv > 0.0f ? __fmul_rn(av, (float)(1.0 / 448.0)) : 0.0f;
     return q;
@@ -382,6 +418,7 @@ adamw_kernel(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ 
     P *const p0 = static_cast<P *>(tab.p[lo]) + i;
     const G *const g0 = static_cast<const G *>(tab.g[lo]) + i;
     const float keep = tab.keep[lo];
+    const uint32_t quad = (uint32_t)(i >> 2);
     const bool aligned = (((uintptr_t)p0 | (uintptr_t)g0) & 15) == 0;
     const int64_t left = (numel + kAdamBlock - 1) / kAdamBlock - rel;
     const int blocks = (int)(left < run ? left : run);
@@ -418,7 +455,7 @@ adamw_kernel(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ 
             float av;
             if (update_fast(c, keep, p, m, v, root, av)) {
                 store_weights<P, MASTER>(s, pp, at, 8, true, p);
-                store_codes(s, encode(c, m, root, av), at, b, lane);
+                store_codes(s, encode(c, m, root, av, quad + r * (kAdamBlock / 4)), at, b, lane);
             } else {
                 again |= 1u << r;
             }
@@ -438,7 +475,7 @@ adamw_kernel(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ 
             if constexpr (EIGHT) {
                 if (update_fast(c, keep, p, m, v, root, av)) {
                     store_weights<P, MASTER>(s, p0 + at, f + at, n, whole, p);
-                    store_codes(s, encode(c, m, root, av), f + at, blk + r, lane);
+                    store_codes(s, encode(c, m, root, av, quad + r * (kAdamBlock / 4)), f + at, blk + r, lane);
                 } else {
                     again |= 1u << r;
                 }
@@ -460,7 +497,7 @@ adamw_kernel(const __grid_constant__ AdamwTable<N> tab, const __grid_constant__ 
             load_block<P, G, true, MASTER>(c, s, p0 + at, g0 + at, f + at, blk + r, n, whole, p, m, v);
             update<true>(c, keep, p, m, v, root);
             store_weights<P, MASTER>(s, p0 + at, f + at, n, whole, p);
-            store_codes(s, encode(c, m, root, top_root(root)), f + at, blk + r, lane);
+            store_codes(s, encode(c, m, root, top_root(root), quad + r * (kAdamBlock / 4)), f + at, blk + r, lane);
         }
     }
 }
@@ -547,6 +584,17 @@ extern "C" int usaf_adamw(int32_t n_tensors, void *const *p, const void *const *
     const double inv_root2 = 1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step));
     c.inv_root2 = twice((float)inv_root2);
     c.usual = eps >= inv_root2 * 0x1p-37 && eps <= 0x1p60;     // a root of 2^-62.5 vanishes beside eps
+    // codes are spread from the step on where a new gradient's weight is below 1/8
+    // (encode); the multipliers, all odd: 2^16 times 0.6180, the golden ratio's inverse, and
+    // 0.7549 and 0.5698, the inverse of the root of x^3 = x + 1 and its square
+    const auto weight = [step](double b) { return (1.0 - b) / (1.0 - std::pow(b, (double)step)); };
+    const auto seed = [step](uint32_t lo, uint32_t hi) {
+        return (((uint32_t)step * lo) & 0xffffu) | ((uint32_t)step * hi) << 16;
+    };
+    c.spread_m = weight(beta1) < 0.125;
+    c.spread_v = weight(beta2) < 0.125;
+    c.seed_m = seed(0x91E1u, 0x9E37u);
+    c.seed_v = seed(0x9E37u, 0xC13Fu);
     c.eps = twice((float)eps);
     c.neg_step = twice(-(float)(lr / (1.0 - std::pow(beta1, (double)step))));
     c.gmul = twice((float)(1.0 / grad_div));
