@@ -19,6 +19,7 @@ from __future__ import annotations
 from array import array
 from bisect import bisect_left
 from itertools import accumulate
+from operator import gt
 from typing import Dict, Iterable, List, Optional, Sequence, Tuple, Union
 
 import torch
@@ -38,12 +39,15 @@ def state_layout(numels: Iterable[int]) -> Tuple[List[int], int]:
     return places[:-1], places[-1]
 
 
-def _check_flat(name: str, t: torch.Tensor, n: int, dtype: torch.dtype, device: torch.device) -> None:
-    if t.numel() != n or t.dtype != dtype or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name}: expected {n} contiguous {dtype} values on {device}, got {t.numel()} {t.dtype} "
-                         f"on {t.device}")
-    if t.data_ptr() % 16:
+def _check_flat(name: str, t: torch.Tensor, n: int, dtype: torch.dtype, index: int) -> int:
+    """The address of a state buffer."""
+    if t.numel() != n or t.dtype is not dtype or t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f"{name}: expected {n} contiguous {dtype} values on CUDA device {index}, got {t.numel()} "
+                         f"{t.dtype} on {t.device}")
+    a = t.data_ptr()
+    if a % 16:
         raise ValueError(f"{name}: must start on a 16-byte boundary")
+    return a
 
 
 def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m: Union[torch.Tensor, Packed],
@@ -98,28 +102,19 @@ def _checked(params, grads, m, v, step, lr, betas, eps, weight_decay, masters, g
     ptr(params[0])      # on a CUDA device, and so are the others
     index = params[0].get_device()
     size = params[0].element_size()
-    numels, at, grads_at, spans = [], [], [], []
-    for p, g in zip(params, grads):
+    numels = list(map(torch.Tensor.numel, params))
+    for i, (p, g, k) in enumerate(zip(params, grads, numels)):
         if p.dtype is not dtype or g.dtype is not g_dtype:
-            raise TypeError(f"tensor {len(at)}: {p.dtype} with a gradient of {g.dtype}, the first has {dtype} and "
-                            f"{g_dtype}")
+            raise TypeError(f"tensor {i}: {p.dtype} with a gradient of {g.dtype}, the first has {dtype} and {g_dtype}")
         if p.get_device() != index or g.get_device() != index:
-            raise ValueError(f"tensor {len(at)}: expected on {dev}")
-        k = p.numel()
+            raise ValueError(f"tensor {i}: expected on {dev}")
         if g.numel() != k or not p.is_contiguous() or not g.is_contiguous():
-            raise ValueError(f"tensor {len(at)}: the parameter and a gradient of its size must be contiguous")
-        a = p.data_ptr()
-        numels.append(k)
-        at.append(a)
-        grads_at.append(g.data_ptr())
-        if k:
-            spans.append((a, a + k * size))
-    spans.sort()
-    end = 0
-    for a, b in spans:
-        if a < end:
-            raise ValueError("a parameter is listed twice, or two share memory")
-        end = b
+            raise ValueError(f"tensor {i}: the parameter and a gradient of its size must be contiguous")
+    at, grads_at = list(map(torch.Tensor.data_ptr, params)), list(map(torch.Tensor.data_ptr, grads))
+    # apart: each one has ended where the next begins (an empty one's address is 0)
+    begins, ends = sorted(at), sorted([a + k * size for a, k in zip(at, numels)])
+    if any(map(gt, ends, begins[1:])):
+        raise ValueError("a parameter is listed twice, or two share memory")
     if starts is None:
         places, total = state_layout(numels)
     else:
@@ -133,35 +128,39 @@ def _checked(params, grads, m, v, step, lr, betas, eps, weight_decay, masters, g
             end = a + -(-k // BLOCK) * BLOCK
         if len(places) != n or not 0 <= end <= total:
             raise ValueError("starts: one multiple of 256 for each tensor, within the states, none overlapping")
-    decays = [float(weight_decay)] * n if isinstance(weight_decay, (int, float)) else [float(d) for d in weight_decay]
+    decays = [float(weight_decay)] * n if isinstance(weight_decay, (int, float)) else list(map(float, weight_decay))
     if len(decays) != n:
         raise ValueError(f"{len(decays)} weight decays for {n} parameters")
     # one host array of each, read before the call returns
     tab = (array("Q", at), array("Q", grads_at), array("q", numels), array("q", places),
            array("d", decays))
-    ms = vs = None
+    f32, e4m3, blocks = torch.float32, torch.float8_e4m3fn, total // BLOCK
     if eight:
         (m, ms), (v, vs) = m, v
-        for nm, t, sc in (("m", m, ms), ("v", v, vs)):
-            _check_flat(nm, t, total, torch.float8_e4m3fn, dev)
-            _check_flat(f"{nm} scales", sc, total // BLOCK, torch.float32, dev)
+        written = [m, v, ms, vs]
+        states = [_check_flat("m", m, total, e4m3, index), _check_flat("v", v, total, e4m3, index),
+                  _check_flat("m scales", ms, blocks, f32, index), _check_flat("v scales", vs, blocks, f32, index)]
+        sizes = [total, total, 4 * blocks, 4 * blocks]
     else:
-        _check_flat("m", m, total, torch.float32, dev)
-        _check_flat("v", v, total, torch.float32, dev)
+        written = [m, v]
+        states = [_check_flat("m", m, total, f32, index), _check_flat("v", v, total, f32, index), None, None]
+        sizes = [4 * total, 4 * total]
+    held, master_at = list(zip(states, sizes)), None
     if masters is not None:
-        _check_flat("masters", masters, total, torch.float32, dev)
-    flat = [t for t in (m, v, ms, vs, masters) if t is not None]
+        written.append(masters)
+        master_at = _check_flat("masters", masters, total, f32, index)
+        held.append((master_at, 4 * total))
     if total:
+        held.sort()
         end = 0
-        for a, b in sorted([(t.data_ptr(), t.data_ptr() + t.nbytes) for t in flat]):
-            i = bisect_left(spans, (b,))        # the parameters before it begin below the buffer's end
-            if a < end or (i and spans[i - 1][1] > a):
+        for a, size in held:
+            i = bisect_left(begins, a + size)       # so many parameters begin below the buffer's end
+            if a < end or (i and ends[i - 1] > a):
                 raise ValueError("m, v, their scales and the masters must not share memory, nor with a parameter")
-            end = b
-    return index, (n, *[a.buffer_info()[0] for a in tab], _lib.dtype_code(dtype), _lib.dtype_code(g_dtype), ptr(masters),
-                   8 if eight else 32, ptr(m), ptr(v), ptr(ms), ptr(vs), float(grad_div), int(step), float(lr),
-                   float(betas[0]), float(betas[1]), float(eps)), tab, [*params, *flat]
-
+            end = a + size
+    return index, (n, *[a.buffer_info()[0] for a in tab], _lib.dtype_code(dtype), _lib.dtype_code(g_dtype), master_at,
+                   8 if eight else 32, *states, float(grad_div), int(step), float(lr), float(betas[0]), float(betas[1]),
+                   float(eps)), tab, [*params, *written]
 
 
 class _Group:
