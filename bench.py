@@ -764,7 +764,9 @@ def run_c3(n_layers: int = 2, steps: int = 5, warmup: int = 2, recompute: bool =
     additions and embedding on the device kernels (qwen3moe.use_dense_kernels);
     "train" also trains them and the gates whole (SparseTrainer's dense_names, 8-bit
     AdamW states); "torch-train" trains the same tensors on torch's operations
-    (torch.optim.AdamW).  One JSON line with the whole-model tokens/s."""
+    (torch.optim.AdamW as it is by default: bf16 weights and states without fp32 copies,
+    no check for infinities, a constant learning rate).  One JSON line with the whole-model
+    tokens/s."""
     from transformers.models.qwen3_moe.configuration_qwen3_moe import Qwen3MoeConfig
     from transformers.models.qwen3_moe.modeling_qwen3_moe import Qwen3MoeForCausalLM
     from usaf_b200 import qwen3moe

@@ -418,10 +418,15 @@ int usaf_embedding_bwd(const void *dy, const void *ids, int32_t ids_bits, int64_
  * bits 32: m, v fp32.  bits 8: m and sqrt(v) as e4m3 bytes, each group of 256
  * values times m_scale / v_scale [values / 256] (fp32; the group's largest
  * magnitude / 448, 0 for a group below 1e-30); a sqrt(v) above zero is stored
- * as the lowest code at least, an infinite one as the largest number's; the
- * quotient m / (...) is within 1/2 + 2^-20 units in its last place (2^-22 of itself
- * where |m| < 2^-101), all else rounded operations.  The values between a tensor's end and the next
- * multiple of 256 stay what they are in 32 bits and are written as zeros in 8. */
+ * as the lowest code at least, an infinite one as the largest number's.  Codes are
+ * the nearest ones while a step moves a value by about their distance, (1 - b) /
+ * (1 - b^step) >= 1/8 with b = beta1 for m and beta2 for v; then the lower or the upper
+ * neighbour, the upper as often as the value's place between them asks for, by
+ * numbers of `step` and the value's place in its tensor (nothing random: a step
+ * repeats bit for bit, and a captured one repeats its step's numbers).  The quotient
+ * m / (...) is within 1/2 + 2^-20 units in its last place (2^-22 of itself where
+ * |m| < 2^-101), all else rounded operations.  The values between a tensor's end and the
+ * next multiple of 256 stay what they are in 32 bits and are written as zeros in 8. */
 int usaf_adamw(int32_t n_tensors, void *const *p, const void *const *g, const int64_t *numel,
                const int64_t *start, const double *weight_decay, int32_t p_dtype, int32_t g_dtype,
                float *master, int32_t bits, void *m, void *v, float *m_scale, float *v_scale,

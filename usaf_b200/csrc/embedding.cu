@@ -3,8 +3,8 @@
 //
 // The gradient takes four launches, each set up while the one before runs:
 //   1. sort: one cluster of 8 CTAs sorts the (token, position) pairs by a stable
-//      radix sort (digits of up to 9 bits, so two passes for a table of up to
-//      2^18 rows);
+//      radix sort (digits of up to 9 bits, so two passes for a table of fewer than
+//      2^18 rows: the number of rows is a key of its own, of padding);
 //      zeros: on the other SMs at the same time, the table's gradient is cleared,
 //      which is where the time goes (V x H values against tokens x H);
 //   2. sum: the sorted positions are cut into chunks of 32, whatever tokens they

@@ -9,9 +9,10 @@
 // result does not depend on timing.
 //
 // HBM bounds both passes: with rows of 8192 x 2048 bf16 (and the residual) the
-// forward pass takes 24 us and the backward pass 21 us, with dw 26, where the
-// bytes take 20.8 at the measured copy rate; 262144 x 128: 25 and 32 (36) against
-// 20.8 and 31.1; 4096 x 6144: 19 and 25 (31) against 15.6 and 23.4.
+// forward pass takes 20 us and the backward pass 21 us, with dw 27, where the
+// bytes take 20.8 at the measured copy rate; 262144 x 128: 22 and 32 (36) against
+// 20.8 and 31.1; 4096 x 6144: 18 and 25 (31) against 15.6 and 23.4 (one after
+// another in a graph, over three sets of rows).
 #include "common.cuh"
 #include "f32x2.cuh"
 
@@ -617,8 +618,9 @@ static int row_grid(const RowPlan &p, int smem, int regs, int64_t rows, int most
 // more: what a row costs beside them, a sum, a root and addresses, was 150 of 229
 // instructions with 32 threads to 131 values), bytes of shared memory.
 // About 8 KB a tensor, so that several CTAs an SM load, compute and store at
-// different times; at most 64 KB in all (8000 x 2050 bf16 with a residual, in 73 KB
-// forward: 39.5 us, a CTA a row 33.7).
+// different times; at most 64 KB in all, three CTAs an SM: with few rows to a large tile
+// most warps have none, and a CTA a row is as fast (8000 x 2050 bf16 with a residual
+// forward, 41 KB: 40 us; 8000 x 2051, whose tile would take 74 KB, a CTA a row: 38).
 struct TilePlan {
     int R, per, smem;
 };

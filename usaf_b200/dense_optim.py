@@ -10,9 +10,14 @@ caller keeps.
 States lie in flat buffers shared by the tensors, each tensor from a multiple
 of 256 values on (:func:`state_layout`).  With 8-bit states the first moment m
 and the root of the second, sqrt(v), are e4m3 values times one fp32 scale per
-256 values: 2.03 bytes a value instead of 8.  Every operation of the step is
-rounded by itself in fp32, in a fixed order; with 8-bit states the update's
-quotient may be off by one in its last place.
+256 values: 2.03 bytes a value instead of 8.  Codes lie 6 to 12 % apart, more than
+a late step moves a value, so from about the tenth step on a value takes the upper
+of its two neighbouring codes as often as its place between them asks for (by
+the step's number and the value's place in its tensor, nothing random): m and v
+follow the betas in the mean, each sqrt(v) within about 25 % of its 32-bit value.
+
+Every operation of the step is rounded by itself in fp32, in a fixed order; with
+8-bit states the update's quotient may be off by one in its last place.
 """
 from __future__ import annotations
 
@@ -64,7 +69,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], m:
     ``masters``: flat fp32 weights that the step updates and ``params`` are
     rounded from.  ``weight_decay``: one value, or one for each tensor.
     ``grad_div`` divides the gradients first.  ``starts`` gives the tensors'
-    places when they are not all that the buffers hold.
+    places when they are not all that the buffers hold.  A captured call repeats
+    its step number: the bias corrections, and the roundings of 8-bit codes.
 
     Parameters, states and masters that share memory are refused; gradients
     must not lie in any of them either."""
