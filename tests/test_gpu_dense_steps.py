@@ -188,9 +188,12 @@ def reversed16(x):
 
 
 def spread_numbers(n, t, lo, hi):
-    """The numbers of a step's values, in 2^-16."""
-    i = torch.arange(n)
-    h = (i // 4) * 0x9E3779B1 & 0xffffffff
+    return numbers_at(torch.arange(n), t, lo, hi)
+
+
+def numbers_at(i, t, lo, hi):
+    """The numbers of a step's values at places i, in 2^-16."""
+    h = (i // 4) * 0x9E3779B1 & 0xffffffff      # places of up to 2^32 here: no overflow of 64 bits
     h = h ^ h >> 15
     h = h ^ ((t * lo & 0xffff) | (t * hi & 0xffff) << 16)
     half = torch.where(i % 4 < 2, h & 0xffff, h >> 16)
@@ -312,3 +315,57 @@ def test_the_first_moment_follows_beta1(dev):
         opt.step({"w": half})
     m = opt.state("w")["m"].abs()
     assert float(m[::2].mean()) <= 1e-5 * float(m.max()), float(m[::2].mean() / m.max())
+
+
+def test_long_runs_of_blocks(dev):
+    """A tensor so large that a warp steps 16 blocks one after another: as in parts of
+    which each block has a warp, also where blocks in between are at the ends of the
+    range; and the spread codes of its blocks are those of their places."""
+    import test_gpu_dense_optim as plain_form
+    from usaf_b200 import dense_optim
+    n = 256 * 480000                     # 123 M values
+    gen = torch.Generator(device=dev).manual_seed(21)
+    p = torch.empty(n, device=dev, dtype=torch.bfloat16).normal_(generator=gen)
+    g = torch.empty(n, device=dev, dtype=torch.bfloat16).normal_(0, 1e-3, generator=gen)
+    kind = torch.randint(0, 8, (n // 256, 1), device=dev, generator=gen)
+    g = (g.view(-1, 256) * torch.where(kind == 0, 1e-20, torch.where(kind == 1, 1e24, torch.where(kind == 2, 0.0, 1.0)))
+         ).to(torch.bfloat16).view(-1)
+
+    def states(k):
+        return [(torch.zeros(k, dtype=torch.float8_e4m3fn, device=dev), torch.zeros(k // 256, device=dev)) for _ in range(2)]
+
+    def bits(ms):
+        return [t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t for pair in ms for t in pair]
+
+    q, whole = p.clone(), states(n)
+    dense_optim.adamw_step([q], [g], *whole, step=1, lr=1e-2)
+    part = 256 * 12000
+    for a in range(0, n, part):
+        r, st = p[a:a + part].clone(), states(part)
+        dense_optim.adamw_step([r], [g[a:a + part]], *st, step=1, lr=1e-2)
+        assert torch.equal(q[a:a + part], r)
+        for t, w, width in zip(bits(st), bits(whole), (256, 1, 256, 1)):
+            assert torch.equal(w[a // 256 * width:(a + part) // 256 * width], t)
+    assert bool(torch.isfinite(q.float()).all())
+    # a late step: 400 blocks anywhere, operation by operation
+    before = [t.clone() for t in bits(whole)]
+    dense_optim.adamw_step([q], [g], *whole, step=1000, lr=1e-2)
+    pick = torch.randperm(n // 256, generator=torch.Generator().manual_seed(3))[:400].sort().values
+    at = (pick.view(-1, 1) * 256 + torch.arange(256)).view(-1)
+    on = at.to(dev)
+    pl = plain_form.Plain(p[on], 8, False)
+    pl.m, pl.v = ((before[i][on].cpu().view(torch.float8_e4m3fn), before[i + 1][pick.to(dev)].cpu()) for i in (0, 2))
+    kept = plain_form.pack
+    plain_form.pack = lambda x, least: pack_spread(
+        x, least, numbers_at(at, 1000, *((0x9E37, 0xC13F) if least else (0x91E1, 0x9E37))))
+    try:
+        pl.step(g[on], 1000, 1e-2, 0.9, 0.999, 1e-8, 0.0, 1.0)
+    finally:
+        plain_form.pack = kept
+    after = bits(whole)
+    # (blocks of infinite moments have scales that the plain form does not bound)
+    fine = ((kind[pick.to(dev), 0] != 1).cpu()).repeat_interleave(256)
+    assert int(fine.sum()) > 300 * 256
+    for i, (codes, scales) in ((0, pl.m), (2, pl.v)):
+        assert torch.equal(after[i][on].cpu()[fine], codes.view(torch.uint8)[fine])
+        assert torch.equal(after[i + 1][pick.to(dev)].cpu()[fine[::256]], scales[fine[::256]])
